@@ -15,6 +15,11 @@ _EXPORTS = {
     "single_gather_shared_attention": "._single_gather_shared",
     "HypergraphAttention": "._autograd",
     "QuickGELU": "._autograd",
+    "norm_rotate": "._norm_rotate",
+    "rotary_table": "._norm_rotate",
+    "gather_cache_append": "._gather_cache",
+    "gather_cache_evict": "._gather_cache",
+    "single_gather_decode": "._gather_cache",
 }
 
 __all__ = sorted(_EXPORTS)

@@ -13,7 +13,7 @@ _LIB_PATH = Path(__file__).resolve().parent / "libatt3_b200.so"
 
 OK, ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_TIMEOUT = range(6)
 
-_vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
+_vp, _i, _sz, _i64, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_int64, C.c_float
 
 # name -> (restype, argtypes); mirrors include/att3_b200.h declaration by declaration
 SIGNATURES = {
@@ -44,6 +44,13 @@ SIGNATURES = {
     "att3_launch_count": (C.c_ulonglong, [_i]),
     "att3_timing_enable": (_i, [_i]),
     "att3_timing_read": (_i, [_i, C.POINTER(C.c_double), C.POINTER(C.c_ulonglong)]),
+    "att3_norm_rotate_forward": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _vp, _i, _i64, _i64, _i, _i, _i, _f, _vp]),
+    "att3_norm_rotate_workspace_bytes": (_sz, [_i] * 2),
+    "att3_norm_rotate_backward": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _vp, _i, _i64, _i64, _i, _i, _i, _f, _vp, _sz, _vp]),
+    "att3_gather_cache_append": (_i, [_vp, _i, _i, _vp, _i, _i, _i] + [_vp] * 5 + [_i] * 3 + [_f, _vp]),
+    "att3_gather_cache_evict": (_i, [_vp] * 10 + [_i] * 6 + [_vp]),
+    "att3_sg_decode_workspace_bytes": (_sz, [_i] * 8),
+    "att3_sg_decode": (_i, [_vp] * 9 + [_i] * 6 + [_vp, _sz, _vp]),
     "att3_umma_selftest": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
     "att3_wait_selftest": (_i, [C.c_uint, _vp]),
 }
@@ -52,6 +59,10 @@ SIGNATURES = {
 class SgExt(C.Structure):
     """att3_sg_ext of include/att3_b200.h."""
     _fields_ = [("window_s", C.c_int), ("mask_words", C.c_void_p), ("layout", C.c_int), ("Y_act", C.c_void_p), ("precise", C.c_int)]
+
+
+# att3_head_rows and att3_gather_pages consist of 8-byte members: the callers pass them as arrays of 64-bit integers.
+HEAD_ROWS_WORDS, GATHER_PAGES_WORDS = 21, 5
 
 
 class Att3Error(RuntimeError):

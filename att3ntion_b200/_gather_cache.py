@@ -1,0 +1,210 @@
+"""Serving the single gather: a paged cache of the rows that later queries need, the gather of one new token over it,
+and eviction from it.  (The reference has no form for single tokens.)
+
+A pool is BF16 [pages, page_size, Hkv, D] contiguous, one each for R, S, Vr and Vs.  `page_table` int32 [B, entries]
+names the page of slots p * page_size .. of every sequence, `lengths` int32 [B] the slots in use.  Both are read on the
+device, so captured graphs follow them; an entry outside its table is never followed, and `device_status()` reports it.
+`GatherCache` keeps all of these for a batch of sequences.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _cuda_kernels as _ck
+from ._cabi import lib
+from ._norm_rotate import (_NO_STRIDES, _TYPE, _check_heads, _check_table, _descriptors, _head_rows, _on_gpu, _scale,
+                           rotary_table)
+
+_BF16 = torch.bfloat16
+_POOLS = ("R", "S", "Vr", "Vs")
+
+
+def _check_pools(who, pools):
+    pools = tuple(pools)
+    if len(pools) != 4:
+        raise RuntimeError(f"{who}: pools are the four tensors R, S, Vr, Vs, got {len(pools)}")
+    for name, p in zip(_POOLS, pools):
+        if not isinstance(p, torch.Tensor) or p.dim() != 4 or p.dtype != _BF16 or not p.is_contiguous():
+            raise RuntimeError(f"{who}: pool {name} must be a contiguous bf16 [pages,page_size,Hkv,D] tensor")
+        if p.shape != pools[0].shape or p.device != pools[0].device:
+            raise RuntimeError(f"{who}: the pools must share one shape and device")
+        if p.numel() == 0:
+            raise RuntimeError(f"{who}: pool {name} is empty")
+    return pools
+
+
+def _check_table_of_pages(who, page_table, lengths, device, name="page_table", B=None):
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.dtype != torch.int32:
+        raise RuntimeError(f"{who}: {name} must be an int32 [B,entries] tensor")
+    if page_table.shape[1] < 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise RuntimeError(f"{who}: {name} needs at least one entry a sequence, neighbours in memory")
+    if B is not None and page_table.shape[0] != B:
+        raise RuntimeError(f"{who}: {name} has {page_table.shape[0]} rows for {B} sequences")
+    if page_table.device != device:
+        raise RuntimeError(f"{who}: {name} must be on the pools' device")
+    if lengths is not None:
+        _check_ints(who, "lengths", lengths, page_table.shape[0], device)
+
+
+def _check_ints(who, name, t, B, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
+        raise RuntimeError(f"{who}: {name} must be a contiguous int32 [{B}] tensor")
+    if t.device != device:
+        raise RuntimeError(f"{who}: {name} must be on the pools' device")
+
+
+def _check_mass(who, mass, pool):
+    if mass is not None and not (isinstance(mass, torch.Tensor) and mass.dtype == torch.float32 and mass.is_contiguous()
+                                 and mass.shape == pool.shape[:3] and mass.device == pool.device):
+        raise RuntimeError(f"{who}: mass must be a contiguous FP32 {tuple(pool.shape[:3])} tensor on the pools' device")
+
+
+def _pages(page_table, pool):
+    return (C.c_int64 * 5)(page_table.data_ptr(), page_table.stride(0), page_table.shape[1], pool.shape[0], pool.shape[1])
+
+
+def _no_grad(who, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{who}: has no gradient; call it under torch.no_grad()")
+
+
+def gather_cache_append(pools, page_table, lengths, R, S, Vr, Vs, *, counts=None, Q=None, weights=None, table=None,
+                        positions=None, mass=None, eps=1e-6, interleaved=False):
+    """Stores new rows R, S, Vr, Vs [B,T,Hkv,D] (any strides; bf16, fp16 or fp32) at slots lengths[b] .. of every
+    sequence; `counts` (int32 [B]) stores only the first counts[b] of them.  `lengths` itself is left as it is.
+
+    weights (a scale [D] or None each for Q, R, S) norms and `table` rotates R and S on the way, as `norm_rotate` does,
+    at positions lengths[b] + t, or positions[b] + t if `positions` (int32 [B]) is given.  Q [B,T,Hq,D], if given, goes
+    through the same pass and is returned as bf16, all T rows of it.  mass, if given, is zeroed at the slots written.
+    No two sequences may write the same slot of a page.  A slot behind the page table's end, or on a page that the pool
+    does not have, is left out and reported by `device_status()`."""
+    who = "gather_cache_append"
+    pools = _check_pools(who, pools)
+    new = (R, S, Vr, Vs) + ((Q,) if Q is not None else ())
+    B, T, D = _check_heads(who, new, ("R", "S", "Vr", "Vs", "Q"))
+    dev = pools[0].device
+    if R.device != dev or D != pools[0].shape[3] or any(x.shape[2] != pools[0].shape[2] for x in new[:4]):
+        raise RuntimeError(f"{who}: new rows must be [B,T,{pools[0].shape[2]},{pools[0].shape[3]}] on the pools' device")
+    _check_table_of_pages(who, page_table, lengths, dev, B=B)
+    if counts is not None:
+        _check_ints(who, "counts", counts, B, dev)
+    if positions is not None:
+        _check_ints(who, "positions", positions, B, dev)
+    _check_mass(who, mass, pools[0])
+    ws = (None,) * 3 if weights is None else tuple(weights)
+    if len(ws) != 3:
+        raise RuntimeError(f"{who}: weights are three scales, of Q, R and S")
+    _no_grad(who, *new, *ws)
+    wq, wr, wsc = (_scale(w, who, f"weight {k}", D, dev) for k, w in enumerate(ws))
+    table, rows, rot = _check_table(who, table, D, dev)
+    if not float(eps) >= 0:
+        raise RuntimeError(f"{who}: eps must not be negative, got {eps}")
+    _on_gpu(who, pools[0])
+    new = [_head_rows(x) for x in new]
+    with torch.cuda.device(dev):
+        turn = rot > 0
+        desc = [(x, w, r, pool, _NO_STRIDES, None, None, None)
+                for x, w, r, pool in zip(new[:4], (wr, wsc, None, None), (turn, turn, False, False), pools)]
+        out = None
+        if Q is not None:
+            Hq = Q.shape[2]
+            out = torch.empty((B, T, Hq, D), dtype=_BF16, device=dev)
+            desc.append((new[4], wq, turn, out, (T * Hq * D, Hq * D, D), None, None, None))
+        _ck._call(lib.att3_gather_cache_append, _descriptors(desc), len(desc), _TYPE[R.dtype], _ck._ptr(table), rows, rot,
+                  int(interleaved), _ck._ptr(positions), _pages(page_table, pools[0]), lengths.data_ptr(),
+                  _ck._ptr(counts), _ck._ptr(mass), B, T, D, float(eps), _ck._stream(pools[0]))
+    return out
+
+
+def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, mass=None):
+    """The gather of one new token of every sequence over its cached rows (the token's own, appended before, among them):
+
+        Y[b,h] = sum_{j,k} softmax_{(j,k)}(Q[b,h] . R_j . S_k / sqrt(D)) Vr_j o Vs_k
+
+    Q [B,Hq,D] (cast to bf16), D in {64,128}, Hq a multiple of the pools' Hkv; returns [B,Hq,D] in Q's type.  window > 0
+    makes the last `window` slots and the first `sinks` visible, window=0 all of them.  A sequence of length 0 gives
+    zeros.  Scores are formed without rounding Q o R (what precise=True does in `single_gather_attention`).
+
+    mass (FP32 [pages,page_size,Hkv]), if given, gains every visible slot's share of the attention: the mean over the
+    key head's query heads of half the probability of the pairs that hold the slot as j plus half of those that hold it
+    as k, 1 in all for every sequence and key head.  No two sequences of a call with masses may share a page."""
+    who = "single_gather_decode"
+    pools = _check_pools(who, pools)
+    pool = pools[0]
+    if not isinstance(Q, torch.Tensor) or Q.dim() != 3 or not Q.is_floating_point():
+        raise RuntimeError(f"{who}: Q must be a [B,Hq,D] tensor")
+    B, Hq, D = Q.shape
+    Hkv = pool.shape[2]
+    if D not in (64, 128):
+        raise RuntimeError(f"{who}: D must be 64 or 128, got {D}")
+    if D != pool.shape[3]:
+        raise RuntimeError(f"{who}: Q has head dim {D}, the pools {pool.shape[3]}")
+    if Hq < 1 or Hq % Hkv:
+        raise RuntimeError(f"{who}: Hq={Hq} is not divisible by Hkv={Hkv}")
+    if Q.device != pool.device:
+        raise RuntimeError(f"{who}: Q must be on the pools' device")
+    _check_table_of_pages(who, page_table, lengths, pool.device, B=B)
+    window, sinks = int(window), int(sinks)
+    if window < 0 or sinks < 0:
+        raise RuntimeError(f"{who}: window and sinks must not be negative, got {window}, {sinks}")
+    if sinks and not window:
+        raise RuntimeError(f"{who}: sinks go with a window")
+    _check_mass(who, mass, pool)
+    _no_grad(who, Q, *pools)
+    _on_gpu(who, Q)
+    slots = page_table.shape[1] * pool.shape[1]
+    window, sinks = min(window, slots), min(sinks, slots)
+    q = Q.to(_BF16).contiguous()
+    if q.data_ptr() % 16:
+        q = q.clone()
+    with torch.cuda.device(Q.device):
+        y = torch.empty((B, Hq, D), dtype=_BF16, device=Q.device)
+        if B == 0:
+            return y.to(Q.dtype)
+        nbytes = lib.att3_sg_decode_workspace_bytes(B, Hq, Hkv, D, window, sinks, slots, int(mass is not None))
+        # scratch of this call alone: a captured graph keeps it in its own pool
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
+        _ck._call(lib.att3_sg_decode, q.data_ptr(), *(p.data_ptr() for p in pools), _ck._ptr(mass), y.data_ptr(),
+                  _pages(page_table, pool), lengths.data_ptr(), B, Hq, Hkv, D, window, sinks, ws.data_ptr(), nbytes,
+                  _ck._stream(Q))
+    return y.to(Q.dtype)
+
+
+def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recent=0, out_table=None):
+    """Trims every sequence and key head to min(lengths[b], keep) slots: the first `sinks`, the last `recent` and, between
+    them, those with the largest `mass` (equal ones: the lowest slots; NaN counts as largest).  The kept rows of all
+    pools move with their mass, in order, to slots 0 .. , in place, or to the pages of `out_table`, which must then name
+    none that a sequence of the call reads.  Slots behind the last kept one are left as they are.  Key heads of a
+    sequence may keep different slots.
+
+    Returns (kept int32 [B,Hkv,keep], the slots that stayed, -1 behind the last; new lengths int32 [B])."""
+    who = "gather_cache_evict"
+    pools = _check_pools(who, pools)
+    pool = pools[0]
+    Hkv, D = pool.shape[2:]
+    if D not in (16, 32, 64, 128):
+        raise RuntimeError(f"{who}: head dim must be 16, 32, 64 or 128, got {D}")
+    if mass is None:
+        raise RuntimeError(f"{who}: needs the mass that it goes by")
+    _check_mass(who, mass, pool)
+    _check_table_of_pages(who, page_table, lengths, pool.device)
+    B = page_table.shape[0]
+    keep, sinks, recent = int(keep), int(sinks), int(recent)
+    if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise RuntimeError(f"{who}: sinks + recent must fit in keep >= 1, got {sinks} + {recent} in {keep}")
+    slots = page_table.shape[1] * pool.shape[1]
+    if out_table is not None:
+        _check_table_of_pages(who, out_table, None, pool.device, "out_table", B)
+        if out_table.shape[1] * pool.shape[1] < min(keep, slots):
+            raise RuntimeError(f"{who}: out_table has no room for {min(keep, slots)} slots")
+    _on_gpu(who, pool)
+    with torch.cuda.device(pool.device):
+        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=pool.device)
+        left = torch.empty(B, dtype=torch.int32, device=pool.device)
+        if B:
+            _ck._call(lib.att3_gather_cache_evict, *(p.data_ptr() for p in pools), mass.data_ptr(), _pages(page_table, pool),
+                      _pages(out_table if out_table is not None else page_table, pool), lengths.data_ptr(), left.data_ptr(),
+                      kept.data_ptr(), B, Hkv, D, keep, sinks, recent, _ck._stream(pool))
+    return kept, left

@@ -1,0 +1,224 @@
+"""Head norms with the position rotation, for the operands of a gather:
+
+    y = Rot(w o x / sqrt(mean(x^2) + eps))
+
+on every head row x of Q, R and S in one pass, with the gradients of x and w.  (The reference's module neither norms
+its heads nor takes positions: att3ntion/_autograd.py:327-329 refuses them.)
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _cuda_kernels as _ck
+from ._cabi import lib
+
+_TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_NO_STRIDES = (0, 0, 0)
+_HEAD_DIMS = (16, 32, 64, 128)
+
+
+def rotary_table(length: int, dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """FP32 [length, dim]: for every position the cosines of its dim / 2 angles position * base^(-2 i / dim), then their
+    sines.  The angles are formed in 64 bits, where positions of any size keep their fraction of a turn."""
+    if length < 1 or dim < 2 or dim % 2:
+        raise ValueError(f"rotary_table: needs length >= 1 and an even dim >= 2, got {length}, {dim}")
+    freq = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim)
+    angle = torch.arange(length, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat((angle.cos(), angle.sin()), 1).float()
+
+
+def _head_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` [B,N,H,D] if the kernels can read its rows where they lie (16-byte aligned, contiguous), else a copy."""
+    step = 16 // t.element_size()
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % step == 0 for n, s in zip(t.shape[:3], t.stride()) if n > 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor):
+    # a dimension of one entry may carry any stride
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()))
+
+
+def _scale(w, who: str, name: str, D: int, device):
+    if w is None:
+        return None
+    if not isinstance(w, torch.Tensor) or w.shape != (D,) or w.dtype not in _TYPE:
+        raise RuntimeError(f"{who}: {name} must be a [{D}] tensor of bf16, fp16 or fp32")
+    if w.device != device:
+        raise RuntimeError(f"{who}: {name} must be on the inputs' device")
+    w = w.detach()
+    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+
+
+def _check_heads(who: str, xs, names):
+    """Common shape contract of [B,N,heads,D] tensors; returns (B, N, D)."""
+    x0 = xs[0]
+    for name, x in zip(names, xs):
+        if not isinstance(x, torch.Tensor) or x.dim() != 4:
+            raise RuntimeError(f"{who}: {name} must be a [B,N,heads,D] tensor")
+        if x.dtype not in _TYPE or x.dtype != x0.dtype:
+            raise RuntimeError(f"{who}: all inputs must share one type of bf16, fp16 and fp32")
+        if x.shape[:2] != x0.shape[:2] or x.shape[3] != x0.shape[3]:
+            raise RuntimeError(f"{who}: {name} is {tuple(x.shape)}, expected batch, length and head dim of {names[0]} "
+                               f"{tuple(x0.shape)}")
+        if x.device != x0.device:
+            raise RuntimeError(f"{who}: all inputs must be on one device")
+        if x.shape[2] < 1:
+            raise RuntimeError(f"{who}: {name} has no heads")
+    if x0.shape[3] not in _HEAD_DIMS:
+        raise RuntimeError(f"{who}: head dim must be 16, 32, 64 or 128, got {x0.shape[3]}")
+    return x0.shape[0], x0.shape[1], x0.shape[3]
+
+
+def _check_table(who: str, table, D: int, device):
+    """(table, rows, rot); no table rotates nothing."""
+    if table is None:
+        return None, 0, 0
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.float32 or table.shape[0] < 1:
+        raise RuntimeError(f"{who}: table must be FP32 [positions, rotated columns] with at least one position")
+    rot = table.shape[1]
+    if rot > D or rot < 8 or (rot % 16 and rot != 8):
+        raise RuntimeError(f"{who}: rotated columns must be 8 or a multiple of 16 up to the head dim {D}, got {rot}")
+    if table.device != device:
+        raise RuntimeError(f"{who}: table must be on the inputs' device")
+    if not table.is_contiguous() or table.data_ptr() % 16:
+        table = table.clone(memory_format=torch.contiguous_format)
+    return table, table.shape[0], rot
+
+
+def _check_positions(who: str, positions, B: int, N: int, device):
+    """(positions or None, bytes, batch stride, position stride)."""
+    if positions is None:
+        return None, 0, 0, 0
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"{who}: positions must be an int32 or int64 tensor")
+    if tuple(positions.shape) not in {(N,), (B, N), (1, N)}:
+        raise RuntimeError(f"{who}: positions must be [{N}] or [{B},{N}], got {tuple(positions.shape)}")
+    if positions.device != device:
+        raise RuntimeError(f"{who}: positions must be on the inputs' device")
+    p = positions.expand(B, N)
+    return positions, positions.element_size(), p.stride(0), p.stride(1)
+
+
+def _on_gpu(who: str, t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{who}: inputs must be CUDA tensors")
+
+
+def _descriptors(rows):
+    """att3_head_rows array from (x, w, rotate, y, y strides, dy, dx, dw) per tensor."""
+    words = []
+    for x, w, rotate, y, y_strides, dy, dx, dw in rows:
+        words.append(x.data_ptr() if x is not None else 0)
+        words += _strides(x) if x is not None else _NO_STRIDES
+        words += (w.data_ptr(), _TYPE[w.dtype]) if w is not None else (0, 0)
+        words.append(1 if rotate else 0)
+        words.append(y.data_ptr() if y is not None else 0)
+        words += y_strides
+        words.append(dy.data_ptr() if dy is not None else 0)
+        words += _strides(dy) if dy is not None else _NO_STRIDES
+        words.append(dx.data_ptr() if dx is not None else 0)
+        words += _strides(dx) if dx is not None else _NO_STRIDES
+        words.append(dw.data_ptr() if dw is not None else 0)
+        words.append((x if x is not None else dx).shape[2])
+    return (C.c_int64 * len(words))(*words)
+
+
+def _forward(xs, ws, table, positions, eps, interleaved, heads_first):
+    who = "norm_rotate"
+    B, N, D = _check_heads(who, xs, [f"input {k}" for k in range(len(xs))])
+    dev = xs[0].device
+    ws = [_scale(w, who, f"weight {k}", D, dev) for k, w in enumerate(ws)]
+    table, rows, rot = _check_table(who, table, D, dev)
+    positions, pos_bytes, pos_b, pos_n = _check_positions(who, positions, B, N, dev)
+    if positions is None and table is not None and N > rows:
+        raise RuntimeError(f"{who}: {N} positions and a table of {rows}")
+    if not float(eps) >= 0:
+        raise RuntimeError(f"{who}: eps must not be negative, got {eps}")
+    _on_gpu(who, xs[0])
+    xs = [_head_rows(x.detach()) for x in xs]
+    with torch.cuda.device(dev):
+        ys, desc = [], []
+        for x, w in zip(xs, ws):
+            H = x.shape[2]
+            if heads_first:
+                y = torch.empty((B, H, N, D), dtype=torch.bfloat16, device=dev)
+                strides = (H * N * D, D, N * D)
+            else:
+                y = torch.empty((B, N, H, D), dtype=torch.bfloat16, device=dev)
+                strides = (N * H * D, H * D, D)
+            ys.append(y)
+            desc.append((x, w, True, y, strides, None, None, None))
+        _ck._call(lib.att3_norm_rotate_forward, _descriptors(desc), len(xs), _TYPE[xs[0].dtype], _ck._ptr(table), rows, rot,
+                  int(interleaved), _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, float(eps), _ck._stream(xs[0]))
+    return ys
+
+
+class _NormRotateFn(Function):
+    @staticmethod
+    def forward(ctx, n, table, positions, eps, interleaved, heads_first, *tensors):
+        xs, ws = tensors[:n], tensors[n:]
+        ys = _forward(xs, ws, table, positions, eps, interleaved, heads_first)
+        ctx.save_for_backward(table, positions, *tensors)
+        ctx.n, ctx.eps, ctx.interleaved, ctx.heads_first = n, eps, interleaved, heads_first
+        return tuple(ys)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *dys):
+        table, positions, *tensors = ctx.saved_tensors
+        xs, ws = tensors[:ctx.n], tensors[ctx.n:]
+        who = "norm_rotate"
+        B, N, _, D = xs[0].shape
+        dev = xs[0].device
+        scales = [_scale(w, who, "weight", D, dev) for w in ws]
+        table, rows, rot = _check_table(who, table, D, dev)
+        positions, pos_bytes, pos_b, pos_n = _check_positions(who, positions, B, N, dev)
+        with torch.cuda.device(dev):
+            desc, dxs, dws = [], [], []
+            for x, w, dy in zip(xs, scales, dys):
+                dy = _head_rows(dy.transpose(1, 2) if ctx.heads_first else dy)
+                dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+                dw = torch.empty(D, dtype=torch.float32, device=dev) if w is not None else None
+                desc.append((_head_rows(x.detach()), w, True, None, _NO_STRIDES, dy, dx, dw))
+                dxs.append(dx)
+                dws.append(dw)
+            nbytes = lib.att3_norm_rotate_workspace_bytes(ctx.n, D)
+            # scratch of this call alone: a captured graph keeps it in its own pool
+            ws_buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            _ck._call(lib.att3_norm_rotate_backward, _descriptors(desc), ctx.n, _TYPE[xs[0].dtype], _ck._ptr(table), rows, rot,
+                      int(ctx.interleaved), _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, float(ctx.eps),
+                      ws_buf.data_ptr(), nbytes, _ck._stream(xs[0]))
+        dws = [None if w is None else dw.to(w.dtype) for w, dw in zip(ws, dws)]
+        return (None,) * 6 + (*dxs, *dws)
+
+
+def norm_rotate(xs, weights=None, table=None, positions=None, *, eps=1e-6, interleaved=False, heads_first=False):
+    """Norms and rotates the head rows of one to five tensors in one pass.
+
+    xs: [B,N,heads,D] tensors (heads may differ; any strides) of one type of bf16, fp16 and fp32, D in {16,32,64,128};
+    a single tensor is taken too.  weights: a [D] scale or None for each, or None; a tensor without a scale is not
+    normed.  table: FP32 [positions, rot], see `rotary_table`; the first `rot` columns (8 or a multiple of 16) of every
+    row are turned by its position's angles, pairing columns (d, d + rot/2), or (2d, 2d + 1) with interleaved=True; None:
+    no rotation.  positions: int32 or int64 [N] or [B,N], None for 0 .. N-1.  A position outside the table is read as
+    position 0 and reported by `device_status()`.
+
+    Returns BF16 tensors, [B,N,heads,D] contiguous, or [B,heads,N,D] with heads_first=True.  Gradients of the inputs come
+    back in their type, those of the scales are summed in FP32 in a fixed order; cotangents are taken as BF16."""
+    single = isinstance(xs, torch.Tensor)
+    xs = (xs,) if single else tuple(xs)
+    if not 1 <= len(xs) <= 5:
+        raise RuntimeError(f"norm_rotate: one to five tensors, got {len(xs)}")
+    ws = (None,) * len(xs) if weights is None else (weights,) if isinstance(weights, torch.Tensor) else tuple(weights)
+    if len(ws) != len(xs):
+        raise RuntimeError(f"norm_rotate: {len(xs)} tensors and {len(ws)} weights")
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (*xs, *ws)):
+        ys = _NormRotateFn.apply(len(xs), table, positions, eps, interleaved, heads_first, *xs, *ws)
+    else:
+        ys = tuple(_forward(xs, ws, table, positions, eps, interleaved, heads_first))
+    return ys[0] if single else ys

@@ -42,6 +42,9 @@ private:
 // the runtime (no link-time dependency on the driver library).  Returns ATT3_OK or records the error.
 int make_row_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, const char* who, int box_rows = 1,
                         int pitch_cols = 0);
+// Tensor map over a row-major BF16 matrix [rows, cols] for row gathers: a box is 64 columns of one row, laid out in
+// shared memory with the 128-byte swizzle of the operand tiles.
+int make_gather_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, const char* who);
 // The same over a [B,H,N,D] operand in either memory layout (0: [B,H,N,D] -> [B*H*N, D]; 1: [B,N,H,D] -> [B*N, H*D],
 // the head being a column offset of the box): the (x, y) a kernel passes come from sgring::RowAddr::tma.
 int make_head_tensor_map(CUtensorMap* out, const void* base, int B, int H, int N, int D, int bnhd, int box_rows,
@@ -74,5 +77,11 @@ int dense_tiles(int N, int n_valid);
 int add_planes(const float* src, int n_src, size_t plane, float* acc, cudaStream_t st);
 int plane_to_bf16(const float* src, void* out, size_t n, cudaStream_t st);
 int dense_status_read_and_clear(int* out);
+
+// ---- serving kernels ------------------------------------------------------------------------
+int* serve_status_ptr();
+int serve_status_read_and_clear(int* out);
+// Sizes of a page table and its pools; records the error.
+int check_gather_pages(const att3_gather_pages* pages, const char* who);
 
 }  // namespace att3

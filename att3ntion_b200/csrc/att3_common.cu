@@ -82,11 +82,10 @@ TimedLaunch::~TimedLaunch() {
     g_time_recs.push_back({id_, start_, stop});
 }
 
-int make_row_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, const char* who, int box_rows,
-                        int pitch_cols) {
-    using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
     static EncodeFn encode = [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult qres;
@@ -95,6 +94,25 @@ int make_row_tensor_map(CUtensorMap* out, const void* base, size_t rows, int col
             fn = nullptr;
         return reinterpret_cast<EncodeFn>(fn);
     }();
+    return encode;
+}
+
+int make_gather_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, const char* who) {
+    const EncodeFn encode = encode_fn();
+    if (!encode) return set_error(ATT3_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", who);
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
+    const cuuint32_t box[2] = {64, 1}, estr[2] = {1, 1};
+    const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
+                              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(ATT3_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (CUresult %d)", who, int(r));
+    return ATT3_OK;
+}
+
+int make_row_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, const char* who, int box_rows,
+                        int pitch_cols) {
+    const EncodeFn encode = encode_fn();
     if (!encode) return set_error(ATT3_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", who);
     if (cols <= 0 || cols > 256 || (cols * 2) % 16 != 0 || reinterpret_cast<uintptr_t>(base) % 16 != 0)
         return set_error(ATT3_ERR_INVALID, "%s: row tensor map needs 16-byte aligned rows of at most 256 BF16", who);

@@ -1,0 +1,701 @@
+// The single gather of one new token over a paged gather cache, sm_100a.
+//
+// For one query head, with E visible slots e (the first `sinks`, the last `window`, or all),
+//
+//     x_jk = sum_d q_d r_jd s_kd / sqrt(D),   p = softmax over all pairs (j, k),   y_d = sum_jk p_jk vr_jd vs_kd.
+//
+// Read as a tile product the pairs are a matrix: rows (q o R_j), columns S_k.  X = (q o R) S^T, P = exp(X - m),
+// U = P Vs are two tensor-core products of 128 x 128 tiles, and y collapses the rows, y = sum_j Vr_j o U_j.  This is
+// 4 D E^2 operations a head on 8 D E bytes a key head: bound by the tensor cores for long caches (64 and more keys a
+// head already do 256 operations a byte with 8 heads a key head), by latency for a few hundred pairs.
+//
+// Scores.  q o R is not rounded: a BF16 x BF16 product has at most 16 significant bits, so its BF16 value and the
+// BF16 residual carry it exactly, and the score is the sum of two products in FP32.  That makes 1.5 times the matrix
+// work of the rounded form; what it buys is that the softmax, the token masses and the comparison with the prompt's
+// pass do not depend on the size of the scores.  P is rounded to BF16 for the second product, as in the prompt's
+// kernels; its sums stay FP32.
+//
+// Strips.  The rows of all query heads of a key head form one list of strips, 32 keys of one head each; a CTA works
+// on tiles of eight strips, two halves of 128 rows with a tensor-memory accumulator each.  A strip is one warp's, so
+// short caches fill a tile with several heads.  A strip's maximum is the warp's: the softmax of a head is joint over
+// all its pairs, so rows far below the strip's maximum may underflow as they would in the end.
+//
+// Splits.  The unit of work is (sequence, key head, tile, 128 keys).  All units lie on one line, each CTA takes an
+// equal stretch of it (one CTA an SM), and a stretch may begin and end inside a tile's key loop: any mix of lengths
+// keeps every SM busy, and one long sequence is split over its keys.  The lengths are read on the device, so a
+// captured graph follows them.  A warp carries (y, m, l) along its strips of one head and writes them out when its
+// stretch leaves the head; decode_join_kernel brings the partials of a head together in a fixed order.
+//
+// Roles.  Warps 0-3 and 4-7: one half each -- build the two operand tiles of q o R, exponentials, collapse.  Warp 8
+// issues the products, warp 9 gathers S and Vs rows through the page table with TMA row gathers (four rows an
+// instruction) into a ring of stages.  While one half exponentiates, the other half's products run.
+#pragma once
+
+#include "att3_abi_internal.h"
+#include "serve_common.cuh"
+#include "sg_ring_common.cuh"
+
+namespace serve {
+
+using namespace sm100;
+using sgring::pipe_wait;
+using sgring::warp_arrive;
+
+constexpr int DEC_THREADS = 384;
+constexpr int DEC_STRIP = 32;              // rows of a strip
+constexpr int DEC_TILE_STRIPS = 8;
+constexpr int DEC_KEYS = 128;              // keys of a unit of work
+
+struct DecodeParams {
+    const __nv_bfloat16* Q;                // [B,Hq,D]
+    const __nv_bfloat16* R;                // pools
+    const __nv_bfloat16* Vr;
+    __nv_bfloat16* Y;                      // [B,Hq,D]
+    float* mass;                           // [pages, page_size, Hkv] or null
+    const int* lengths;
+    Pages pages;
+    int B, Hq, Hkv, G, window, sinks;
+    float c2;                              // log2(e) / sqrt(D)
+    // workspace
+    float* part;                           // [head + CTA][8 warps] records of D + 4 floats: y, m, l
+    float* rows;                           // mass: [tile + CTA][8 warps][32] row sums
+    float* row_ref;                        // mass: [tile + CTA][8 warps] the maximum they are relative to
+    float* cols;                           // mass: [unit][2 halves][128] column sums
+    float* col_ref;                        // mass: [unit][2]
+    float* lse;                            // mass: [B,Hq] log2 of the softmax sum
+    long long* unit_base;                  // [B + 1]
+    long long* tile_base;                  // [B + 1]
+    int* status;
+    CUtensorMap tmS, tmVs;                 // pools as [pages * page_size, Hkv * D], box one row of 64, 128-byte swizzle
+};
+
+// What one sequence's work looks like.
+struct Shape {
+    int n, seen, skip;                     // length, visible slots, slots between the sinks and the window
+    int per_head, strips, tiles, steps;    // strips of a head, of a key head; its tiles; key steps
+    __device__ __forceinline__ long long units(int Hkv) const { return static_cast<long long>(Hkv) * tiles * steps; }
+};
+
+template <bool MASS>
+__device__ __forceinline__ Shape shape_of(const DecodeParams& p, int b, bool tell = false) {
+    Shape s;
+    s.n = p.pages.length(p.lengths, b, p.status, tell);
+    s.seen = p.window > 0 ? min(s.n, p.window + p.sinks) : s.n;
+    s.skip = s.n - s.seen;
+    // with masses a tile keeps to one head, so that its column sums are one head's
+    s.per_head = MASS ? (s.seen + 255) / 256 * DEC_TILE_STRIPS : (s.seen + DEC_STRIP - 1) / DEC_STRIP;
+    s.strips = p.G * s.per_head;
+    s.tiles = (s.strips + DEC_TILE_STRIPS - 1) / DEC_TILE_STRIPS;
+    s.steps = (s.seen + DEC_KEYS - 1) / DEC_KEYS;
+    return s;
+}
+
+__device__ __forceinline__ int slot_of(const DecodeParams& p, const Shape& s, int e) {
+    return p.window > 0 && e >= p.sinks ? e + s.skip : e;
+}
+
+// The stretch of CTA c: [total * c / n, total * (c + 1) / n).  The last CTA whose stretch begins at or before `unit`:
+__device__ __forceinline__ int cta_of(long long unit, long long total, int n) {
+    return static_cast<int>(((unit + 1) * n - 1) / total);
+}
+
+// A CTA's way along its stretch, one tile's key range at a time; every role walks it by itself.
+template <bool MASS>
+struct Walk {
+    Shape s;
+    int b, head, tile, k0, k1;             // sequence, key head, tile, key steps [k0, k1)
+    long long left, unit, slot;            // units still to do, of the first step, partial slot
+    __device__ __forceinline__ void start(const DecodeParams& p, int b0, long long off, long long count, long long tile_base,
+                                          long long unit0) {
+        b = b0;
+        s = shape_of<MASS>(p, b);
+        const long long per = static_cast<long long>(s.tiles) * s.steps;
+        head = static_cast<int>(off / per);
+        const long long r = off - head * per;
+        tile = static_cast<int>(r / s.steps);
+        k0 = static_cast<int>(r - static_cast<long long>(tile) * s.steps);
+        left = count;
+        unit = unit0;
+        slot = tile_base + static_cast<long long>(head) * s.tiles + tile + blockIdx.x;
+        k1 = static_cast<int>(min(static_cast<long long>(s.steps), k0 + left));
+    }
+    // false when the stretch is done
+    __device__ __forceinline__ bool next(const DecodeParams& p) {
+        left -= k1 - k0;
+        unit += k1 - k0;
+        if (left <= 0) return false;
+        k0 = 0;
+        ++slot;
+        if (++tile == s.tiles) {
+            tile = 0;
+            if (++head == p.Hkv) {
+                head = 0;
+                do { ++b; if (b >= p.B) return false; s = shape_of<MASS>(p, b); } while (s.seen == 0);
+            }
+        }
+        k1 = static_cast<int>(min(static_cast<long long>(s.steps), left));
+        return true;
+    }
+    // whether a half of the tile holds any strip (with masses: any key)
+    __device__ __forceinline__ bool live(int half) const {
+        if (MASS) return tile % (s.per_head / DEC_TILE_STRIPS) * 256 + half * 128 < s.seen;
+        return tile * DEC_TILE_STRIPS + half * 4 < s.strips;
+    }
+};
+
+template <int D>
+struct DecSmem {
+    static constexpr int TILE = 128 * D * 2;                   // one [128][D] BF16 operand tile
+    static constexpr int STAGES = D == 128 ? 3 : 8;
+    static constexpr int OFF_A = 0;                            // [half][value, residual]
+    static constexpr int OFF_KV = 4 * TILE;
+    static constexpr int OFF_COL = OFF_KV + STAGES * TILE;     // mass: [half][2][128] column sums being added up
+    static constexpr int OFF_SCAN = OFF_COL + 2048;            // per warp units and tiles, start of the stretch
+    static constexpr int OFF_BARS = OFF_SCAN + 256;
+    static constexpr int BYTES = OFF_BARS + 256;
+    static_assert(BYTES <= 232448, "227 KB of shared memory");
+};
+
+enum DecBar { DB_A_FULL0 = 0, DB_A_FULL1, DB_S_FULL0, DB_S_FULL1, DB_P_FULL0, DB_P_FULL1, DB_O_DONE0, DB_O_DONE1, DB_DRAIN,
+              DB_COL0, DB_COL1,
+              DB_KV_FULL0, DB_KV_EMPTY0 = DB_KV_FULL0 + 8, DB_COUNT = DB_KV_EMPTY0 + 8 };
+
+__device__ __forceinline__ void tma_gather4(void* dst, const void* map, int x, const int (&y)[4], uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+
+template <int D, bool MASS>
+__global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_constant__ DecodeParams p) {
+    using L = DecSmem<D>;
+    constexpr int REC = D + 4, COLS = D / 32;
+    constexpr float GROW = 8.f;            // a strip's reference maximum is renewed when a score exceeds it by 2^8
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if ((smem_u32(smem) & 1023u) != 0) {   // the operand tiles' swizzle wants it; there is no room to align by hand
+        if (threadIdx.x == 0) report(p.status, 10);
+        return;
+    }
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BARS);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_BARS + DB_COUNT * 8);
+    volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* sh_ref = reinterpret_cast<float*>(tmem_slot + 2);                   // [8]
+    long long (*sh_sum)[2] = reinterpret_cast<long long (*)[2]>(smem + L::OFF_SCAN);
+    long long* sh_start = reinterpret_cast<long long*>(smem + L::OFF_SCAN) + 2 * (DEC_THREADS / 32);
+    static_assert((2 * (DEC_THREADS / 32) + 5) * 8 <= 256 && DB_COUNT * 8 + 8 + 32 <= 256, "shared bookkeeping");
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // ---- this CTA's stretch: units and tiles before every sequence, a run of sequences a thread
+    long long total;
+    {
+        const int per = (p.B + DEC_THREADS - 1) / DEC_THREADS;
+        const int lo = min(tid * per, p.B), hi = min(lo + per, p.B);
+        long long units = 0, tiles = 0;
+        for (int b = lo; b < hi; ++b) {
+            const Shape s = shape_of<MASS>(p, b, blockIdx.x == 0);
+            units += s.units(p.Hkv);
+            tiles += static_cast<long long>(p.Hkv) * s.tiles;
+        }
+        long long iu = units, it = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long yu = __shfl_up_sync(0xFFFFFFFFu, iu, o), yt = __shfl_up_sync(0xFFFFFFFFu, it, o);
+            if (lane >= o) { iu += yu; it += yt; }
+        }
+        if (lane == 31) { sh_sum[warp][0] = iu; sh_sum[warp][1] = it; }
+        if (tid == 0) {
+            mbar_init(&bars[DB_A_FULL0], 4); mbar_init(&bars[DB_A_FULL1], 4);
+            mbar_init(&bars[DB_S_FULL0], 1); mbar_init(&bars[DB_S_FULL1], 1);
+            mbar_init(&bars[DB_P_FULL0], 4); mbar_init(&bars[DB_P_FULL1], 4);
+            mbar_init(&bars[DB_O_DONE0], 1); mbar_init(&bars[DB_O_DONE1], 1);
+            mbar_init(&bars[DB_DRAIN], 1);
+            mbar_init(&bars[DB_COL0], 4); mbar_init(&bars[DB_COL1], 4);
+            for (int x = 0; x < 8; ++x) { mbar_init(&bars[DB_KV_FULL0 + x], 1); mbar_init(&bars[DB_KV_EMPTY0 + x], 1); }
+            fence_mbar_init();
+            *fail = 0;
+        }
+        if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+        __syncthreads();
+        long long bu = 0, bt = 0, tt = 0;
+        total = 0;
+        for (int w = 0; w < DEC_THREADS / 32; ++w) {
+            if (w < warp) { bu += sh_sum[w][0]; bt += sh_sum[w][1]; }
+            total += sh_sum[w][0];
+            tt += sh_sum[w][1];
+        }
+        bu += iu - units;
+        bt += it - tiles;
+        const long long begin = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
+        if (blockIdx.x == 0 && tid == 0) { p.unit_base[p.B] = total; p.tile_base[p.B] = tt; }
+        for (int b = lo; b < hi; ++b) {
+            const Shape s = shape_of<MASS>(p, b);
+            const long long u = s.units(p.Hkv);
+            if (blockIdx.x == 0) { p.unit_base[b] = bu; p.tile_base[b] = bt; }
+            if (begin < end && begin >= bu && begin < bu + u) {
+                sh_start[4] = b;
+                sh_start[0] = begin - bu;
+                sh_start[1] = end - begin;
+                sh_start[2] = bt;
+                sh_start[3] = begin;
+            }
+            bu += u;
+            bt += static_cast<long long>(p.Hkv) * s.tiles;
+        }
+        if (tid == 0 && begin >= end) sh_start[4] = -1;
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    }
+    const uint32_t tmem = *tmem_slot;
+    const bool busy = sh_start[4] >= 0;
+    Walk<MASS> w;
+    if (busy) w.start(p, static_cast<int>(sh_start[4]), sh_start[0], sh_start[1], sh_start[2], sh_start[3]);
+
+    if (warp < 8) {
+        // ================================================================== builders, exponentials, collapse
+        sgring::reg_inc<208>();
+        const int half = warp >> 2, wq = warp & 3;
+        const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
+        const uint32_t tS = tmem + lanes + half * 128, tO = tmem + lanes + 256 + half * 128;
+        uint8_t* tile_hi = smem + L::OFF_A + half * 2 * L::TILE;
+        constexpr int CH = D / 8, RPP = 32 / CH, PASSES = DEC_STRIP / RPP;      // chunks a row, rows a pass
+        const int chunk = lane % CH, sub = lane / CH;
+        int seg = 0, n = 0, cols_phase = 0;
+        bool go = busy, ok = true;
+        // what the warp carries for head `cur`: lane L the columns L, 32 + L, ... of y
+        int cur = -1;
+        float cm = -INFINITY, cl = 0.f, cy[COLS];
+        auto flush = [&]() {
+            if (cur < 0) return;
+            float* out = p.part + (static_cast<long long>(cur) + blockIdx.x) * DEC_TILE_STRIPS * REC + warp * REC;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) out[c * 32 + lane] = cy[c];
+            if (lane == 0) { out[D] = cm; out[D + 1] = cl; }
+        };
+#pragma unroll 1
+        while (go && ok) {
+            const int strip = w.tile * DEC_TILE_STRIPS + warp;
+            if (!w.live(half)) { go = w.next(p); continue; }
+            const bool live = strip < w.s.strips;
+            const int g = live ? strip / w.s.per_head : 0, j0 = live ? (strip - g * w.s.per_head) * DEC_STRIP : 0;
+            const int valid = live ? max(0, min(DEC_STRIP, w.s.seen - j0)) : 0;     // rows of the strip
+            // the lane's own row of the strip, in the pools (a row on no valid page reads row 0 and is reported)
+            int row = 0;
+            if (lane < valid) {
+                row = p.pages.row(w.b, slot_of(p, w.s, j0 + lane));
+                if (row < 0) { report(p.status, ST_PAGE); row = 0; }
+            }
+            // ---- operand tiles: value and residual of q o R
+            {
+                const size_t q_at = (static_cast<size_t>(w.b) * p.Hq + w.head * p.G + g) * D + chunk * 8;
+                const uint4 q = *reinterpret_cast<const uint4*>(p.Q + q_at);
+                constexpr int BATCH = PASSES < 8 ? PASSES : 8;
+#pragma unroll
+                for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
+                    uint4 r[BATCH];
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) {
+                        const int in = (i0 + i) * RPP + sub;
+                        const int from = __shfl_sync(0xFFFFFFFFu, row, in);
+                        r[i] = make_uint4(0, 0, 0, 0);
+                        if (in < valid)
+                            r[i] = __ldg(reinterpret_cast<const uint4*>(p.R + (static_cast<size_t>(from) * p.Hkv + w.head) * D + chunk * 8));
+                    }
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) {
+                        const int in = wq * 32 + (i0 + i) * RPP + sub;
+                        uint4 hi, lo;
+                        hi.x = mul_bf16x2(q.x, r[i].x); hi.y = mul_bf16x2(q.y, r[i].y);
+                        hi.z = mul_bf16x2(q.z, r[i].z); hi.w = mul_bf16x2(q.w, r[i].w);
+                        lo.x = sgring::mul_residual_bf16x2(q.x, r[i].x, hi.x); lo.y = sgring::mul_residual_bf16x2(q.y, r[i].y, hi.y);
+                        lo.z = sgring::mul_residual_bf16x2(q.z, r[i].z, hi.z); lo.w = sgring::mul_residual_bf16x2(q.w, r[i].w, hi.w);
+                        const uint32_t at = sw128_offset<128>(in, chunk);
+                        st_shared_v4(tile_hi + at, hi.x, hi.y, hi.z, hi.w);
+                        st_shared_v4(tile_hi + L::TILE + at, lo.x, lo.y, lo.z, lo.w);
+                    }
+                }
+            }
+            fence_async_smem();
+            warp_arrive(&bars[DB_A_FULL0 + half], lane);
+
+            // ---- key steps
+            float ref = 0.f, sum = 0.f;                    // reference maximum (scaled, base 2) of the strip; this row's sum
+#pragma unroll 1
+            for (int k = w.k0; k < w.k1; ++k, ++n) {
+                ok = pipe_wait(&bars[DB_S_FULL0 + half], n & 1, fail, 2);
+                if (!ok) break;
+                tc_fence_after();
+                float col[4] = {0.f, 0.f, 0.f, 0.f};       // with masses: this warp's sums of columns c * 32 + lane
+                if (valid > 0) {
+                    uint32_t x[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, x[c]);
+                    tmem_wait_ld();
+                    const int cols = w.s.seen - k * DEC_KEYS;          // visible columns of this step
+                    if (cols < DEC_KEYS) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (c * 32 + i >= cols) x[c][i] = 0xFF800000u;          // -inf
+                    }
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[c][i]));
+                    mx = lane < valid ? mx * p.c2 : -INFINITY;
+                    if (k == w.k0) ref = warp_max(mx);
+                    else if (__any_sync(0xFFFFFFFFu, mx > ref + GROW)) {
+                        // the products issued so far are complete (this step's scores came after them)
+                        const float now = warp_max(mx), f = fast_exp2(ref - now);
+                        ref = now;
+                        sum *= f;
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(tO + c * 32, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(tO + c * 32, o);
+                        }
+                    }
+                    // rows behind the last key contribute nothing: their exponent is -inf throughout
+                    const uint64_t scale = pair_f32(p.c2, p.c2);
+                    const float shift1 = lane < valid ? -ref : -INFINITY;
+                    const uint64_t shift = pair_f32(shift1, shift1);
+                    uint64_t s0 = pair_f32(0.f, 0.f), s1 = s0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float a, b;
+                            unpair_f32(fma_f32x2(pair_b32(x[c][i], x[c][i + 1]), scale, shift), a, b);
+                            v[i] = fast_exp2(a);
+                            v[i + 1] = fast_exp2(b);
+                            if (i & 2) s1 = add_f32x2(s1, pair_f32(v[i], v[i + 1]));
+                            else s0 = add_f32x2(s0, pair_f32(v[i], v[i + 1]));
+                            x[c >> 1][(c & 1) * 16 + i / 2] = pack_bf16x2(v[i], v[i + 1]);
+                        }
+                        if (MASS) col[c] = sgring::warp_transpose_sum(v, lane);
+                    }
+                    tmem_st32(tS, x[0]);
+                    tmem_st32(tS + 32, x[1]);
+                    tmem_wait_st();
+                    float a, b;
+                    unpair_f32(add_f32x2(s0, s1), a, b);
+                    sum += a + b;
+                }
+                tc_fence_before();
+                warp_arrive(&bars[DB_P_FULL0 + half], lane);
+                if (MASS) {
+                    // The half's column sums, relative to the largest of its four maxima: warps 2 and 3 hand theirs to
+                    // 0 and 1, then 1 to 0.  (The first warp of a live half has keys, so that maximum is finite.)
+                    float* buf = reinterpret_cast<float*>(smem + L::OFF_COL) + half * 256;
+                    if (lane == 0) sh_ref[half * 4 + wq] = valid > 0 ? ref : -INFINITY;
+                    if (wq >= 2) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) buf[(wq - 2) * 128 + c * 32 + lane] = col[c];
+                    }
+                    warp_arrive(&bars[DB_COL0 + half], lane);
+                    ok = pipe_wait(&bars[DB_COL0 + half], cols_phase++ & 1, fail, 11);
+                    if (!ok) break;
+                    const float* rf = sh_ref + half * 4;
+                    const float top = fmaxf(fmaxf(rf[0], rf[1]), fmaxf(rf[2], rf[3]));
+                    if (wq < 2) {
+                        const float f0 = fast_exp2(rf[wq] - top), f1 = fast_exp2(rf[wq + 2] - top);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            col[c] = col[c] * f0 + buf[wq * 128 + c * 32 + lane] * f1;
+                            if (wq == 1) buf[128 + c * 32 + lane] = col[c];
+                        }
+                    }
+                    warp_arrive(&bars[DB_COL0 + half], lane);
+                    ok = pipe_wait(&bars[DB_COL0 + half], cols_phase++ & 1, fail, 11);
+                    if (!ok) break;
+                    if (wq == 0) {
+                        const long long at = (w.unit + (k - w.k0)) * 2 + half;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) p.cols[at * 128 + c * 32 + lane] = col[c] + buf[128 + c * 32 + lane];
+                        if (lane == 0) p.col_ref[at] = top;
+                    }
+                    warp_arrive(&bars[DB_COL0 + half], lane);
+                    ok = pipe_wait(&bars[DB_COL0 + half], cols_phase++ & 1, fail, 11);
+                    if (!ok) break;
+                }
+            }
+            if (!ok) break;
+
+            // ---- collapse: y = sum over the strip's rows of Vr o U
+            ok = pipe_wait(&bars[DB_O_DONE0 + half], seg & 1, fail, 3);
+            if (!ok) break;
+            tc_fence_after();
+            if (valid > 0) {
+                const uint4* vr = reinterpret_cast<const uint4*>(p.Vr + (static_cast<size_t>(row) * p.Hkv + w.head) * D);
+                float l = lane < valid ? sum : 0.f;
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+                const int head = w.b * p.Hq + w.head * p.G + g;
+                if (head != cur) {
+                    flush();
+                    cur = head;
+                    cm = ref;
+                    cl = 0.f;
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c) cy[c] = 0.f;
+                }
+                const float m = fmaxf(cm, ref), f0 = fast_exp2(cm - m), f1 = fast_exp2(ref - m);
+                cm = m;
+                cl = cl * f0 + l * f1;
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(tO + c * 32, o);
+                    uint4 t[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) t[i] = __ldg(vr + c * 4 + i);
+                    tmem_wait_ld();
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t u[4] = {t[i].x, t[i].y, t[i].z, t[i].w};
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float2 f = unpack_bf16x2(u[q]);
+                            const int d = i * 8 + q * 2;
+                            v[d] = f.x * __uint_as_float(o[d]);
+                            v[d + 1] = f.y * __uint_as_float(o[d + 1]);
+                        }
+                    }
+                    if (valid < DEC_STRIP && lane >= valid) {          // rows behind the last key
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                    }
+                    cy[c] = cy[c] * f0 + sgring::warp_transpose_sum(v, lane) * f1;
+                }
+                if (MASS) {
+                    const long long rec = w.slot * DEC_TILE_STRIPS + warp;
+                    p.rows[rec * DEC_STRIP + lane] = lane < valid ? sum : 0.f;
+                    if (lane == 0) p.row_ref[rec] = ref;
+                }
+            }
+            tc_fence_before();
+            ++seg;
+            go = w.next(p);
+        }
+        flush();
+    } else {
+        sgring::reg_dec<88>();
+        if (warp == 8 && busy) {
+            // ================================================================== products
+            const uint32_t issuer = elect_one();
+            const uint32_t idesc_x = make_idesc_bf16(128, 128, 0, 0);
+            const uint32_t idesc_u = make_idesc_bf16(128, D, 0, 1);
+            int n[2] = {0, 0}, seg[2] = {0, 0};            // steps and segments so far, per half
+            int fill = 0;                                  // stages consumed
+            bool go = true, ok = true;
+            auto stage_desc = [&](int f, bool mn) {
+                return make_smem_desc(smem_u32(smem + L::OFF_KV + (f % L::STAGES) * L::TILE), mn ? 128 * 128 : 16, 1024, SWIZZLE_128B);
+            };
+            auto stage_wait = [&](int f) { return pipe_wait(&bars[DB_KV_FULL0 + f % L::STAGES], (f / L::STAGES) & 1, fail, 4); };
+            auto scores = [&](int t, int f) {
+                const uint64_t b = stage_desc(f, false);
+                const uint32_t tX = tmem + t * 128;
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    const uint64_t a = make_smem_desc(smem_u32(smem + L::OFF_A + (2 * t + part) * L::TILE), 16, 1024, SWIZZLE_128B);
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = ((kk >> 2) * 128 * 128 + (kk & 3) * 32) / 16;
+                        umma_ss_pred(tX, a + off, b + off, idesc_x, part > 0 || kk > 0, issuer);
+                    }
+                }
+                umma_commit_pred(&bars[DB_S_FULL0 + t], issuer);
+            };
+#pragma unroll 1
+            while (go && ok) {
+                const bool two = w.live(1);
+                ok = stage_wait(fill);
+                for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
+                    ok = pipe_wait(&bars[DB_A_FULL0 + t], seg[t] & 1, fail, 5);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(t, fill);
+                }
+                if (!ok) break;
+                umma_commit_pred(&bars[DB_KV_EMPTY0 + fill % L::STAGES], issuer);
+#pragma unroll 1
+                for (int k = w.k0; k < w.k1 && ok; ++k) {
+                    const bool more = k + 1 < w.k1;
+                    ok = stage_wait(fill + 1);
+                    for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
+                        ok = pipe_wait(&bars[DB_P_FULL0 + t], n[t] & 1, fail, 6);
+                        if (!ok) break;
+                        ++n[t];
+                        tc_fence_after();
+                        const uint64_t b = stage_desc(fill + 1, true);
+#pragma unroll
+                        for (int kk = 0; kk < 8; ++kk)
+                            umma_ts_pred(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, b + kk * (2048 / 16), idesc_u, k > w.k0 || kk > 0, issuer);
+                        if (!more) umma_commit_pred(&bars[DB_O_DONE0 + t], issuer);
+                        else {
+                            if (t == 0) ok = stage_wait(fill + 2);
+                            if (!ok) break;
+                            scores(t, fill + 2);
+                        }
+                    }
+                    if (!ok) break;
+                    umma_commit_pred(&bars[DB_KV_EMPTY0 + (fill + 1) % L::STAGES], issuer);
+                    if (more) umma_commit_pred(&bars[DB_KV_EMPTY0 + (fill + 2) % L::STAGES], issuer);
+                    fill += 2;
+                }
+                ++seg[0];
+                if (two) ++seg[1];
+                go = w.next(p);
+            }
+            // nothing of this warp's is in flight when the tensor memory is given back
+            umma_commit_pred(&bars[DB_DRAIN], issuer);
+            pipe_wait(&bars[DB_DRAIN], 0, fail, 7);
+        } else if (warp == 9 && busy) {
+            // ================================================================== rows of S and Vs
+            int fill = 0;
+            bool go = true, ok = true;
+#pragma unroll 1
+            while (go && ok) {
+#pragma unroll 1
+                for (int k = w.k0; k < w.k1 && ok; ++k) {
+                    int row[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // columns behind the last key repeat its row: they are masked, and a finite row stays finite
+                        const int e = min(k * DEC_KEYS + lane * 4 + i, w.s.seen - 1);
+                        row[i] = p.pages.row(w.b, slot_of(p, w.s, e));
+                        if (row[i] < 0) { report(p.status, ST_PAGE); row[i] = 0; }
+                    }
+#pragma unroll 1
+                    for (int kind = 0; kind < 2; ++kind, ++fill) {
+                        const int st = fill % L::STAGES;
+                        if (fill >= L::STAGES) ok = pipe_wait(&bars[DB_KV_EMPTY0 + st], (fill / L::STAGES - 1) & 1, fail, 8);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(&bars[DB_KV_FULL0 + st], L::TILE);
+                        __syncwarp();
+                        uint8_t* dst = smem + L::OFF_KV + st * L::TILE + lane * 512;
+                        const void* map = kind ? &p.tmVs : &p.tmS;
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h)
+                            tma_gather4(dst + h * 128 * 128, map, w.head * D + h * 64, row, &bars[DB_KV_FULL0 + st]);
+                    }
+                }
+                go = go && w.next(p);
+            }
+            // every copy that was asked for has landed before the CTA ends
+            for (int f = max(0, fill - L::STAGES); f < fill; ++f)
+                pipe_wait(&bars[DB_KV_FULL0 + f % L::STAGES], (f / L::STAGES) & 1, fail, 9);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_dealloc(tmem, 512);
+    if (tid == 0 && *fail) report(p.status, *fail & 0xFF);
+}
+
+// The partials of one head, CTA by CTA in a fixed order.  Warp w takes what warp w of each CTA wrote, its lanes the
+// columns.
+template <int D, bool MASS>
+__global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant__ DecodeParams p, int ctas) {
+    constexpr int REC = D + 4, COLS = D / 32;
+    __shared__ float sh_m[8], sh_l[8], sh_y[8][D];
+    const int b = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq, kv = hq / p.G, g = hq % p.G;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Shape s = shape_of<MASS>(p, b);
+    __nv_bfloat16* y = p.Y + static_cast<size_t>(blockIdx.x) * D;
+    if (s.seen == 0) {
+        if (threadIdx.x < D) y[threadIdx.x] = __float2bfloat16_rn(0.f);
+        return;
+    }
+    const long long total = p.unit_base[p.B], units0 = p.unit_base[b] + static_cast<long long>(kv) * s.tiles * s.steps;
+    const int lo = g * s.per_head, hi = lo + (s.seen + DEC_STRIP - 1) / DEC_STRIP;         // the head's strips with keys
+    const long long u0 = units0 + static_cast<long long>(lo / DEC_TILE_STRIPS) * s.steps;
+    const long long u1 = units0 + static_cast<long long>((hi - 1) / DEC_TILE_STRIPS + 1) * s.steps;
+    const int c0 = cta_of(u0, total, ctas), c1 = cta_of(u1 - 1, total, ctas);
+    float m = -INFINITY, l = 0.f, acc[COLS];
+#pragma unroll
+    for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
+    for (int c = c0; c <= c1; ++c) {
+        // the tiles of the head that CTA c went through, and whether this warp had a strip of the head in them
+        const long long from = max(total * c / ctas, u0), to = min(total * (c + 1) / ctas, u1);
+        if (from >= to) continue;
+        const int ta = static_cast<int>((from - units0) / s.steps), tb = static_cast<int>((to - 1 - units0) / s.steps);
+        int strip = ta * DEC_TILE_STRIPS + warp;
+        if (strip < lo) strip += (lo - strip + DEC_TILE_STRIPS - 1) / DEC_TILE_STRIPS * DEC_TILE_STRIPS;
+        if (strip >= hi || strip / DEC_TILE_STRIPS > tb) continue;
+        const float* r = p.part + (static_cast<long long>(blockIdx.x) + c) * DEC_TILE_STRIPS * REC + warp * REC;
+        const float rm = r[D], top = fmaxf(m, rm), f0 = fast_exp2(m - top), f1 = fast_exp2(rm - top);
+        m = top;
+        l = l * f0 + r[D + 1] * f1;
+#pragma unroll
+        for (int q = 0; q < COLS; ++q) acc[q] = acc[q] * f0 + r[q * 32 + lane] * f1;
+    }
+    if (lane == 0) { sh_m[warp] = m; sh_l[warp] = l; }
+#pragma unroll
+    for (int q = 0; q < COLS; ++q) sh_y[warp][q * 32 + lane] = acc[q];
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float top = sh_m[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, sh_m[i]);
+        float a = 0.f, ls = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = fast_exp2(sh_m[i] - top);
+            a += sh_y[i][threadIdx.x] * f;
+            ls += sh_l[i] * f;
+        }
+        y[threadIdx.x] = __float2bfloat16_rn(a / ls);
+        if (MASS && threadIdx.x == 0) p.lse[blockIdx.x] = top + log2f(ls);
+    }
+}
+
+// Adds every visible slot's share of the attention to its mass: a thread a slot, the heads and partials in a fixed order.
+__global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant__ DecodeParams p, int ctas) {
+    const int b = blockIdx.y / p.Hkv, kv = blockIdx.y % p.Hkv;
+    const Shape s = shape_of<true>(p, b);
+    const int e = blockIdx.x * 128 + threadIdx.x;
+    if (e >= s.seen) return;
+    const int row = p.pages.row(b, slot_of(p, s, e));
+    if (row < 0) return;
+    const long long total = p.unit_base[p.B], units0 = p.unit_base[b] + static_cast<long long>(kv) * s.tiles * s.steps;
+    const long long tiles0 = p.tile_base[b] + static_cast<long long>(kv) * s.tiles;
+    const int step = e / DEC_KEYS, col = e % DEC_KEYS, per_head = s.per_head / DEC_TILE_STRIPS;
+    float share = 0.f;
+    for (int g = 0; g < p.G; ++g) {
+        const float lse = p.lse[b * p.Hq + kv * p.G + g];
+        const int tile = g * per_head + e / 256;
+        const long long u = units0 + static_cast<long long>(tile) * s.steps;
+        const int c0 = cta_of(u, total, ctas), c1 = cta_of(u + s.steps - 1, total, ctas);
+        for (int c = c0; c <= c1; ++c) {
+            if (total * c / ctas >= total * (c + 1) / ctas) continue;
+            const long long rec = (tiles0 + tile + c) * DEC_TILE_STRIPS + (e % 256) / DEC_STRIP;
+            share += p.rows[rec * DEC_STRIP + e % DEC_STRIP] * fast_exp2(p.row_ref[rec] - lse);
+        }
+        for (int t = 0; t < per_head; ++t) {
+            const long long at = (units0 + static_cast<long long>(g * per_head + t) * s.steps + step) * 2;
+            share += p.cols[at * 128 + col] * fast_exp2(p.col_ref[at] - lse);
+            if (t * 256 + 128 < s.seen) share += p.cols[(at + 1) * 128 + col] * fast_exp2(p.col_ref[at + 1] - lse);
+        }
+    }
+    p.mass[static_cast<long long>(row) * p.Hkv + kv] += share / (2.f * p.G);
+}
+
+}  // namespace serve

@@ -125,7 +125,14 @@ extern "C" int att3_device_status(void* stream) {
     e = cudaMemcpyFromSymbol(&h, g_sg_status, sizeof(int));
     if (e != cudaSuccess) return att3::set_cuda_error(e, "att3_device_status: read");
     if (int rc = att3::dense_status_read_and_clear(&h2)) return rc;
+    int h3 = 0;
+    if (int rc = att3::serve_status_read_and_clear(&h3)) return rc;
     if (h == 0) h = h2;
+    if (h == 0) h = h3 & 0xFF;             // a wait of the serving kernels; the bits above it are bad table entries
+    if (h == 0 && h3 != 0)
+        return att3::set_error(ATT3_ERR_INVALID, "a serving kernel met%s%s%s outside its table (status 0x%x)",
+                               h3 & 0x100 ? " a page number" : "", h3 & 0x200 ? " a position" : "",
+                               h3 & 0x400 ? " a length" : "", h3);
     if (h != 0) {
         const int zero = 0;
         cudaMemcpyToSymbol(g_sg_status, &zero, sizeof(int));

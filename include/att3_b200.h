@@ -268,6 +268,96 @@ int att3_hg_backward_axes(const void* gYq, const void* gYr, const void* gYs,
                           int gather_mode, int scatter, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------- *
+ * Serving the single gather (no counterpart in the reference, which has no
+ * form for single tokens): head norms with the position rotation, a paged cache
+ * of the rows that later queries need, the gather of one new token over it, and
+ * eviction from it.  These entry points take head rows in any order of batch,
+ * position and head (strides in elements; the D elements of a row contiguous,
+ * every row on a 16-byte boundary) and in BF16, FP16 or FP32; what goes to the
+ * attention or the cache is BF16.  D is 16, 32, 64 or 128 (64 or 128 for the
+ * gather).  Tables, page numbers, positions and lengths are read on the device:
+ * an entry outside its table is left out, never followed, and the next
+ * att3_device_status() reports ATT3_ERR_INVALID with its kind.
+ * ------------------------------------------------------------------------- */
+
+/* Element types. */
+#define ATT3_BF16 0
+#define ATT3_FP16 1
+#define ATT3_FP32 2
+
+/* One tensor of head rows [B, N, heads, D].  Every member is 8 bytes wide. */
+typedef struct att3_head_rows {
+    const void* x;
+    int64_t x_stride[3];       /* batch, position, head */
+    const void* w;             /* scale [D], or NULL: not normed */
+    int64_t w_type;
+    int64_t rotate;            /* 0: not rotated */
+    void* y;                   /* BF16 result; appending: the pool (Q: a result) */
+    int64_t y_stride[3];       /* unused for a pool */
+    const void* dy;            /* backward: BF16 cotangent of y */
+    int64_t dy_stride[3];
+    void* dx;                  /* backward: gradient of x, of x's type */
+    int64_t dx_stride[3];
+    float* dw;                 /* backward: gradient of w, FP32 [D] */
+    int64_t heads;
+} att3_head_rows;
+
+/* y = Rot(w o x / sqrt(mean(x^2) + eps)) for up to five tensors in one pass.  Rot turns pairs of the first `rot`
+ * columns (0, 8 or a multiple of 16), (d, d + rot/2) or with `interleaved` (2d, 2d + 1), by the angles of the row's
+ * position: table is FP32 [table_rows, rot], the cosines of a position and then its sines.  positions: 4 or 8 byte
+ * integers with strides pos_b, pos_n, or NULL for 0 .. N-1. */
+int att3_norm_rotate_forward(const att3_head_rows* tensors, int n, int x_type, const float* table, int table_rows,
+                             int rot, int interleaved, const void* positions, int pos_bytes, int64_t pos_b,
+                             int64_t pos_n, int B, int N, int D, float eps, void* stream);
+/* Gradients of x (of x's type) and w (FP32) from the BF16 cotangents.  Sums have a fixed order: repeated calls agree
+ * to the bit. */
+size_t att3_norm_rotate_workspace_bytes(int n, int D);
+int att3_norm_rotate_backward(const att3_head_rows* tensors, int n, int x_type, const float* table, int table_rows,
+                              int rot, int interleaved, const void* positions, int pos_bytes, int64_t pos_b,
+                              int64_t pos_n, int B, int N, int D, float eps, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Pages of a gather cache.  A pool is BF16 [pages, page_size, Hkv, D] contiguous; entry [b, p] of the table names the
+ * page with slots p * page_size .. of sequence b.  Every member is 8 bytes wide. */
+typedef struct att3_gather_pages {
+    const int32_t* table;
+    int64_t table_stride;      /* entries between the rows of two sequences */
+    int64_t per_sequence;      /* entries of a row */
+    int64_t pages;             /* pages in a pool */
+    int64_t page_size;
+} att3_gather_pages;
+
+/* Stores T new rows of R, S, Vr, Vs (tensors 0 .. 3, y = the pools) at slots lengths[b] .. of sequence b, the first
+ * counts[b] of them if counts is given; tensors with a scale are normed, those with `rotate` rotated by the position
+ * positions[b] + t (lengths[b] + t without positions) on the way.  Tensor 4, if given, is Q: all T of its rows go to
+ * y.  mass [pages, page_size, Hkv], if given, is zeroed at the slots written.  lengths is not changed. */
+int att3_gather_cache_append(const att3_head_rows* tensors, int n, int x_type, const float* table, int table_rows,
+                             int rot, int interleaved, const int32_t* positions, const att3_gather_pages* pages,
+                             const int32_t* lengths, const int32_t* counts, float* mass, int B, int T, int D, float eps,
+                             void* stream);
+
+/* Keeps min(lengths[b], keep) slots of every sequence and key head: the first `sinks`, the last `recent` and, between
+ * them, those with the largest mass (equal ones: the lowest slots; NaN counts as largest).  They move, in order, to
+ * slots 0 .. of out_table's pages, with their mass; all pools are handled by the one call.  out is the page table
+ * itself (in place) or names pages that no sequence of the call reads.  kept [B, Hkv, keep] receives the slots (-1
+ * behind the last), new_lengths [B] the counts. */
+int att3_gather_cache_evict(void* R, void* S, void* Vr, void* Vs, float* mass, const att3_gather_pages* pages,
+                            const att3_gather_pages* out, const int32_t* lengths, int32_t* new_lengths, int32_t* kept,
+                            int B, int Hkv, int D, int keep, int sinks, int recent, void* stream);
+
+/* One new token of each sequence: Q [B, Hq, D] BF16 over the cached slots 0 .. lengths[b]-1 (the token's own rows among
+ * them), Y [B, Hq, D] BF16.  window > 0: a slot is visible if it is among the last `window` or the first `sinks`;
+ * window == 0: all are.  A sequence of length 0 gives zeros.  Scores are formed from Q o R split into its BF16 value
+ * and the BF16 residual, without rounding.  mass, if given, is FP32 [pages, page_size, Hkv] and gains every visible
+ * slot's share of the attention: half the probability of the pairs with it on the R side plus half of those with it
+ * on the S side, averaged over the query heads of the key head (1 in all a sequence and key head).  Heads, the
+ * table's width and B fix the workspace; the lengths do not. */
+size_t att3_sg_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int window, int sinks, int max_slots, int with_mass);
+int att3_sg_decode(const void* Q, const void* R, const void* S, const void* Vr, const void* Vs, float* mass, void* Y,
+                   const att3_gather_pages* pages, const int32_t* lengths, int B, int Hq, int Hkv, int D, int window,
+                   int sinks, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- *
  * Host-side helpers (no GPU needed).
  * ------------------------------------------------------------------------- */
 

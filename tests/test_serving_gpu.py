@@ -1,0 +1,463 @@
+"""Head norms with rotation, gather-cache append, single-token gather and eviction on the GPU against their definitions
+in 64 bits.
+
+Tolerances.  A rounding to BF16 is off by at most 2^-8 of the value.  The gather's result has one, and one of every
+probability before the second product: |Y - Y64| <= 2^-8 |Y| + 2^-8 A with A = sum P |Vr o Vs|, both times 1 + 2^-8
+for the order of the two.  What remains is FP32: a score is a sum of 2 D products of magnitude |q r s| / sqrt(D), a
+relative error of the probabilities of at most 2 D 2^-24 sum|q r s| / sqrt(D) (1e-4 for the largest used here, and a
+tensor core may cut where it would round, so twice that)."""
+import pytest
+import torch
+
+from helpers import serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+HALF = 2.0 ** -8                        # BF16
+
+
+def rand(g, *shape, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+def close(got, want, tol, what=""):
+    d = (got.double().cpu() - want).abs()
+    bad = d > tol
+    assert not bad.any() and torch.isfinite(got).all(), f"{what}: off by {d.max():.3g}, {int(bad.sum())} of {bad.numel()} over, worst excess {(d - tol).max():.3g}"
+
+
+# --------------------------------------------------------------------------- head norms with rotation
+
+NORM_CASES = [
+    # B, N, heads, D, rot, type, interleaved, heads_first
+    (1, 1, (1,), 16, 8, torch.float32, False, False),
+    (2, 5, (3, 1), 16, 16, torch.bfloat16, False, True),
+    (2, 7, (4, 2, 2), 32, 16, torch.float16, True, False),
+    (3, 33, (8, 1, 1), 64, 32, torch.bfloat16, False, False),
+    (1, 129, (5, 5, 5), 64, 64, torch.float32, True, True),
+    (2, 65, (8, 2, 2), 128, 128, torch.bfloat16, False, False),
+    (1, 31, (6, 3, 1), 128, 48, torch.float32, False, True),
+    (2, 40, (2, 2, 2, 2, 2), 128, 0, torch.bfloat16, False, False),
+    (1, 1000, (9, 1, 1), 128, 64, torch.float16, True, True),
+]
+
+
+@pytest.mark.parametrize("B,N,heads,D,rot,dtype,interleaved,heads_first", NORM_CASES)
+@pytest.mark.parametrize("scaled", ["all", "some"])
+def test_norm_rotate_and_gradients(B, N, heads, D, rot, dtype, interleaved, heads_first, scaled):
+    from att3ntion_b200 import norm_rotate, rotary_table
+    g = torch.Generator().manual_seed(B * 1000 + N)
+    eps = 1e-5
+    table = rotary_table(N + 500, rot) if rot else None
+    pos = torch.randint(0, N + 500, (B, N), generator=g)
+    xs = [rand(g, B, N, h, D, dtype=dtype) * 2 for h in heads]
+    ws = [None if scaled == "some" and k % 2 else 1 + 0.3 * torch.randn(D, generator=g) for k in range(len(heads))]
+    dys = [rand(g, B, h, N, D) if heads_first else rand(g, B, N, h, D) for h in heads]
+    leaves = [x.cuda().requires_grad_() for x in xs]
+    scales = [None if w is None else w.cuda().requires_grad_() for w in ws]
+    ys = norm_rotate(leaves, scales, table.cuda() if rot else None, pos.cuda(), eps=eps, interleaved=interleaved, heads_first=heads_first)
+    torch.autograd.backward(ys, [d.cuda() for d in dys])
+    for x, w, dy, y, leaf, scale in zip(xs, ws, dys, ys, leaves, scales):
+        x64 = x.double().requires_grad_()
+        w64 = None if w is None else w.double().requires_grad_()
+        y64 = ref.norm_rotate(x64, w64, table.double() if rot else None, pos, eps, interleaved)
+        shaped = y64.transpose(1, 2) if heads_first else y64
+        # one rounding, and a dozen FP32 operations on values of the row's size
+        slack = 2e-6 * y64.detach().abs().amax(-1, keepdim=True)
+        close(y, shaped.detach(), HALF * shaped.detach().abs() + (slack.transpose(1, 2) if heads_first else slack), "y")
+        shaped.backward(dy.double())
+        half = torch.finfo(dtype).eps / 2
+        close(leaf.grad, x64.grad, half * x64.grad.abs() + 4e-6 * x64.grad.abs().amax(-1, keepdim=True) + 1e-6 * (0 if w is None else 1), "dx")
+        assert leaf.grad.dtype == dtype
+        if w is not None:
+            # B N heads terms, each with a few FP32 roundings, summed in two levels
+            u = (x64 * (x64.pow(2).mean(-1, keepdim=True) + eps).rsqrt()).detach()
+            terms = (dy.double().transpose(1, 2) if heads_first else dy.double()).abs().amax(-1, keepdim=True) * u.abs()
+            close(scale.grad, w64.grad, 3e-6 * terms.sum((0, 1, 2)) + 1e-7, "dw")
+
+
+@pytest.mark.parametrize("make", ["sliced", "transposed", "expanded", "odd offset", "columns apart"])
+def test_norm_rotate_takes_any_strides(make):
+    from att3ntion_b200 import norm_rotate, rotary_table
+    g = torch.Generator().manual_seed(5)
+    B, N, H, D = 2, 19, 3, 64
+    if make == "sliced":                                 # the heads of a joint projection
+        x = rand(g, B, N, H + 4, D).cuda()[:, :, 2:2 + H]
+    elif make == "transposed":
+        x = rand(g, B, H, N, D).cuda().transpose(1, 2)
+    elif make == "expanded":
+        x = rand(g, B, 1, H, D).cuda().expand(B, N, H, D)
+    elif make == "odd offset":
+        x = rand(g, B * N * H * D + 1).cuda()[1:].view(B, N, H, D)
+    else:
+        x = rand(g, B, N, H, D * 2).cuda()[..., ::2]
+    w, table = (1 + torch.rand(D + 1, generator=g)).cuda()[1:], rotary_table(N, 32).cuda()
+    x = x.detach().requires_grad_()
+    y = norm_rotate(x, w, table)
+    want = norm_rotate(x.detach().contiguous().clone(), w.clone(), table)
+    assert torch.equal(y, want)
+    dy = rand(g, B, H, N, D).cuda().transpose(1, 2)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    x2 = x.detach().contiguous().clone().requires_grad_()
+    (dx2,) = torch.autograd.grad(norm_rotate(x2, w.clone(), table), x2, dy.contiguous())
+    assert torch.equal(dx, dx2)
+
+
+def test_norm_rotate_empty_and_repeatable():
+    from att3ntion_b200 import norm_rotate
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    x = torch.empty(2, 0, 3, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = norm_rotate(x, w)
+    assert y.shape == x.shape
+    gx, gw = torch.autograd.grad(y, [x, w], torch.empty_like(y))
+    assert gx.shape == x.shape and not gw.any()
+    x = torch.randn(3, 700, 5, 64, device="cuda", requires_grad=True)
+    dy = torch.randn(3, 700, 5, 64, device="cuda").bfloat16()
+    first = torch.autograd.grad(norm_rotate(x, w), [x, w], dy)
+    for _ in range(3):
+        for a, b in zip(first, torch.autograd.grad(norm_rotate(x, w), [x, w], dy)):
+            assert torch.equal(a, b)
+
+
+def test_norm_rotate_reports_a_position_outside_its_table():
+    from att3ntion_b200 import _cuda_kernels as ck, norm_rotate, rotary_table
+    x = torch.randn(1, 4, 2, 64, device="cuda")
+    table = rotary_table(8, 64).cuda()
+    pos = torch.tensor([0, 7, 3, 1], device="cuda")
+    norm_rotate(x, None, table, pos)
+    ck.device_status()
+    for bad in (8, -1, 1 << 40):
+        got = norm_rotate(x, None, table, torch.tensor([0, bad, 3, 1], device="cuda"))
+        with pytest.raises(RuntimeError, match="position"):
+            ck.device_status()
+        assert torch.isfinite(got).all()
+        ck.device_status()                               # reported once
+
+
+# --------------------------------------------------------------------------- a cache to work on
+
+class Made:
+    """Pools with random rows, pages handed out in random order, -1 in the entries behind each sequence's last page."""
+
+    def __init__(self, seed, lengths, Hkv, D, page, room=0, scale=1.0):
+        g = self.g = torch.Generator().manual_seed(seed)
+        self.B, self.page = len(lengths), page
+        need = [-(-(n + room) // page) for n in lengths]
+        total = sum(need) + 2
+        order = torch.randperm(total, generator=g).int()
+        self.table = torch.full((self.B, max(max(need), 1)), -1, dtype=torch.int32)
+        at = 0
+        for b, k in enumerate(need):
+            self.table[b, :k] = order[at: at + k]
+            at += k
+        self.free = order[at:]
+        self.pools = [rand(g, total, page, Hkv, D) * scale for _ in range(4)]
+        self.mass = torch.rand(total, page, Hkv, generator=g)
+        self.lengths = torch.tensor(lengths, dtype=torch.int32)
+
+    def gpu(self):
+        return [p.cuda() for p in self.pools], self.table.cuda(), self.lengths.cuda()
+
+
+# --------------------------------------------------------------------------- append
+
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,page,dtype,interleaved", [
+    (1, 1, 1, 1, 16, 1, torch.float32, False),
+    (3, 1, 8, 1, 128, 16, torch.bfloat16, False),
+    (4, 37, 6, 2, 64, 7, torch.float16, True),
+    (2, 130, 4, 4, 128, 64, torch.float32, False),
+])
+@pytest.mark.parametrize("normed", [True, False])
+def test_append(B, T, Hq, Hkv, D, page, dtype, interleaved, normed):
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append, rotary_table
+    g = torch.Generator().manual_seed(T + page)
+    have = [int(torch.randint(0, 3 * page, (1,), generator=g)) for _ in range(B)]
+    c = Made(1, have, Hkv, D, page, room=T)
+    pools, table, lengths = c.gpu()
+    mass = c.mass.cuda()
+    new = [rand(g, B, T, Hkv, D, dtype=dtype) for _ in range(4)]
+    Q = rand(g, B, T, Hq, D, dtype=dtype)
+    counts = torch.randint(0, T + 1, (B,), generator=g).int()
+    counts[0] = T
+    start = torch.randint(0, 300, (B,), generator=g).int()
+    ws = [1 + 0.3 * torch.randn(D, generator=g) for _ in range(3)] if normed else None
+    rot = rotary_table(300 + T, D // 2) if normed else None
+    out = gather_cache_append(pools, table, lengths, *[x.cuda() for x in new], counts=counts.cuda(), Q=Q.cuda(),
+                              weights=None if ws is None else [w.cuda() for w in ws], table=None if rot is None else rot.cuda(),
+                              positions=start.cuda(), mass=mass, interleaved=interleaved)
+    ck.device_status()
+    pos = start.long()[:, None] + torch.arange(T)
+    want = [p.double() for p in c.pools]
+    rows = [x.double() for x in new]
+    q64 = Q.double()
+    if normed:
+        t64 = rot.double()
+        q64 = ref.norm_rotate(q64, ws[0].double(), t64, pos, 1e-6, interleaved)
+        rows[0] = ref.norm_rotate(rows[0], ws[1].double(), t64, pos, 1e-6, interleaved)
+        rows[1] = ref.norm_rotate(rows[1], ws[2].double(), t64, pos, 1e-6, interleaved)
+    wmass = c.mass.clone()
+    for b in range(B):
+        for t in range(int(counts[b])):
+            e = have[b] + t
+            at = (int(c.table[b, e // page]), e % page)
+            for w, r in zip(want, rows):
+                w[at] = r[b, t]
+            wmass[at] = 0
+    close(out, q64, HALF * q64.abs() + 1e-5, "Q")
+    for k, (p, w) in enumerate(zip(pools, want)):
+        close(p, w, HALF * w.abs() + (1e-5 if normed and k < 2 else 0), f"pool {k}")
+    assert torch.equal(mass.cpu(), wmass) and torch.equal(lengths.cpu(), c.lengths)
+
+
+def test_append_leaves_out_what_has_no_page():
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append
+    c = Made(2, [3, 30], 1, 64, 16, room=2)
+    c.table[0, 0] = 999                                  # a page that the pool does not have
+    c.lengths[1] = 47                                    # the second of two new slots lies behind the table's end
+    pools, table, lengths = c.gpu()
+    new = [torch.randn(2, 2, 1, 64, device="cuda") for _ in range(4)]
+    gather_cache_append(pools, table, lengths, *new)
+    with pytest.raises(RuntimeError, match="page"):
+        ck.device_status()
+    for p, old, x in zip(pools, c.pools, new):
+        want = old.cuda()
+        if table.shape[1] > 2:
+            want[int(c.table[1, 2]), 15] = x[1, 0].bfloat16()
+        assert torch.equal(p, want)
+
+
+# --------------------------------------------------------------------------- the gather of one new token
+
+DECODE_CASES = [
+    # lengths, Hq, Hkv, D, page, window, sinks
+    ([1], 1, 1, 128, 16, 0, 0),
+    ([0, 1, 2, 0], 4, 2, 64, 16, 0, 0),
+    ([128], 8, 1, 128, 16, 128, 0),
+    ([5, 200, 127, 128, 129], 8, 1, 128, 16, 128, 0),
+    ([300, 17, 132, 131, 133], 8, 2, 128, 32, 128, 4),
+    ([31, 32, 33, 64, 65, 96, 97], 3, 1, 128, 7, 0, 0),
+    ([700, 1, 259], 2, 2, 128, 64, 0, 0),
+    ([1000], 1, 1, 64, 128, 0, 0),
+    ([513, 40], 6, 3, 64, 1, 0, 0),
+    ([77, 900, 16], 16, 1, 128, 16, 16, 0),
+    ([77, 900, 16], 8, 8, 64, 16, 1, 3),
+    ([600, 256], 4, 1, 128, 256, 300, 37),
+    ([50] * 40, 8, 4, 128, 16, 33, 1),
+]
+
+
+@pytest.mark.parametrize("lengths,Hq,Hkv,D,page,window,sinks", DECODE_CASES)
+@pytest.mark.parametrize("with_mass", [False, True])
+def test_decode(lengths, Hq, Hkv, D, page, window, sinks, with_mass):
+    from att3ntion_b200 import _cuda_kernels as ck, single_gather_decode
+    c = Made(3, lengths, Hkv, D, page)
+    Q = rand(c.g, c.B, Hq, D)
+    Y64, A, share = ref.decode(Q, c.pools, c.table, lengths, window, sinks)
+    pools, table, dev_lengths = c.gpu()
+    mass = c.mass.cuda() if with_mass else None
+    Y = single_gather_decode(Q.cuda(), pools, table, dev_lengths, window=window, sinks=sinks, mass=mass)
+    ck.device_status()
+    close(Y, Y64, (1 + HALF) * HALF * (Y64.abs() + A) + 2e-4 * A, "Y")
+    if with_mass:
+        want = c.mass.double()
+        for at, v in share.items():
+            want[at] += v
+        # FP32 sums and exponentials, and the old value's rounding
+        close(mass, want, 2.0 ** -24 * want + 2e-5 * (want - c.mass.double()), "mass")
+        untouched = want == c.mass.double()
+        assert torch.equal(mass.cpu()[untouched], c.mass[untouched])
+
+
+@pytest.mark.parametrize("scale", [1e-3, 4.0])
+def test_decode_small_and_large_scores(scale):
+    """Scores from 1e-9 to hundreds: the softmax is flat, or one pair takes everything."""
+    from att3ntion_b200 import single_gather_decode
+    lengths = [300, 70]
+    c = Made(4, lengths, 1, 128, 16, scale=scale)
+    Q = rand(c.g, 2, 4, 128) * scale
+    Y64, A, _ = ref.decode(Q, c.pools, c.table, lengths)
+    pools, table, n = c.gpu()
+    Y = single_gather_decode(Q.cuda(), pools, table, n)
+    # sum |q r s| / sqrt(D) is 64 times larger at scale 4
+    close(Y, Y64, (1 + HALF) * HALF * (Y64.abs() + A) + 2e-4 * max(1.0, scale ** 3) * A, "Y")
+
+
+def test_decode_never_reads_behind_the_lengths():
+    """NaN and infinity in every slot that is not visible, in spare pages too."""
+    from att3ntion_b200 import single_gather_decode
+    lengths, page, window, sinks = [150, 20, 77], 16, 60, 5
+    c = Made(6, lengths, 2, 64, page)
+    Q = rand(c.g, 3, 4, 64)
+    pools, table, n = c.gpu()
+    want = single_gather_decode(Q.cuda(), pools, table, n, window=window, sinks=sinks)
+    seen = torch.zeros(c.pools[0].shape[:2], dtype=torch.bool)
+    for b, length in enumerate(lengths):
+        for e in ref.visible(length, window, sinks):
+            seen[int(c.table[b, e // page]), e % page] = True
+    for k, p in enumerate(pools):
+        p[~seen.cuda()] = float("nan") if k % 2 else float("inf")
+    got = single_gather_decode(Q.cuda(), pools, table, n, window=window, sinks=sinks)
+    assert torch.isfinite(want).all() and torch.equal(got, want)
+
+
+def test_decode_does_not_depend_on_the_batch_around_it():
+    """A sequence's result alone and in a batch differs by the order of FP32 sums at most."""
+    from att3ntion_b200 import single_gather_decode
+    lengths = [400, 1, 260, 33, 900, 0, 128]
+    c = Made(7, lengths, 2, 128, 16)
+    Q = rand(c.g, c.B, 8, 128).cuda()
+    pools, table, n = c.gpu()
+    Y = single_gather_decode(Q, pools, table, n)
+    for b in range(c.B):
+        one = single_gather_decode(Q[b: b + 1], pools, table[b: b + 1], n[b: b + 1])
+        # both round an FP32 sum to BF16 once; P's rounding moves with the strip's reference: compare as two estimates
+        _, A, _ = ref.decode(Q[b: b + 1].cpu(), c.pools, c.table[b: b + 1], lengths[b: b + 1])
+        close(one, Y[b: b + 1].double().cpu(), 2 * ((1 + HALF) * HALF * (Y[b: b + 1].double().cpu().abs() + A) + 2e-4 * A))
+    again = single_gather_decode(Q, pools, table, n)
+    assert torch.equal(Y, again)
+
+
+def test_decode_reports_bad_tables():
+    from att3ntion_b200 import _cuda_kernels as ck, single_gather_decode
+    c = Made(8, [100, 40], 1, 128, 16)
+    Q = rand(c.g, 2, 4, 128).cuda()
+    pools, table, n = c.gpu()
+    want = single_gather_decode(Q, pools, table, n)
+    ck.device_status()
+    bad = table.clone()
+    bad[0, 3] = 10 ** 6
+    got = single_gather_decode(Q, pools, bad, n)
+    with pytest.raises(RuntimeError, match="page"):
+        ck.device_status()
+    assert torch.equal(got[1], want[1])
+    for length in (-5, 10 ** 6):
+        m = n.clone()
+        m[0] = length
+        got = single_gather_decode(Q, pools, torch.where(table < 0, torch.zeros_like(table), table), m)
+        with pytest.raises(RuntimeError, match="length"):
+            ck.device_status()
+        assert torch.equal(got[1], want[1])
+    assert not single_gather_decode(Q, pools, table, torch.zeros_like(n)).any()
+    ck.device_status()
+
+
+# --------------------------------------------------------------------------- eviction
+
+@pytest.mark.parametrize("lengths,Hkv,D,page,keep,sinks,recent", [
+    ([1], 1, 64, 16, 1, 0, 0),
+    ([0, 5, 100], 2, 128, 16, 40, 4, 10),
+    ([333, 334, 332], 3, 64, 7, 333, 0, 333),
+    ([700, 2, 699], 1, 16, 64, 100, 50, 50),
+    ([1500], 2, 128, 128, 1499, 1, 1),
+    ([3000, 2100, 1025], 1, 32, 32, 1024, 4, 500),
+])
+@pytest.mark.parametrize("masses", ["random", "ties", "odd values"])
+@pytest.mark.parametrize("where", ["in place", "fresh pages", "copy of the table"])
+def test_evict(lengths, Hkv, D, page, keep, sinks, recent, masses, where):
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_evict
+    c = Made(9, lengths, Hkv, D, page)
+    if masses == "ties":
+        c.mass = (c.mass * 4).floor()
+    elif masses == "odd values":
+        odd = torch.tensor([0.0, -0.0, -1.0, float("inf"), -float("inf"), float("nan"), 1e-42, 3.0])
+        c.mass = odd[(c.mass * 8).long()]
+    slots = ref.evict(c.mass, c.table, lengths, keep, sinks, recent)
+    out = c.table
+    if where == "fresh pages":
+        per = -(-min(keep, c.table.shape[1] * page) // page)
+        base = c.pools[0].shape[0]
+        out = (base + torch.randperm(c.B * per, generator=c.g)).int().view(c.B, per)
+        c.pools = [torch.cat([p, rand(c.g, c.B * per, *p.shape[1:])]) for p in c.pools]
+        c.mass = torch.cat([c.mass, torch.rand(c.B * per, page, Hkv, generator=c.g)])
+    want, wmass = [p.clone() for p in c.pools], c.mass.clone()
+    for b in range(c.B):
+        for h in range(Hkv):
+            for r, e in enumerate(slots[b][h]):
+                to, frm = (int(out[b, r // page]), r % page, h), (int(c.table[b, e // page]), e % page, h)
+                for w, p in zip(want, c.pools):
+                    w[to] = p[frm]
+                wmass[to] = c.mass[frm]
+    pools, table, n = c.gpu()
+    mass = c.mass.cuda()
+    to = None if where == "in place" else out.cuda() if where == "fresh pages" else table.clone()
+    kept, left = gather_cache_evict(pools, mass, table, n, keep, sinks=sinks, recent=recent, out_table=to)
+    ck.device_status()
+    assert left.tolist() == [min(k, keep) for k in lengths]
+    for b in range(c.B):
+        for h in range(Hkv):
+            assert kept[b, h].tolist() == slots[b][h] + [-1] * (keep - len(slots[b][h]))
+    for p, w in zip(pools, want):
+        assert torch.equal(p.cpu(), w)
+    assert torch.equal(mass.cpu().view(torch.int32), wmass.view(torch.int32))
+
+
+def test_evict_long_sequence_reads_the_mass_again():
+    """More slots than the keys' shared memory holds."""
+    from att3ntion_b200 import gather_cache_evict
+    n, keep, page = 60001, 777, 128
+    c = Made(10, [n], 1, 16, page)
+    c.mass = (c.mass * 1000).floor()
+    pools, table, length = c.gpu()
+    kept, left = gather_cache_evict(pools, c.mass.cuda(), table, length, keep, sinks=3, recent=7)
+    m = ref.rows_of(c.mass, c.table, 0, list(range(n)))[:, 0].double()
+    m[:3] = m[n - 7:] = float("inf")
+    want = m.sort(descending=True, stable=True).indices[:keep].sort().values
+    assert torch.equal(kept[0, 0].long().cpu(), want) and left.item() == keep
+
+
+# --------------------------------------------------------------------------- streams, graphs, together
+
+def test_other_stream_and_device_guard():
+    from att3ntion_b200 import norm_rotate, single_gather_decode
+    c = Made(11, [500, 300], 1, 128, 16)
+    Q = rand(c.g, 2, 8, 128).cuda()
+    pools, table, n = c.gpu()
+    x = torch.randn(2, 300, 4, 64, device="cuda")
+    want = single_gather_decode(Q, pools, table, n), norm_rotate(x)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append((single_gather_decode(Q, pools, table, n), norm_rotate(x)))
+    torch.cuda.synchronize()
+    for y, z in got:
+        assert torch.equal(y, want[0]) and torch.equal(z, want[1])
+
+
+def test_captured_step_follows_the_lengths():
+    """Append and decode captured once, replayed while the sequences grow, two graphs in turn."""
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append, rotary_table, single_gather_decode
+    B, Hq, Hkv, D, page = 2, 4, 1, 64, 16
+    c = Made(12, [10, 120], Hkv, D, page, room=40)
+    pools, table, n = c.gpu()
+    twin = [p.clone() for p in pools]
+    rot = rotary_table(200, D).cuda()
+    w = [torch.ones(D, device="cuda")] * 3
+    new = [torch.randn(B, 1, Hkv, D, device="cuda") for _ in range(4)]
+    Q = torch.randn(B, 1, Hq, D, device="cuda")
+    one = torch.ones(B, dtype=torch.int32, device="cuda")
+
+    def step(ps, lengths):
+        q = gather_cache_append(ps, table, lengths, *new, Q=Q, weights=w, table=rot)
+        lengths.add_(one)
+        return single_gather_decode(q[:, 0], ps, table, lengths, window=64, sinks=2)
+
+    m = n.clone()
+    step([p.clone() for p in pools], n.clone())                        # warm-up outside the capture
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            y = step(pools, n)
+        graphs.append((gr, y))
+    for k in range(24):
+        for x in (*new, Q):
+            x.normal_()
+        gr, y = graphs[k % 2]
+        gr.replay()
+        want = step(twin, m)
+        assert torch.equal(y, want) and torch.equal(n, m)
+    for p, t in zip(pools, twin):
+        assert torch.equal(p, t)
+    ck.device_status()
