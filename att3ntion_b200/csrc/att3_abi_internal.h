@@ -42,9 +42,9 @@ private:
 // the runtime (no link-time dependency on the driver library).  Returns ATT3_OK or records the error.
 int make_row_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, const char* who, int box_rows = 1,
                         int pitch_cols = 0);
-// Tensor map over a row-major BF16 matrix [rows, cols] for row gathers: a box is 64 columns of one row, laid out in
-// shared memory with the 128-byte swizzle of the operand tiles.
-int make_gather_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, const char* who);
+// Tensor map over a row-major BF16 matrix [rows, cols] whose box is 64 columns of `box_rows` rows, laid out in shared
+// memory with the 128-byte swizzle of the operand tiles.  box_rows = 1 is the form that row gathers take.
+int make_gather_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, int box_rows, const char* who);
 // The same over a [B,H,N,D] operand in either memory layout (0: [B,H,N,D] -> [B*H*N, D]; 1: [B,N,H,D] -> [B*N, H*D],
 // the head being a column offset of the box): the (x, y) a kernel passes come from sgring::RowAddr::tma.
 int make_head_tensor_map(CUtensorMap* out, const void* base, int B, int H, int N, int D, int bnhd, int box_rows,

@@ -97,12 +97,12 @@ static EncodeFn encode_fn() {
     return encode;
 }
 
-int make_gather_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, const char* who) {
+int make_gather_tensor_map(CUtensorMap* out, const void* base, size_t rows, int cols, int box_rows, const char* who) {
     const EncodeFn encode = encode_fn();
     if (!encode) return set_error(ATT3_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", who);
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
-    const cuuint32_t box[2] = {64, 1}, estr[2] = {1, 1};
+    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)}, estr[2] = {1, 1};
     const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
                               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

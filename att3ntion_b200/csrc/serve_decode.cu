@@ -90,6 +90,16 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     p.Q = static_cast<const __nv_bfloat16*>(Q);
     p.R = static_cast<const __nv_bfloat16*>(R);
     p.Vr = static_cast<const __nv_bfloat16*>(Vr);
+    // boxes of the largest power of two that divides the page, from 8 rows on (below that a box saves nothing over a gather)
+    p.box = static_cast<int>(std::min<int64_t>(pages->page_size & -pages->page_size, serve::DEC_KEYS));
+    if (window > 0 || p.box < 8) p.box = 0;
+    const size_t rows = static_cast<size_t>(pages->pages) * pages->page_size;
+    if (int rc = att3::make_gather_tensor_map(&p.tmS, S, rows, Hkv * D, 1, who)) return rc;
+    if (int rc = att3::make_gather_tensor_map(&p.tmVs, Vs, rows, Hkv * D, 1, who)) return rc;
+    if (p.box) {
+        if (int rc = att3::make_gather_tensor_map(&p.tmS_box, S, rows, Hkv * D, p.box, who)) return rc;
+        if (int rc = att3::make_gather_tensor_map(&p.tmVs_box, Vs, rows, Hkv * D, p.box, who)) return rc;
+    }
     p.Y = static_cast<__nv_bfloat16*>(Y);
     p.mass = mass;
     p.lengths = lengths;
@@ -107,9 +117,6 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     p.col_ref = reinterpret_cast<float*>(ws + lay.col_ref);
     p.lse = reinterpret_cast<float*>(ws + lay.lse);
     if (!(p.status = att3::serve_status_ptr())) return att3::set_error(ATT3_ERR_CUDA, "%s: status word not resolvable", who);
-    const size_t rows = static_cast<size_t>(pages->pages) * pages->page_size;
-    if (int rc = att3::make_gather_tensor_map(&p.tmS, S, rows, Hkv * D, who)) return rc;
-    if (int rc = att3::make_gather_tensor_map(&p.tmVs, Vs, rows, Hkv * D, who)) return rc;
     const long long seen = window > 0 ? std::min<long long>(most, static_cast<long long>(window) + sinks) : most;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (D == 128) return mass ? launch<128, true>(p, lay, seen, st, who) : launch<128, false>(p, lay, seen, st, who);

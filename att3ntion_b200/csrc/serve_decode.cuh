@@ -27,8 +27,12 @@
 // stretch leaves the head; decode_join_kernel brings the partials of a head together in a fixed order.
 //
 // Roles.  Warps 0-3 and 4-7: one half each -- build the two operand tiles of q o R, exponentials, collapse.  Warp 8
-// issues the products, warp 9 gathers S and Vs rows through the page table with TMA row gathers (four rows an
-// instruction) into a ring of stages.  While one half exponentiates, the other half's products run.
+// issues the products, warps 9-11 bring S and Vs rows through the page table into a ring of stages by TMA: whole boxes
+// of a page where every slot is visible (no window, a full key step), else row gathers, four rows an instruction, for
+// which neither the page size nor where a window begins matters.  Issuing is what costs: a tile of 128 rows of 128
+// takes 4200 cycles as row gathers from one warp (62 an instruction), 1700 from three, 930 as boxes of 16 rows and 720
+// as boxes of 64; 16-byte asynchronous copies from three warps took 3000.  While one half exponentiates, the other
+// half's products run.
 #pragma once
 
 #include "att3_abi_internal.h"
@@ -38,13 +42,13 @@
 namespace serve {
 
 using namespace sm100;
-using sgring::pipe_wait;
 using sgring::warp_arrive;
 
 constexpr int DEC_THREADS = 384;
 constexpr int DEC_STRIP = 32;              // rows of a strip
 constexpr int DEC_TILE_STRIPS = 8;
 constexpr int DEC_KEYS = 128;              // keys of a unit of work
+constexpr int DEC_COPY_WARPS = 3;
 
 struct DecodeParams {
     const __nv_bfloat16* Q;                // [B,Hq,D]
@@ -66,7 +70,9 @@ struct DecodeParams {
     long long* unit_base;                  // [B + 1]
     long long* tile_base;                  // [B + 1]
     int* status;
-    CUtensorMap tmS, tmVs;                 // pools as [pages * page_size, Hkv * D], box one row of 64, 128-byte swizzle
+    // pools as [pages * page_size, Hkv * D], 64 columns of one row, or of `box` rows of a page (0: not used)
+    CUtensorMap tmS, tmVs, tmS_box, tmVs_box;
+    int box;
 };
 
 // What one sequence's work looks like.
@@ -160,11 +166,17 @@ enum DecBar { DB_A_FULL0 = 0, DB_A_FULL1, DB_S_FULL0, DB_S_FULL1, DB_P_FULL0, DB
               DB_COL0, DB_COL1,
               DB_KV_FULL0, DB_KV_EMPTY0 = DB_KV_FULL0 + 8, DB_COUNT = DB_KV_EMPTY0 + 8 };
 
+// Four rows (y) of 64 columns from x on, to four consecutive 128-byte lines.
 __device__ __forceinline__ void tma_gather4(void* dst, const void* map, int x, const int (&y)[4], uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
         ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(smem_u32(bar))
         : "memory");
+}
+
+// A bounded wait whose outcome is the whole warp's: no lane goes on into a warp-wide instruction that another has left.
+__device__ __forceinline__ bool pipe_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int code) {
+    return __all_sync(0xFFFFFFFFu, sgring::pipe_wait(bar, parity, fail, code));
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -566,34 +578,48 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             // nothing of this warp's is in flight when the tensor memory is given back
             umma_commit_pred(&bars[DB_DRAIN], issuer);
             pipe_wait(&bars[DB_DRAIN], 0, fail, 7);
-        } else if (warp == 9 && busy) {
+        } else if (warp >= 9 && busy) {
             // ================================================================== rows of S and Vs
+            const int mine = lane * DEC_COPY_WARPS + warp - 9;         // this lane's box, or group of four rows
             int fill = 0;
             bool go = true, ok = true;
 #pragma unroll 1
             while (go && ok) {
 #pragma unroll 1
                 for (int k = w.k0; k < w.k1 && ok; ++k) {
-                    int row[4];
+                    const bool boxes = p.box > 0 && (k + 1) * DEC_KEYS <= w.s.seen;
+                    const int rows = boxes ? p.box : 4;
+                    const bool any = mine * rows < DEC_KEYS;
+                    int row[4] = {0, 0, 0, 0};
+                    if (any) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        // columns behind the last key repeat its row: they are masked, and a finite row stays finite
-                        const int e = min(k * DEC_KEYS + lane * 4 + i, w.s.seen - 1);
-                        row[i] = p.pages.row(w.b, slot_of(p, w.s, e));
-                        if (row[i] < 0) { report(p.status, ST_PAGE); row[i] = 0; }
+                        for (int i = 0; i < 4; ++i) {
+                            if (i > 0 && boxes) break;
+                            // columns behind the last key repeat its row: they are masked, and a finite row stays finite
+                            const int e = min(k * DEC_KEYS + mine * rows + i, w.s.seen - 1);
+                            row[i] = p.pages.row(w.b, slot_of(p, w.s, e));
+                            if (row[i] < 0) { report(p.status, ST_PAGE); row[i] = 0; }
+                        }
                     }
 #pragma unroll 1
                     for (int kind = 0; kind < 2; ++kind, ++fill) {
                         const int st = fill % L::STAGES;
+                        uint64_t* full = &bars[DB_KV_FULL0 + st];
                         if (fill >= L::STAGES) ok = pipe_wait(&bars[DB_KV_EMPTY0 + st], (fill / L::STAGES - 1) & 1, fail, 8);
                         if (!ok) break;
-                        if (lane == 0) mbar_arrive_expect_tx(&bars[DB_KV_FULL0 + st], L::TILE);
+                        // one arrival, of the thread that names the bytes; other warps' bytes may come before it
+                        if (warp == 9 && lane == 0) mbar_arrive_expect_tx(full, L::TILE);
                         __syncwarp();
-                        uint8_t* dst = smem + L::OFF_KV + st * L::TILE + lane * 512;
-                        const void* map = kind ? &p.tmVs : &p.tmS;
+                        if (any) {
+                            uint8_t* dst = smem + L::OFF_KV + st * L::TILE + mine * rows * 128;
 #pragma unroll
-                        for (int h = 0; h < D / 64; ++h)
-                            tma_gather4(dst + h * 128 * 128, map, w.head * D + h * 64, row, &bars[DB_KV_FULL0 + st]);
+                            for (int h = 0; h < D / 64; ++h) {
+                                const int x = w.head * D + h * 64;
+                                if (boxes) tma_load_2d(dst + h * DEC_KEYS * 128, kind ? &p.tmVs_box : &p.tmS_box, x, row[0], full);
+                                else tma_gather4(dst + h * DEC_KEYS * 128, kind ? &p.tmVs : &p.tmS, x, row, full);
+                            }
+                        }
+                        __syncwarp();
                     }
                 }
                 go = go && w.next(p);
