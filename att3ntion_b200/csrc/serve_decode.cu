@@ -24,8 +24,8 @@ Layout layout(int B, int Hq, int Hkv, int D, int window, int sinks, long long ma
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
     o.part = take((static_cast<size_t>(B) * Hq + o.ctas) * 8 * (D + 4) * 4);
-    o.unit_base = take((static_cast<size_t>(B) + 1) * 8);
-    o.tile_base = take((static_cast<size_t>(B) + 1) * 8);
+    o.unit_base = take((static_cast<size_t>(B) + 1) * 4);
+    o.tile_base = take((static_cast<size_t>(B) + 1) * 4);
     if (mass) {
         o.rows = take((static_cast<size_t>(tiles) + o.ctas) * 8 * 32 * 4);
         o.row_ref = take((static_cast<size_t>(tiles) + o.ctas) * 8 * 4);
@@ -83,6 +83,8 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     if (mass && static_cast<long long>(B) * Hkv > 65535)
         return att3::set_error(ATT3_ERR_INVALID, "%s: with masses at most 65535 sequences times key heads, got %lld", who, static_cast<long long>(B) * Hkv);
     const Layout lay = layout(B, Hq, Hkv, D, window, sinks, most, mass != nullptr);
+    if (lay.units > 0x7FFFFFFFll)
+        return att3::set_error(ATT3_ERR_INVALID, "%s: the table's width, sequences and heads admit more than 2^31 - 1 units of work", who);
     if (!workspace || workspace_bytes < lay.bytes || reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
         return att3::set_error(ATT3_ERR_WORKSPACE, "%s: a 256-byte aligned workspace of %zu bytes is needed", who, lay.bytes);
     if (!att3::require_sm100(who)) return ATT3_ERR_UNSUPPORTED;
@@ -109,8 +111,8 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     p.c2 = sgring::LOG2E / std::sqrt(static_cast<float>(D));
     char* ws = static_cast<char*>(workspace);
     p.part = reinterpret_cast<float*>(ws + lay.part);
-    p.unit_base = reinterpret_cast<long long*>(ws + lay.unit_base);
-    p.tile_base = reinterpret_cast<long long*>(ws + lay.tile_base);
+    p.unit_base = reinterpret_cast<int*>(ws + lay.unit_base);
+    p.tile_base = reinterpret_cast<int*>(ws + lay.tile_base);
     p.rows = reinterpret_cast<float*>(ws + lay.rows);
     p.row_ref = reinterpret_cast<float*>(ws + lay.row_ref);
     p.cols = reinterpret_cast<float*>(ws + lay.cols);

@@ -67,8 +67,8 @@ struct DecodeParams {
     float* cols;                           // mass: [unit][2 halves][128] column sums
     float* col_ref;                        // mass: [unit][2]
     float* lse;                            // mass: [B,Hq] log2 of the softmax sum
-    long long* unit_base;                  // [B + 1]
-    long long* tile_base;                  // [B + 1]
+    int* unit_base;                        // [B + 1]; the host admits no more than 2^31 - 1 units
+    int* tile_base;                        // [B + 1]
     int* status;
     // pools as [pages * page_size, Hkv * D], 64 columns of one row, or of `box` rows of a page (0: not used)
     CUtensorMap tmS, tmVs, tmS_box, tmVs_box;
@@ -79,7 +79,7 @@ struct DecodeParams {
 struct Shape {
     int n, seen, skip;                     // length, visible slots, slots between the sinks and the window
     int per_head, strips, tiles, steps;    // strips of a head, of a key head; its tiles; key steps
-    __device__ __forceinline__ long long units(int Hkv) const { return static_cast<long long>(Hkv) * tiles * steps; }
+    __device__ __forceinline__ int units(int Hkv) const { return Hkv * tiles * steps; }
 };
 
 template <bool MASS>
@@ -101,29 +101,29 @@ __device__ __forceinline__ int slot_of(const DecodeParams& p, const Shape& s, in
 }
 
 // The stretch of CTA c: [total * c / n, total * (c + 1) / n).  The last CTA whose stretch begins at or before `unit`:
-__device__ __forceinline__ int cta_of(long long unit, long long total, int n) {
-    return static_cast<int>(((unit + 1) * n - 1) / total);
+__device__ __forceinline__ int cta_of(int unit, int total, int n) {
+    return static_cast<int>(((static_cast<long long>(unit) + 1) * n - 1) / total);
 }
+__device__ __forceinline__ int stretch(int total, int c, int n) { return static_cast<int>(static_cast<long long>(total) * c / n); }
 
 // A CTA's way along its stretch, one tile's key range at a time; every role walks it by itself.
 template <bool MASS>
 struct Walk {
     Shape s;
     int b, head, tile, k0, k1;             // sequence, key head, tile, key steps [k0, k1)
-    long long left, unit, slot;            // units still to do, of the first step, partial slot
-    __device__ __forceinline__ void start(const DecodeParams& p, int b0, long long off, long long count, long long tile_base,
-                                          long long unit0) {
+    int left, unit, slot;                  // units still to do, of the first step, row sums' slot
+    __device__ __forceinline__ void start(const DecodeParams& p, int b0, int off, int count, int tile_base, int unit0) {
         b = b0;
         s = shape_of<MASS>(p, b);
-        const long long per = static_cast<long long>(s.tiles) * s.steps;
-        head = static_cast<int>(off / per);
-        const long long r = off - head * per;
-        tile = static_cast<int>(r / s.steps);
-        k0 = static_cast<int>(r - static_cast<long long>(tile) * s.steps);
+        const int per = s.tiles * s.steps;
+        head = off / per;
+        const int r = off - head * per;
+        tile = r / s.steps;
+        k0 = r - tile * s.steps;
         left = count;
         unit = unit0;
-        slot = tile_base + static_cast<long long>(head) * s.tiles + tile + blockIdx.x;
-        k1 = static_cast<int>(min(static_cast<long long>(s.steps), k0 + left));
+        slot = tile_base + head * s.tiles + tile + blockIdx.x;
+        k1 = min(s.steps, k0 + left);
     }
     // false when the stretch is done
     __device__ __forceinline__ bool next(const DecodeParams& p) {
@@ -139,7 +139,7 @@ struct Walk {
                 do { ++b; if (b >= p.B) return false; s = shape_of<MASS>(p, b); } while (s.seen == 0);
             }
         }
-        k1 = static_cast<int>(min(static_cast<long long>(s.steps), left));
+        k1 = min(s.steps, left);
         return true;
     }
     // whether a half of the tile holds any strip (with masses: any key)
@@ -147,6 +147,8 @@ struct Walk {
         if (MASS) return tile % (s.per_head / DEC_TILE_STRIPS) * 256 + half * 128 < s.seen;
         return tile * DEC_TILE_STRIPS + half * 4 < s.strips;
     }
+    // columns of key step k in chunks of 32 (the last step's tiles and products are cut to them)
+    __device__ __forceinline__ int chunks(int k) const { return min(4, (s.seen - k * DEC_KEYS + 31) / 32); }
 };
 
 template <int D>
@@ -199,27 +201,27 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_BARS + DB_COUNT * 8);
     volatile int* fail = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* sh_ref = reinterpret_cast<float*>(tmem_slot + 2);                   // [8]
-    long long (*sh_sum)[2] = reinterpret_cast<long long (*)[2]>(smem + L::OFF_SCAN);
-    long long* sh_start = reinterpret_cast<long long*>(smem + L::OFF_SCAN) + 2 * (DEC_THREADS / 32);
-    static_assert((2 * (DEC_THREADS / 32) + 5) * 8 <= 256 && DB_COUNT * 8 + 8 + 32 <= 256, "shared bookkeeping");
+    int (*sh_sum)[2] = reinterpret_cast<int (*)[2]>(smem + L::OFF_SCAN);
+    int* sh_start = reinterpret_cast<int*>(smem + L::OFF_SCAN) + 2 * (DEC_THREADS / 32);
+    static_assert((2 * (DEC_THREADS / 32) + 5) * 4 <= 256 && DB_COUNT * 8 + 8 + 32 <= 256, "shared bookkeeping");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // ---- this CTA's stretch: units and tiles before every sequence, a run of sequences a thread
-    long long total;
+    int total;
     {
         const int per = (p.B + DEC_THREADS - 1) / DEC_THREADS;
         const int lo = min(tid * per, p.B), hi = min(lo + per, p.B);
-        long long units = 0, tiles = 0;
+        int units = 0, tiles = 0;
         for (int b = lo; b < hi; ++b) {
             const Shape s = shape_of<MASS>(p, b, blockIdx.x == 0);
             units += s.units(p.Hkv);
-            tiles += static_cast<long long>(p.Hkv) * s.tiles;
+            tiles += p.Hkv * s.tiles;
         }
-        long long iu = units, it = tiles;
+        int iu = units, it = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long yu = __shfl_up_sync(0xFFFFFFFFu, iu, o), yt = __shfl_up_sync(0xFFFFFFFFu, it, o);
+            const int yu = __shfl_up_sync(0xFFFFFFFFu, iu, o), yt = __shfl_up_sync(0xFFFFFFFFu, it, o);
             if (lane >= o) { iu += yu; it += yt; }
         }
         if (lane == 31) { sh_sum[warp][0] = iu; sh_sum[warp][1] = it; }
@@ -236,8 +238,9 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         }
         if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
         __syncthreads();
-        long long bu = 0, bt = 0, tt = 0;
+        int bu = 0, bt = 0, tt = 0;
         total = 0;
+#pragma unroll
         for (int w = 0; w < DEC_THREADS / 32; ++w) {
             if (w < warp) { bu += sh_sum[w][0]; bt += sh_sum[w][1]; }
             total += sh_sum[w][0];
@@ -245,21 +248,23 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         }
         bu += iu - units;
         bt += it - tiles;
-        const long long begin = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
+        const int begin = stretch(total, blockIdx.x, gridDim.x), end = stretch(total, blockIdx.x + 1, gridDim.x);
         if (blockIdx.x == 0 && tid == 0) { p.unit_base[p.B] = total; p.tile_base[p.B] = tt; }
-        for (int b = lo; b < hi; ++b) {
-            const Shape s = shape_of<MASS>(p, b);
-            const long long u = s.units(p.Hkv);
-            if (blockIdx.x == 0) { p.unit_base[b] = bu; p.tile_base[b] = bt; }
-            if (begin < end && begin >= bu && begin < bu + u) {
-                sh_start[4] = b;
-                sh_start[0] = begin - bu;
-                sh_start[1] = end - begin;
-                sh_start[2] = bt;
-                sh_start[3] = begin;
+        if (blockIdx.x == 0 || (begin < end && begin >= bu && begin < bu + units)) {
+            for (int b = lo; b < hi; ++b) {
+                const Shape s = shape_of<MASS>(p, b);
+                const int u = s.units(p.Hkv);
+                if (blockIdx.x == 0) { p.unit_base[b] = bu; p.tile_base[b] = bt; }
+                if (begin < end && begin >= bu && begin < bu + u) {
+                    sh_start[0] = begin - bu;
+                    sh_start[1] = end - begin;
+                    sh_start[2] = bt;
+                    sh_start[3] = begin;
+                    sh_start[4] = b;
+                }
+                bu += u;
+                bt += p.Hkv * s.tiles;
             }
-            bu += u;
-            bt += static_cast<long long>(p.Hkv) * s.tiles;
         }
         if (tid == 0 && begin >= end) sh_start[4] = -1;
         tc_fence_before();
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
     const uint32_t tmem = *tmem_slot;
     const bool busy = sh_start[4] >= 0;
     Walk<MASS> w;
-    if (busy) w.start(p, static_cast<int>(sh_start[4]), sh_start[0], sh_start[1], sh_start[2], sh_start[3]);
+    if (busy) w.start(p, sh_start[4], sh_start[0], sh_start[1], sh_start[2], sh_start[3]);
 
     if (warp < 8) {
         // ================================================================== builders, exponentials, collapse
@@ -285,6 +290,21 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         // what the warp carries for head `cur`: lane L the columns L, 32 + L, ... of y
         int cur = -1;
         float cm = -INFINITY, cl = 0.f, cy[COLS];
+        // A strip's place in a tile: query head g of the key head, its first key, how many keys it holds; and the lane's
+        // own row of it in the pools (a row on no valid page reads row 0 and is reported).
+        int g = 0, valid = 0, row = 0;
+        auto look = [&](const Walk<MASS>& at) {
+            const int strip = at.tile * DEC_TILE_STRIPS + warp;
+            const bool live = strip < at.s.strips;
+            g = live ? strip / at.s.per_head : 0;
+            const int j0 = live ? (strip - g * at.s.per_head) * DEC_STRIP : 0;
+            valid = live ? max(0, min(DEC_STRIP, at.s.seen - j0)) : 0;
+            row = 0;
+            if (lane < valid) {
+                row = p.pages.row(at.b, slot_of(p, at.s, j0 + lane));
+                if (row < 0) { report(p.status, ST_PAGE); row = 0; }
+            }
+        };
         auto flush = [&]() {
             if (cur < 0) return;
             float* out = p.part + (static_cast<long long>(cur) + blockIdx.x) * DEC_TILE_STRIPS * REC + warp * REC;
@@ -292,35 +312,33 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             for (int c = 0; c < COLS; ++c) out[c * 32 + lane] = cy[c];
             if (lane == 0) { out[D] = cm; out[D + 1] = cl; }
         };
+        while (go && !w.live(half)) go = w.next(p);
+        if (go) look(w);
 #pragma unroll 1
         while (go && ok) {
-            const int strip = w.tile * DEC_TILE_STRIPS + warp;
-            if (!w.live(half)) { go = w.next(p); continue; }
-            const bool live = strip < w.s.strips;
-            const int g = live ? strip / w.s.per_head : 0, j0 = live ? (strip - g * w.s.per_head) * DEC_STRIP : 0;
-            const int valid = live ? max(0, min(DEC_STRIP, w.s.seen - j0)) : 0;     // rows of the strip
-            // the lane's own row of the strip, in the pools (a row on no valid page reads row 0 and is reported)
-            int row = 0;
-            if (lane < valid) {
-                row = p.pages.row(w.b, slot_of(p, w.s, j0 + lane));
-                if (row < 0) { report(p.status, ST_PAGE); row = 0; }
-            }
             // ---- operand tiles: value and residual of q o R
             {
                 const size_t q_at = (static_cast<size_t>(w.b) * p.Hq + w.head * p.G + g) * D + chunk * 8;
                 const uint4 q = *reinterpret_cast<const uint4*>(p.Q + q_at);
-                constexpr int BATCH = PASSES < 8 ? PASSES : 8;
-#pragma unroll
-                for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
-                    uint4 r[BATCH];
+                constexpr int BATCH = 4;                   // passes a turn, the next turn's rows in flight
+                const uint32_t pitch = p.Hkv * D * 2;
+                const char* src = reinterpret_cast<const char*>(p.R + static_cast<size_t>(w.head) * D + chunk * 8);
+                uint4 r[BATCH], next[BATCH];
+                auto fetch = [&](int i0, uint4 (&to)[BATCH]) {
 #pragma unroll
                     for (int i = 0; i < BATCH; ++i) {
                         const int in = (i0 + i) * RPP + sub;
-                        const int from = __shfl_sync(0xFFFFFFFFu, row, in);
-                        r[i] = make_uint4(0, 0, 0, 0);
-                        if (in < valid)
-                            r[i] = __ldg(reinterpret_cast<const uint4*>(p.R + (static_cast<size_t>(from) * p.Hkv + w.head) * D + chunk * 8));
+                        const uint32_t from = __shfl_sync(0xFFFFFFFFu, row, in);
+                        to[i] = make_uint4(0, 0, 0, 0);
+                        if (in < valid) to[i] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<uint64_t>(from) * pitch));
                     }
+                };
+                fetch(0, next);
+#pragma unroll 1
+                for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) r[i] = next[i];
+                    if (i0 + BATCH < PASSES) fetch(i0 + BATCH, next);
 #pragma unroll
                     for (int i = 0; i < BATCH; ++i) {
                         const int in = wq * 32 + (i0 + i) * RPP + sub;
@@ -346,43 +364,40 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 if (!ok) break;
                 tc_fence_after();
                 float col[4] = {0.f, 0.f, 0.f, 0.f};       // with masses: this warp's sums of columns c * 32 + lane
-                if (valid > 0) {
+                // Raises the strip's reference to the maximum over its rows if a row exceeds it by 2^8; what was summed so
+                // far follows.  (The products issued so far are complete: this step's scores came after them.)
+                auto renew = [&](float mx) {
+                    mx = lane < valid ? mx * p.c2 : -INFINITY;
+                    if (k == w.k0) ref = warp_max(mx);
+                    else if (__any_sync(0xFFFFFFFFu, mx > ref + GROW)) {
+                        const float now = warp_max(mx), f = fast_exp2(ref - now);
+                        ref = now;
+                        sum *= f;
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(tO + c * 16, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st16(tO + c * 16, o);
+                        }
+                    }
+                };
+                const uint64_t scale = pair_f32(p.c2, p.c2);
+                if (valid > 0 && w.s.seen - k * DEC_KEYS >= DEC_KEYS) {
+                    // a full step: 128 scores in registers
                     uint32_t x[4][32];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, x[c]);
                     tmem_wait_ld();
-                    const int cols = w.s.seen - k * DEC_KEYS;          // visible columns of this step
-                    if (cols < DEC_KEYS) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (c * 32 + i >= cols) x[c][i] = 0xFF800000u;          // -inf
-                    }
                     float mx = -INFINITY;
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
 #pragma unroll
                         for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[c][i]));
-                    mx = lane < valid ? mx * p.c2 : -INFINITY;
-                    if (k == w.k0) ref = warp_max(mx);
-                    else if (__any_sync(0xFFFFFFFFu, mx > ref + GROW)) {
-                        // the products issued so far are complete (this step's scores came after them)
-                        const float now = warp_max(mx), f = fast_exp2(ref - now);
-                        ref = now;
-                        sum *= f;
-#pragma unroll 1
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(tO + c * 32, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(tO + c * 32, o);
-                        }
-                    }
+                    renew(mx);
                     // rows behind the last key contribute nothing: their exponent is -inf throughout
-                    const uint64_t scale = pair_f32(p.c2, p.c2);
                     const float shift1 = lane < valid ? -ref : -INFINITY;
                     const uint64_t shift = pair_f32(shift1, shift1);
                     uint64_t s0 = pair_f32(0.f, 0.f), s1 = s0;
@@ -407,6 +422,45 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     float a, b;
                     unpair_f32(add_f32x2(s0, s1), a, b);
                     sum += a + b;
+                } else if (valid > 0) {
+                    // the last step: the chunks of 32 columns that hold keys, one after the other.  P of chunk c covers
+                    // score columns 16 c .. 16 c + 15, which are read by then.
+                    const int cols = w.s.seen - k * DEC_KEYS, chunks = w.chunks(k);
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < chunks; ++c) {
+                        uint32_t x[32];
+                        tmem_ld32(tS + c * 32, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, c * 32 + i < cols ? __uint_as_float(x[i]) : -INFINITY);
+                    }
+                    renew(mx);
+                    const float shift1 = lane < valid ? -ref : -INFINITY;
+                    const uint64_t shift = pair_f32(shift1, shift1);
+#pragma unroll 1
+                    for (int c = 0; c < chunks; ++c) {
+                        uint32_t x[32], packed[16];
+                        tmem_ld32(tS + c * 32, x);
+                        tmem_wait_ld();
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            float a, b;
+                            unpair_f32(fma_f32x2(pair_b32(x[i], x[i + 1]), scale, shift), a, b);
+                            v[i] = c * 32 + i < cols ? fast_exp2(a) : 0.f;
+                            v[i + 1] = c * 32 + i + 1 < cols ? fast_exp2(b) : 0.f;
+                            sum += v[i] + v[i + 1];
+                            packed[i / 2] = pack_bf16x2(v[i], v[i + 1]);
+                        }
+                        tmem_st16(tS + c * 16, packed);
+                        if (MASS) {
+                            const float s = sgring::warp_transpose_sum(v, lane);
+                            col[0] = c == 0 ? s : col[0]; col[1] = c == 1 ? s : col[1];
+                            col[2] = c == 2 ? s : col[2]; col[3] = c == 3 ? s : col[3];
+                        }
+                    }
+                    tmem_wait_st();
                 }
                 tc_fence_before();
                 warp_arrive(&bars[DB_P_FULL0 + half], lane);
@@ -436,7 +490,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     ok = pipe_wait(&bars[DB_COL0 + half], cols_phase++ & 1, fail, 11);
                     if (!ok) break;
                     if (wq == 0) {
-                        const long long at = (w.unit + (k - w.k0)) * 2 + half;
+                        const size_t at = (static_cast<size_t>(w.unit) + (k - w.k0)) * 2 + half;
 #pragma unroll
                         for (int c = 0; c < 4; ++c) p.cols[at * 128 + c * 32 + lane] = col[c] + buf[128 + c * 32 + lane];
                         if (lane == 0) p.col_ref[at] = top;
@@ -448,16 +502,23 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             }
             if (!ok) break;
 
-            // ---- collapse: y = sum over the strip's rows of Vr o U
+            // ---- collapse: y = sum over the strip's rows of Vr o U.  The rows of Vr and the next strip's place are
+            // fetched while the products finish.
+            const int head = w.b * p.Hq + w.head * p.G + g, valid_now = valid;
+            const uint4* vr = reinterpret_cast<const uint4*>(p.Vr + (static_cast<size_t>(row) * p.Hkv + w.head) * D);
+            uint4 t[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = __ldg(vr + i);
+            const int rec = w.slot * DEC_TILE_STRIPS + warp;
+            do go = w.next(p); while (go && !w.live(half));
+            if (go) look(w);
             ok = pipe_wait(&bars[DB_O_DONE0 + half], seg & 1, fail, 3);
             if (!ok) break;
             tc_fence_after();
-            if (valid > 0) {
-                const uint4* vr = reinterpret_cast<const uint4*>(p.Vr + (static_cast<size_t>(row) * p.Hkv + w.head) * D);
-                float l = lane < valid ? sum : 0.f;
+            if (valid_now > 0) {
+                float l = lane < valid_now ? sum : 0.f;
 #pragma unroll
                 for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-                const int head = w.b * p.Hq + w.head * p.G + g;
                 if (head != cur) {
                     flush();
                     cur = head;
@@ -469,18 +530,16 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 const float m = fmaxf(cm, ref), f0 = fast_exp2(cm - m), f1 = fast_exp2(ref - m);
                 cm = m;
                 cl = cl * f0 + l * f1;
-#pragma unroll
-                for (int c = 0; c < COLS; ++c) {
+#pragma unroll 1
+                for (int c = 0; c < COLS; ++c) {           // kept as a loop: the instruction cache holds all roles' code
                     uint32_t o[32];
                     tmem_ld32(tO + c * 32, o);
-                    uint4 t[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) t[i] = __ldg(vr + c * 4 + i);
                     tmem_wait_ld();
                     float v[32];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const uint32_t u[4] = {t[i].x, t[i].y, t[i].z, t[i].w};
+                        if (c + 1 < COLS) t[i] = __ldg(vr + (c + 1) * 4 + i);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             const float2 f = unpack_bf16x2(u[q]);
@@ -489,21 +548,21 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                             v[d + 1] = f.y * __uint_as_float(o[d + 1]);
                         }
                     }
-                    if (valid < DEC_STRIP && lane >= valid) {          // rows behind the last key
+                    if (valid_now < DEC_STRIP && lane >= valid_now) {          // rows behind the last key
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = 0.f;
                     }
-                    cy[c] = cy[c] * f0 + sgring::warp_transpose_sum(v, lane) * f1;
+                    const float y = sgring::warp_transpose_sum(v, lane) * f1;
+#pragma unroll
+                    for (int q = 0; q < COLS; ++q) cy[q] = q == c ? cy[q] * f0 + y : cy[q];
                 }
                 if (MASS) {
-                    const long long rec = w.slot * DEC_TILE_STRIPS + warp;
-                    p.rows[rec * DEC_STRIP + lane] = lane < valid ? sum : 0.f;
+                    p.rows[static_cast<size_t>(rec) * DEC_STRIP + lane] = lane < valid_now ? sum : 0.f;
                     if (lane == 0) p.row_ref[rec] = ref;
                 }
             }
             tc_fence_before();
             ++seg;
-            go = w.next(p);
         }
         flush();
     } else {
@@ -511,7 +570,6 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         if (warp == 8 && busy) {
             // ================================================================== products
             const uint32_t issuer = elect_one();
-            const uint32_t idesc_x = make_idesc_bf16(128, 128, 0, 0);
             const uint32_t idesc_u = make_idesc_bf16(128, D, 0, 1);
             int n[2] = {0, 0}, seg[2] = {0, 0};            // steps and segments so far, per half
             int fill = 0;                                  // stages consumed
@@ -520,7 +578,8 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 return make_smem_desc(smem_u32(smem + L::OFF_KV + (f % L::STAGES) * L::TILE), mn ? 128 * 128 : 16, 1024, SWIZZLE_128B);
             };
             auto stage_wait = [&](int f) { return pipe_wait(&bars[DB_KV_FULL0 + f % L::STAGES], (f / L::STAGES) & 1, fail, 4); };
-            auto scores = [&](int t, int f) {
+            auto scores = [&](int t, int f, int chunks) {
+                const uint32_t idesc_x = make_idesc_bf16(128, chunks * 32, 0, 0);
                 const uint64_t b = stage_desc(f, false);
                 const uint32_t tX = tmem + t * 128;
 #pragma unroll
@@ -542,13 +601,14 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     ok = pipe_wait(&bars[DB_A_FULL0 + t], seg[t] & 1, fail, 5);
                     if (!ok) break;
                     tc_fence_after();
-                    scores(t, fill);
+                    scores(t, fill, w.chunks(w.k0));
                 }
                 if (!ok) break;
                 umma_commit_pred(&bars[DB_KV_EMPTY0 + fill % L::STAGES], issuer);
 #pragma unroll 1
                 for (int k = w.k0; k < w.k1 && ok; ++k) {
                     const bool more = k + 1 < w.k1;
+                    const int chunks = w.chunks(k);
                     ok = stage_wait(fill + 1);
                     for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
                         ok = pipe_wait(&bars[DB_P_FULL0 + t], n[t] & 1, fail, 6);
@@ -556,14 +616,21 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                         ++n[t];
                         tc_fence_after();
                         const uint64_t b = stage_desc(fill + 1, true);
-#pragma unroll
-                        for (int kk = 0; kk < 8; ++kk)
+                        auto product = [&](int kk) {
                             umma_ts_pred(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, b + kk * (2048 / 16), idesc_u, k > w.k0 || kk > 0, issuer);
+                        };
+                        if (chunks == 4) {
+#pragma unroll
+                            for (int kk = 0; kk < 8; ++kk) product(kk);
+                        } else {
+#pragma unroll 1
+                            for (int kk = 0; kk < 2 * chunks; ++kk) product(kk);
+                        }
                         if (!more) umma_commit_pred(&bars[DB_O_DONE0 + t], issuer);
                         else {
                             if (t == 0) ok = stage_wait(fill + 2);
                             if (!ok) break;
-                            scores(t, fill + 2);
+                            scores(t, fill + 2, w.chunks(k + 1));
                         }
                     }
                     if (!ok) break;
@@ -589,7 +656,8 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 for (int k = w.k0; k < w.k1 && ok; ++k) {
                     const bool boxes = p.box > 0 && (k + 1) * DEC_KEYS <= w.s.seen;
                     const int rows = boxes ? p.box : 4;
-                    const bool any = mine * rows < DEC_KEYS;
+                    const int wanted = w.chunks(k) * 32;
+                    const bool any = mine * rows < wanted;
                     int row[4] = {0, 0, 0, 0};
                     if (any) {
 #pragma unroll
@@ -608,7 +676,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                         if (fill >= L::STAGES) ok = pipe_wait(&bars[DB_KV_EMPTY0 + st], (fill / L::STAGES - 1) & 1, fail, 8);
                         if (!ok) break;
                         // one arrival, of the thread that names the bytes; other warps' bytes may come before it
-                        if (warp == 9 && lane == 0) mbar_arrive_expect_tx(full, L::TILE);
+                        if (warp == 9 && lane == 0) mbar_arrive_expect_tx(full, wanted * D * 2);
                         __syncwarp();
                         if (any) {
                             uint8_t* dst = smem + L::OFF_KV + st * L::TILE + mine * rows * 128;
@@ -650,19 +718,18 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant_
         if (threadIdx.x < D) y[threadIdx.x] = __float2bfloat16_rn(0.f);
         return;
     }
-    const long long total = p.unit_base[p.B], units0 = p.unit_base[b] + static_cast<long long>(kv) * s.tiles * s.steps;
+    const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const int lo = g * s.per_head, hi = lo + (s.seen + DEC_STRIP - 1) / DEC_STRIP;         // the head's strips with keys
-    const long long u0 = units0 + static_cast<long long>(lo / DEC_TILE_STRIPS) * s.steps;
-    const long long u1 = units0 + static_cast<long long>((hi - 1) / DEC_TILE_STRIPS + 1) * s.steps;
+    const int u0 = units0 + lo / DEC_TILE_STRIPS * s.steps, u1 = units0 + ((hi - 1) / DEC_TILE_STRIPS + 1) * s.steps;
     const int c0 = cta_of(u0, total, ctas), c1 = cta_of(u1 - 1, total, ctas);
     float m = -INFINITY, l = 0.f, acc[COLS];
 #pragma unroll
     for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
     for (int c = c0; c <= c1; ++c) {
         // the tiles of the head that CTA c went through, and whether this warp had a strip of the head in them
-        const long long from = max(total * c / ctas, u0), to = min(total * (c + 1) / ctas, u1);
+        const int from = max(stretch(total, c, ctas), u0), to = min(stretch(total, c + 1, ctas), u1);
         if (from >= to) continue;
-        const int ta = static_cast<int>((from - units0) / s.steps), tb = static_cast<int>((to - 1 - units0) / s.steps);
+        const int ta = (from - units0) / s.steps, tb = (to - 1 - units0) / s.steps;
         int strip = ta * DEC_TILE_STRIPS + warp;
         if (strip < lo) strip += (lo - strip + DEC_TILE_STRIPS - 1) / DEC_TILE_STRIPS * DEC_TILE_STRIPS;
         if (strip >= hi || strip / DEC_TILE_STRIPS > tb) continue;
@@ -701,22 +768,22 @@ __global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant_
     if (e >= s.seen) return;
     const int row = p.pages.row(b, slot_of(p, s, e));
     if (row < 0) return;
-    const long long total = p.unit_base[p.B], units0 = p.unit_base[b] + static_cast<long long>(kv) * s.tiles * s.steps;
-    const long long tiles0 = p.tile_base[b] + static_cast<long long>(kv) * s.tiles;
+    const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
+    const int tiles0 = p.tile_base[b] + kv * s.tiles;
     const int step = e / DEC_KEYS, col = e % DEC_KEYS, per_head = s.per_head / DEC_TILE_STRIPS;
     float share = 0.f;
     for (int g = 0; g < p.G; ++g) {
         const float lse = p.lse[b * p.Hq + kv * p.G + g];
         const int tile = g * per_head + e / 256;
-        const long long u = units0 + static_cast<long long>(tile) * s.steps;
+        const int u = units0 + tile * s.steps;
         const int c0 = cta_of(u, total, ctas), c1 = cta_of(u + s.steps - 1, total, ctas);
         for (int c = c0; c <= c1; ++c) {
-            if (total * c / ctas >= total * (c + 1) / ctas) continue;
-            const long long rec = (tiles0 + tile + c) * DEC_TILE_STRIPS + (e % 256) / DEC_STRIP;
+            if (stretch(total, c, ctas) >= stretch(total, c + 1, ctas)) continue;
+            const size_t rec = static_cast<size_t>(tiles0 + tile + c) * DEC_TILE_STRIPS + (e % 256) / DEC_STRIP;
             share += p.rows[rec * DEC_STRIP + e % DEC_STRIP] * fast_exp2(p.row_ref[rec] - lse);
         }
         for (int t = 0; t < per_head; ++t) {
-            const long long at = (units0 + static_cast<long long>(g * per_head + t) * s.steps + step) * 2;
+            const size_t at = (static_cast<size_t>(units0) + (g * per_head + t) * s.steps + step) * 2;
             share += p.cols[at * 128 + col] * fast_exp2(p.col_ref[at] - lse);
             if (t * 256 + 128 < s.seen) share += p.cols[(at + 1) * 128 + col] * fast_exp2(p.col_ref[at + 1] - lse);
         }
