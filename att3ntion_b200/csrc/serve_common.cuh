@@ -25,9 +25,10 @@ struct Pages {
     int per_seq;      // entries of a sequence's row in the table
     int count;        // pages in the pool
     int size;         // slots in a page
+    int shift;        // its logarithm, or -1 if it is no power of two
     // Row (page * page_size + slot in page) of `slot`, or -1 if the table has no valid page for it.
     __device__ __forceinline__ int row(int b, int slot) const {
-        const unsigned p = static_cast<unsigned>(slot) / static_cast<unsigned>(size);
+        const unsigned p = shift >= 0 ? static_cast<unsigned>(slot) >> shift : static_cast<unsigned>(slot) / static_cast<unsigned>(size);
         if (slot < 0 || p >= static_cast<unsigned>(per_seq)) return -1;
         const int page = __ldg(table + b * stride + p);
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(count)) return -1;
@@ -41,6 +42,13 @@ struct Pages {
         return n < 0 ? 0 : most;
     }
 };
+
+inline Pages make_pages(const int* table, long long stride, long long per_seq, long long count, long long size) {
+    int shift = -1;
+    for (int k = 0; k < 31; ++k)
+        if (size == 1ll << k) shift = k;
+    return Pages{table, stride, static_cast<int>(per_seq), static_cast<int>(count), static_cast<int>(size), shift};
+}
 
 // Eight consecutive elements of a 16-bit or 32-bit type, as FP32.
 template <typename T> struct Eight;

@@ -53,10 +53,23 @@ int launch(const serve::DecodeParams& p, const Layout& lay, long long max_seen, 
     cudaError_t e = cudaFuncSetAttribute(serve::decode_kernel<D, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return att3::set_cuda_error(e, who);
     serve::decode_kernel<D, MASS><<<lay.ctas, serve::DEC_THREADS, smem, st>>>(p);
-    serve::decode_join_kernel<D, MASS><<<p.B * p.Hq, 256, 0, st>>>(p, lay.ctas);
+    // the joining kernels may be set up while the one before them runs out; they wait for its end themselves
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3(p.B * p.Hq);
+    cfg.blockDim = dim3(256);
+    e = cudaLaunchKernelEx(&cfg, serve::decode_join_kernel<D, MASS>, p, lay.ctas);
+    if (e != cudaSuccess) return att3::set_cuda_error(e, who);
     if (MASS) {
-        const dim3 grid(static_cast<unsigned>((max_seen + 127) / 128), p.B * p.Hkv);
-        serve::decode_mass_kernel<<<grid, 128, 0, st>>>(p, lay.ctas);
+        cfg.gridDim = dim3(static_cast<unsigned>((max_seen + 127) / 128), p.B * p.Hkv);
+        cfg.blockDim = dim3(128);
+        e = cudaLaunchKernelEx(&cfg, serve::decode_mass_kernel, p, lay.ctas);
+        if (e != cudaSuccess) return att3::set_cuda_error(e, who);
     }
     e = cudaGetLastError();
     return e == cudaSuccess ? ATT3_OK : att3::set_cuda_error(e, who);
@@ -105,8 +118,7 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     p.Y = static_cast<__nv_bfloat16*>(Y);
     p.mass = mass;
     p.lengths = lengths;
-    p.pages = serve::Pages{pages->table, pages->table_stride, static_cast<int>(pages->per_sequence), static_cast<int>(pages->pages),
-                           static_cast<int>(pages->page_size)};
+    p.pages = serve::make_pages(pages->table, pages->table_stride, pages->per_sequence, pages->pages, pages->page_size);
     p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.window = window; p.sinks = sinks;
     p.c2 = sgring::LOG2E / std::sqrt(static_cast<float>(D));
     char* ws = static_cast<char*>(workspace);

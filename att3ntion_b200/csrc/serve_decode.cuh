@@ -176,6 +176,14 @@ __device__ __forceinline__ void tma_gather4(void* dst, const void* map, int x, c
         : "memory");
 }
 
+// 16 bytes from global to shared memory, asynchronously; a thread's copies complete in groups.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // A bounded wait whose outcome is the whole warp's: no lane goes on into a warp-wide instruction that another has left.
 __device__ __forceinline__ bool pipe_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int code) {
     return __all_sync(0xFFFFFFFFu, sgring::pipe_wait(bar, parity, fail, code));
@@ -312,46 +320,47 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             for (int c = 0; c < COLS; ++c) out[c * 32 + lane] = cy[c];
             if (lane == 0) { out[D] = cm; out[D + 1] = cl; }
         };
+        // The strip's 32 rows of a pool, coalesced, to the warp's own rows of one of the half's operand tiles.  Both tiles
+        // are free between a segment's last score product and the next segment's first: Vr waits in the value tile for
+        // the collapse, the next segment's R in the residual tile for the build, which replaces it in place.
+        const uint32_t tiles_at = smem_u32(tile_hi);
+        auto fetch = [&](const __nv_bfloat16* pool, const Walk<MASS>& at, uint32_t tile, int from_row, int rows) {
+            const char* src = reinterpret_cast<const char*>(pool + static_cast<size_t>(at.head) * D + chunk * 8);
+            const uint32_t pitch = p.Hkv * D * 2;
+#pragma unroll 4
+            for (int i = 0; i < PASSES; ++i) {
+                const int in = i * RPP + sub;
+                const uint32_t from = __shfl_sync(0xFFFFFFFFu, from_row, in);
+                if (in < rows) copy16(tile + sw128_offset<128>(wq * 32 + in, chunk), src + static_cast<uint64_t>(from) * pitch);
+            }
+            copy_commit();
+        };
+        uint4 q = make_uint4(0, 0, 0, 0);
+        auto prepare = [&](const Walk<MASS>& at) {
+            look(at);
+            fetch(p.R, at, tiles_at + L::TILE, row, valid);
+            q = *reinterpret_cast<const uint4*>(p.Q + (static_cast<size_t>(at.b) * p.Hq + at.head * p.G + g) * D + chunk * 8);
+        };
         while (go && !w.live(half)) go = w.next(p);
-        if (go) look(w);
+        if (go) prepare(w);
 #pragma unroll 1
         while (go && ok) {
             // ---- operand tiles: value and residual of q o R
-            {
-                const size_t q_at = (static_cast<size_t>(w.b) * p.Hq + w.head * p.G + g) * D + chunk * 8;
-                const uint4 q = *reinterpret_cast<const uint4*>(p.Q + q_at);
-                constexpr int BATCH = 4;                   // passes a turn, the next turn's rows in flight
-                const uint32_t pitch = p.Hkv * D * 2;
-                const char* src = reinterpret_cast<const char*>(p.R + static_cast<size_t>(w.head) * D + chunk * 8);
-                uint4 r[BATCH], next[BATCH];
-                auto fetch = [&](int i0, uint4 (&to)[BATCH]) {
-#pragma unroll
-                    for (int i = 0; i < BATCH; ++i) {
-                        const int in = (i0 + i) * RPP + sub;
-                        const uint32_t from = __shfl_sync(0xFFFFFFFFu, row, in);
-                        to[i] = make_uint4(0, 0, 0, 0);
-                        if (in < valid) to[i] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<uint64_t>(from) * pitch));
-                    }
-                };
-                fetch(0, next);
-#pragma unroll 1
-                for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
-#pragma unroll
-                    for (int i = 0; i < BATCH; ++i) r[i] = next[i];
-                    if (i0 + BATCH < PASSES) fetch(i0 + BATCH, next);
-#pragma unroll
-                    for (int i = 0; i < BATCH; ++i) {
-                        const int in = wq * 32 + (i0 + i) * RPP + sub;
-                        uint4 hi, lo;
-                        hi.x = mul_bf16x2(q.x, r[i].x); hi.y = mul_bf16x2(q.y, r[i].y);
-                        hi.z = mul_bf16x2(q.z, r[i].z); hi.w = mul_bf16x2(q.w, r[i].w);
-                        lo.x = sgring::mul_residual_bf16x2(q.x, r[i].x, hi.x); lo.y = sgring::mul_residual_bf16x2(q.y, r[i].y, hi.y);
-                        lo.z = sgring::mul_residual_bf16x2(q.z, r[i].z, hi.z); lo.w = sgring::mul_residual_bf16x2(q.w, r[i].w, hi.w);
-                        const uint32_t at = sw128_offset<128>(in, chunk);
-                        st_shared_v4(tile_hi + at, hi.x, hi.y, hi.z, hi.w);
-                        st_shared_v4(tile_hi + L::TILE + at, lo.x, lo.y, lo.z, lo.w);
-                    }
-                }
+            copy_wait<0>();
+            __syncwarp();
+#pragma unroll 4
+            for (int i = 0; i < PASSES; ++i) {
+                const int in = i * RPP + sub;
+                const uint32_t at = sw128_offset<128>(wq * 32 + in, chunk);
+                uint4 r = *reinterpret_cast<const uint4*>(tile_hi + L::TILE + at), hi, lo;
+                if (in >= valid) r = make_uint4(0, 0, 0, 0);
+                hi.x = mul_bf16x2(q.x, r.x); hi.y = mul_bf16x2(q.y, r.y);
+                hi.z = mul_bf16x2(q.z, r.z); hi.w = mul_bf16x2(q.w, r.w);
+                lo.x = sgring::mul_residual_bf16x2(q.x, r.x, hi.x); lo.y = sgring::mul_residual_bf16x2(q.y, r.y, hi.y);
+                lo.z = sgring::mul_residual_bf16x2(q.z, r.z, hi.z); lo.w = sgring::mul_residual_bf16x2(q.w, r.w, hi.w);
+                if (in >= valid) hi = lo = make_uint4(0, 0, 0, 0);
+                st_shared_v4(tile_hi + at, hi.x, hi.y, hi.z, hi.w);
+                st_shared_v4(tile_hi + L::TILE + at, lo.x, lo.y, lo.z, lo.w);
             }
             fence_async_smem();
             warp_arrive(&bars[DB_A_FULL0 + half], lane);
@@ -363,6 +372,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 ok = pipe_wait(&bars[DB_S_FULL0 + half], n & 1, fail, 2);
                 if (!ok) break;
                 tc_fence_after();
+                if (k + 1 == w.k1) fetch(p.Vr, w, tiles_at, row, valid);          // the tiles' last reader is done
                 float col[4] = {0.f, 0.f, 0.f, 0.f};       // with masses: this warp's sums of columns c * 32 + lane
                 // Raises the strip's reference to the maximum over its rows if a row exceeds it by 2^8; what was summed so
                 // far follows.  (The products issued so far are complete: this step's scores came after them.)
@@ -505,13 +515,12 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             // ---- collapse: y = sum over the strip's rows of Vr o U.  The rows of Vr and the next strip's place are
             // fetched while the products finish.
             const int head = w.b * p.Hq + w.head * p.G + g, valid_now = valid;
-            const uint4* vr = reinterpret_cast<const uint4*>(p.Vr + (static_cast<size_t>(row) * p.Hkv + w.head) * D);
-            uint4 t[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = __ldg(vr + i);
             const int rec = w.slot * DEC_TILE_STRIPS + warp;
             do go = w.next(p); while (go && !w.live(half));
-            if (go) look(w);
+            if (go) prepare(w);
+            else copy_commit();                            // an empty group: Vr is the last but one either way
+            copy_wait<1>();
+            __syncwarp();
             ok = pipe_wait(&bars[DB_O_DONE0 + half], seg & 1, fail, 3);
             if (!ok) break;
             tc_fence_after();
@@ -538,8 +547,8 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     float v[32];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t u[4] = {t[i].x, t[i].y, t[i].z, t[i].w};
-                        if (c + 1 < COLS) t[i] = __ldg(vr + (c + 1) * 4 + i);
+                        const uint4 t = *reinterpret_cast<const uint4*>(tile_hi + sw128_offset<128>(wq * 32 + lane, c * 4 + i));
+                        const uint32_t u[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
                             const float2 f = unpack_bf16x2(u[q]);
@@ -564,6 +573,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             tc_fence_before();
             ++seg;
         }
+        copy_wait<0>();
         flush();
     } else {
         sgring::reg_dec<88>();
@@ -704,6 +714,9 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
     if (tid == 0 && *fail) report(p.status, *fail & 0xFF);
 }
 
+// Waits for the kernel before it in the stream, which it may have been started ahead of.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // The partials of one head, CTA by CTA in a fixed order.  Warp w takes what warp w of each CTA wrote, its lanes the
 // columns.
 template <int D, bool MASS>
@@ -715,9 +728,11 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant_
     const Shape s = shape_of<MASS>(p, b);
     __nv_bfloat16* y = p.Y + static_cast<size_t>(blockIdx.x) * D;
     if (s.seen == 0) {
+        wait_for_previous_kernel();
         if (threadIdx.x < D) y[threadIdx.x] = __float2bfloat16_rn(0.f);
         return;
     }
+    wait_for_previous_kernel();
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const int lo = g * s.per_head, hi = lo + (s.seen + DEC_STRIP - 1) / DEC_STRIP;         // the head's strips with keys
     const int u0 = units0 + lo / DEC_TILE_STRIPS * s.steps, u1 = units0 + ((hi - 1) / DEC_TILE_STRIPS + 1) * s.steps;
@@ -768,6 +783,7 @@ __global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant_
     if (e >= s.seen) return;
     const int row = p.pages.row(b, slot_of(p, s, e));
     if (row < 0) return;
+    wait_for_previous_kernel();
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const int tiles0 = p.tile_base[b] + kv * s.tiles;
     const int step = e / DEC_KEYS, col = e % DEC_KEYS, per_head = s.per_head / DEC_TILE_STRIPS;

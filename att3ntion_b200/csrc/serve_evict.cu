@@ -228,8 +228,7 @@ extern "C" int att3_gather_cache_evict(void* R, void* S, void* Vr, void* Vs, flo
     for (int k = 0; k < 4; ++k) p.pool[k] = static_cast<uint4*>(pools[k]);
     p.mass = mass;
     auto view = [](const att3_gather_pages* g) {
-        return serve::Pages{g->table, g->table_stride, static_cast<int>(g->per_sequence), static_cast<int>(g->pages),
-                            static_cast<int>(g->page_size)};
+        return serve::make_pages(g->table, g->table_stride, g->per_sequence, g->pages, g->page_size);
     };
     p.src = view(pages);
     p.dst = view(out);

@@ -527,8 +527,7 @@ extern "C" int att3_gather_cache_append(const att3_head_rows* tensors, int n, in
     }
     if (!att3::require_sm100(who)) return ATT3_ERR_UNSUPPORTED;
     p.positions = positions;
-    p.pages = serve::Pages{pages->table, pages->table_stride, static_cast<int>(pages->per_sequence), static_cast<int>(pages->pages),
-                           static_cast<int>(pages->page_size)};
+    p.pages = serve::make_pages(pages->table, pages->table_stride, pages->per_sequence, pages->pages, pages->page_size);
     p.lengths = lengths;
     p.counts = counts;
     p.mass = mass;
