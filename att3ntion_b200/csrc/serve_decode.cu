@@ -17,8 +17,10 @@ Layout layout(int B, int Hq, int Hkv, int D, int window, int sinks, long long ma
     Layout o = {};
     const long long seen = window > 0 ? std::min<long long>(max_slots, static_cast<long long>(window) + sinks) : max_slots;
     const long long G = Hq / Hkv;
-    const long long per_head = mass ? (seen + 255) / 256 * 8 : (seen + 31) / 32;
-    const long long tiles = static_cast<long long>(B) * Hkv * ((G * per_head + 7) / 8);
+    const long long groups = (seen + 31) / 32;
+    auto block = [&](long long heads) { return (heads * groups + 7) / 8; };          // tiles of a block of heads
+    const long long per_key_head = mass ? G * block(1) : G / 8 * groups + (G & 4 ? block(4) : 0) + (G & 2 ? block(2) : 0) + (G & 1 ? block(1) : 0);
+    const long long tiles = static_cast<long long>(B) * Hkv * per_key_head;
     o.units = tiles * ((seen + 127) / 128);
     o.ctas = static_cast<int>(std::max<long long>(1, std::min<long long>(att3::sm_count(), o.units)));
     size_t at = 0;

@@ -15,10 +15,12 @@
 // pass do not depend on the size of the scores.  P is rounded to BF16 for the second product, as in the prompt's
 // kernels; its sums stay FP32.
 //
-// Strips.  The rows of all query heads of a key head form one list of strips, 32 keys of one head each; a CTA works
-// on tiles of eight strips, two halves of 128 rows with a tensor-memory accumulator each.  A strip is one warp's, so
-// short caches fill a tile with several heads.  A strip's maximum is the warp's: the softmax of a head is joint over
-// all its pairs, so rows far below the strip's maximum may underflow as they would in the end.
+// Strips.  A strip is 32 keys of one query head, and one warp's; a CTA works on tiles of eight strips, two halves of
+// 128 rows with a tensor-memory accumulator each.  The query heads of a key head are taken in blocks of 8, 4, 2 and 1,
+// and a block's strips in the order of their keys, all its heads side by side: a tile of eight heads reads 32 rows of R
+// and Vr once for all of them, a short cache fills its tiles with several heads, and a warp stays with one head through
+// a block.  A strip's maximum is the warp's: the softmax of a head is joint over all its pairs, so rows far below the
+// strip's maximum may underflow as they would in the end.
 //
 // Splits.  The unit of work is (sequence, key head, tile, 128 keys).  All units lie on one line, each CTA takes an
 // equal stretch of it (one CTA an SM), and a stretch may begin and end inside a tile's key loop: any mix of lengths
@@ -75,10 +77,13 @@ struct DecodeParams {
     int box;
 };
 
+// Tiles of a block of `heads` (1, 2, 4 or 8) heads with `groups` strips each.
+__device__ __forceinline__ int block_tiles(int heads, int groups) { return (heads * groups + DEC_TILE_STRIPS - 1) / DEC_TILE_STRIPS; }
+
 // What one sequence's work looks like.
 struct Shape {
     int n, seen, skip;                     // length, visible slots, slots between the sinks and the window
-    int per_head, strips, tiles, steps;    // strips of a head, of a key head; its tiles; key steps
+    int groups, tiles, steps;              // strips of a head; tiles of a key head; key steps
     __device__ __forceinline__ int units(int Hkv) const { return Hkv * tiles * steps; }
 };
 
@@ -88,12 +93,66 @@ __device__ __forceinline__ Shape shape_of(const DecodeParams& p, int b, bool tel
     s.n = p.pages.length(p.lengths, b, p.status, tell);
     s.seen = p.window > 0 ? min(s.n, p.window + p.sinks) : s.n;
     s.skip = s.n - s.seen;
-    // with masses a tile keeps to one head, so that its column sums are one head's
-    s.per_head = MASS ? (s.seen + 255) / 256 * DEC_TILE_STRIPS : (s.seen + DEC_STRIP - 1) / DEC_STRIP;
-    s.strips = p.G * s.per_head;
-    s.tiles = (s.strips + DEC_TILE_STRIPS - 1) / DEC_TILE_STRIPS;
+    s.groups = (s.seen + DEC_STRIP - 1) / DEC_STRIP;
+    if (MASS) s.tiles = p.G * block_tiles(1, s.groups);
+    else s.tiles = p.G / 8 * s.groups + (p.G & 4 ? block_tiles(4, s.groups) : 0) + (p.G & 2 ? block_tiles(2, s.groups) : 0) +
+                   (p.G & 1 ? block_tiles(1, s.groups) : 0);
     s.steps = (s.seen + DEC_KEYS - 1) / DEC_KEYS;
     return s;
+}
+
+// A block of query heads: `heads` of them from g0 on (inside the key head), its tiles from tile0 on.  With masses every
+// block is one head, so that a tile's column sums are one head's.
+struct Block { int g0, log_heads, tile0; };
+
+template <bool MASS>
+__device__ __forceinline__ Block block_of_tile(const DecodeParams& p, const Shape& s, int tile) {
+    if (MASS) {
+        const int per = block_tiles(1, s.groups), g = tile / per;
+        return Block{g, 0, g * per};
+    }
+    const int eights = p.G / 8, whole = eights * s.groups;
+    if (tile < whole) {
+        const int k = eights == 1 ? 0 : tile / s.groups;
+        return Block{8 * k, 3, k * s.groups};
+    }
+    Block k{8 * eights, 2, whole};
+    if (p.G & 4) {
+        const int n = block_tiles(4, s.groups);
+        if (tile < k.tile0 + n) return k;
+        k.g0 += 4;
+        k.tile0 += n;
+    }
+    k.log_heads = 1;
+    if (p.G & 2) {
+        const int n = block_tiles(2, s.groups);
+        if (tile < k.tile0 + n) return k;
+        k.g0 += 2;
+        k.tile0 += n;
+    }
+    k.log_heads = 0;
+    return k;
+}
+
+template <bool MASS>
+__device__ __forceinline__ Block block_of_head(const DecodeParams& p, const Shape& s, int g) {
+    if (MASS) return Block{g, 0, g * block_tiles(1, s.groups)};
+    const int eights = p.G / 8;
+    if (g < 8 * eights) return Block{g & ~7, 3, g / 8 * s.groups};
+    Block k{8 * eights, 2, eights * s.groups};
+    if (p.G & 4) {
+        if (g < k.g0 + 4) return k;
+        k.g0 += 4;
+        k.tile0 += block_tiles(4, s.groups);
+    }
+    k.log_heads = 1;
+    if (p.G & 2) {
+        if (g < k.g0 + 2) return k;
+        k.g0 += 2;
+        k.tile0 += block_tiles(2, s.groups);
+    }
+    k.log_heads = 0;
+    return k;
 }
 
 __device__ __forceinline__ int slot_of(const DecodeParams& p, const Shape& s, int e) {
@@ -142,10 +201,10 @@ struct Walk {
         k1 = min(s.steps, left);
         return true;
     }
-    // whether a half of the tile holds any strip (with masses: any key)
-    __device__ __forceinline__ bool live(int half) const {
-        if (MASS) return tile % (s.per_head / DEC_TILE_STRIPS) * 256 + half * 128 < s.seen;
-        return tile * DEC_TILE_STRIPS + half * 4 < s.strips;
+    // whether a half of the tile holds any key
+    __device__ __forceinline__ bool live(const DecodeParams& p, int half) const {
+        const Block k = block_of_tile<MASS>(p, s, tile);
+        return (((tile - k.tile0) * DEC_TILE_STRIPS + half * 4) >> k.log_heads) < s.groups;
     }
     // columns of key step k in chunks of 32 (the last step's tiles and products are cut to them)
     __device__ __forceinline__ int chunks(int k) const { return min(4, (s.seen - k * DEC_KEYS + 31) / 32); }
@@ -176,9 +235,17 @@ __device__ __forceinline__ void tma_gather4(void* dst, const void* map, int x, c
         : "memory");
 }
 
+// Residual of a packed BF16 product hi = bf16x2(a b): a b - hi has at most 8 significant bits, so the fused
+// multiply-add, which rounds once, gives it exactly.
+__device__ __forceinline__ uint32_t residual_bf16x2(uint32_t a, uint32_t b, uint32_t hi) {
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b),
+                                     __hneg2(*reinterpret_cast<const __nv_bfloat162*>(&hi)));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
 // 16 bytes from global to shared memory, asynchronously; a thread's copies complete in groups.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -187,6 +254,18 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 // A bounded wait whose outcome is the whole warp's: no lane goes on into a warp-wide instruction that another has left.
 __device__ __forceinline__ bool pipe_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int code) {
     return __all_sync(0xFFFFFFFFu, sgring::pipe_wait(bar, parity, fail, code));
+}
+
+// 16 lanes by 32 columns of tensor memory: lane L receives, for k = 0 .. 3, columns 8 k + 2 (L % 4), + 1 of row L / 4 in
+// registers 4 k, 4 k + 1 and of row L / 4 + 8 in 4 k + 2, 4 k + 3.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -295,18 +374,19 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         const int chunk = lane % CH, sub = lane / CH;
         int seg = 0, n = 0, cols_phase = 0;
         bool go = busy, ok = true;
-        // what the warp carries for head `cur`: lane L the columns L, 32 + L, ... of y
+        // What the warp carries for head `cur`: a lane one column of every 32 of y, the column 16 b4 + 8 b3 + b2 + 2 (b1 b0)
+        // of its bits (the order in which the collapse leaves them).
+        const int my_col = (lane & 16) + (lane & 8) + ((lane >> 2) & 1) + 2 * (lane & 3);
         int cur = -1;
         float cm = -INFINITY, cl = 0.f, cy[COLS];
         // A strip's place in a tile: query head g of the key head, its first key, how many keys it holds; and the lane's
         // own row of it in the pools (a row on no valid page reads row 0 and is reported).
         int g = 0, valid = 0, row = 0;
         auto look = [&](const Walk<MASS>& at) {
-            const int strip = at.tile * DEC_TILE_STRIPS + warp;
-            const bool live = strip < at.s.strips;
-            g = live ? strip / at.s.per_head : 0;
-            const int j0 = live ? (strip - g * at.s.per_head) * DEC_STRIP : 0;
-            valid = live ? max(0, min(DEC_STRIP, at.s.seen - j0)) : 0;
+            const Block k = block_of_tile<MASS>(p, at.s, at.tile);
+            const int strip = (at.tile - k.tile0) * DEC_TILE_STRIPS + warp, j0 = (strip >> k.log_heads) * DEC_STRIP;
+            g = k.g0 + (strip & ((1 << k.log_heads) - 1));
+            valid = max(0, min(DEC_STRIP, at.s.seen - j0));
             row = 0;
             if (lane < valid) {
                 row = p.pages.row(at.b, slot_of(p, at.s, j0 + lane));
@@ -317,7 +397,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             if (cur < 0) return;
             float* out = p.part + (static_cast<long long>(cur) + blockIdx.x) * DEC_TILE_STRIPS * REC + warp * REC;
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) out[c * 32 + lane] = cy[c];
+            for (int c = 0; c < COLS; ++c) out[c * 32 + my_col] = cy[c];
             if (lane == 0) { out[D] = cm; out[D + 1] = cl; }
         };
         // The strip's 32 rows of a pool, coalesced, to the warp's own rows of one of the half's operand tiles.  Both tiles
@@ -341,7 +421,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             fetch(p.R, at, tiles_at + L::TILE, row, valid);
             q = *reinterpret_cast<const uint4*>(p.Q + (static_cast<size_t>(at.b) * p.Hq + at.head * p.G + g) * D + chunk * 8);
         };
-        while (go && !w.live(half)) go = w.next(p);
+        while (go && !w.live(p, half)) go = w.next(p);
         if (go) prepare(w);
 #pragma unroll 1
         while (go && ok) {
@@ -356,8 +436,8 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 if (in >= valid) r = make_uint4(0, 0, 0, 0);
                 hi.x = mul_bf16x2(q.x, r.x); hi.y = mul_bf16x2(q.y, r.y);
                 hi.z = mul_bf16x2(q.z, r.z); hi.w = mul_bf16x2(q.w, r.w);
-                lo.x = sgring::mul_residual_bf16x2(q.x, r.x, hi.x); lo.y = sgring::mul_residual_bf16x2(q.y, r.y, hi.y);
-                lo.z = sgring::mul_residual_bf16x2(q.z, r.z, hi.z); lo.w = sgring::mul_residual_bf16x2(q.w, r.w, hi.w);
+                lo.x = residual_bf16x2(q.x, r.x, hi.x); lo.y = residual_bf16x2(q.y, r.y, hi.y);
+                lo.z = residual_bf16x2(q.z, r.z, hi.z); lo.w = residual_bf16x2(q.w, r.w, hi.w);
                 if (in >= valid) hi = lo = make_uint4(0, 0, 0, 0);
                 st_shared_v4(tile_hi + at, hi.x, hi.y, hi.z, hi.w);
                 st_shared_v4(tile_hi + L::TILE + at, lo.x, lo.y, lo.z, lo.w);
@@ -516,7 +596,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             // fetched while the products finish.
             const int head = w.b * p.Hq + w.head * p.G + g, valid_now = valid;
             const int rec = w.slot * DEC_TILE_STRIPS + warp;
-            do go = w.next(p); while (go && !w.live(half));
+            do go = w.next(p); while (go && !w.live(p, half));
             if (go) prepare(w);
             else copy_commit();                            // an empty group: Vr is the last but one either way
             copy_wait<1>();
@@ -539,29 +619,39 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 const float m = fmaxf(cm, ref), f0 = fast_exp2(cm - m), f1 = fast_exp2(ref - m);
                 cm = m;
                 cl = cl * f0 + l * f1;
+                // Lane L holds rows L/4 + 8 i and columns 8 k + 2 (L % 4), + 1 of 32 columns: four rows are added in the lane,
+                // the eight lanes of a column pair by an exchange of halves, after which lane L has column L of the 32.
 #pragma unroll 1
                 for (int c = 0; c < COLS; ++c) {           // kept as a loop: the instruction cache holds all roles' code
-                    uint32_t o[32];
-                    tmem_ld32(tO + c * 32, o);
+                    uint32_t o[2][16];
+                    tmem_ld_16x256b_x4(tO + c * 32, o[0]);
+                    tmem_ld_16x256b_x4(tO + (16u << 16) + c * 32, o[1]);
                     tmem_wait_ld();
-                    float v[32];
+                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint4 t = *reinterpret_cast<const uint4*>(tile_hi + sw128_offset<128>(wq * 32 + lane, c * 4 + i));
-                        const uint32_t u[4] = {t.x, t.y, t.z, t.w};
+                        const int in = (lane >> 2) + 8 * i;
+                        if (in >= valid_now) continue;     // rows behind the last key
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const float2 f = unpack_bf16x2(u[q]);
-                            const int d = i * 8 + q * 2;
-                            v[d] = f.x * __uint_as_float(o[d]);
-                            v[d + 1] = f.y * __uint_as_float(o[d + 1]);
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t u = *reinterpret_cast<const uint32_t*>(tile_hi + sw128_offset<128>(wq * 32 + in, c * 4 + k) + (lane & 3) * 4);
+                            const float2 f = unpack_bf16x2(u);
+                            v[2 * k] += f.x * __uint_as_float(o[i >> 1][k * 4 + (i & 1) * 2]);
+                            v[2 * k + 1] += f.y * __uint_as_float(o[i >> 1][k * 4 + (i & 1) * 2 + 1]);
                         }
                     }
-                    if (valid_now < DEC_STRIP && lane >= valid_now) {          // rows behind the last key
+                    // v[2 k + e]: column 8 k + 2 (lane % 4) + e.  Bits 4, 3, 2 of the lane choose k's bits and e.
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+                    for (int st = 0; st < 3; ++st) {
+                        const int o2 = 16 >> st, keep_n = 4 >> st;
+                        const bool up = (lane & o2) != 0;
+#pragma unroll
+                        for (int k = 0; k < keep_n; ++k) {
+                            const float send = up ? v[k] : v[k + keep_n], mine = up ? v[k + keep_n] : v[k];
+                            v[k] = mine + __shfl_xor_sync(0xFFFFFFFFu, send, o2);
+                        }
                     }
-                    const float y = sgring::warp_transpose_sum(v, lane) * f1;
+                    const float y = v[0] * f1;
 #pragma unroll
                     for (int q = 0; q < COLS; ++q) cy[q] = q == c ? cy[q] * f0 + y : cy[q];
                 }
@@ -605,7 +695,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             };
 #pragma unroll 1
             while (go && ok) {
-                const bool two = w.live(1);
+                const bool two = w.live(p, 1);
                 ok = stage_wait(fill);
                 for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
                     ok = pipe_wait(&bars[DB_A_FULL0 + t], seg[t] & 1, fail, 5);
@@ -717,8 +807,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
 // Waits for the kernel before it in the stream, which it may have been started ahead of.
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// The partials of one head, CTA by CTA in a fixed order.  Warp w takes what warp w of each CTA wrote, its lanes the
-// columns.
+// The partials of one head, shared out over eight warps and added in a fixed order; a warp's lanes take the columns.
 template <int D, bool MASS>
 __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant__ DecodeParams p, int ctas) {
     constexpr int REC = D + 4, COLS = D / 32;
@@ -734,28 +823,30 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant_
     }
     wait_for_previous_kernel();
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
-    const int lo = g * s.per_head, hi = lo + (s.seen + DEC_STRIP - 1) / DEC_STRIP;         // the head's strips with keys
-    const int u0 = units0 + lo / DEC_TILE_STRIPS * s.steps, u1 = units0 + ((hi - 1) / DEC_TILE_STRIPS + 1) * s.steps;
+    const Block k = block_of_head<MASS>(p, s, g);
+    const int u0 = units0 + k.tile0 * s.steps, u1 = u0 + block_tiles(1 << k.log_heads, s.groups) * s.steps;
     const int c0 = cta_of(u0, total, ctas), c1 = cta_of(u1 - 1, total, ctas);
+    // records: of every CTA on the head's tiles, those of the 8 / heads warps that had its strips; shared out over the warps
+    const int log_warps = 3 - k.log_heads, records = (c1 - c0 + 1) << log_warps;
     float m = -INFINITY, l = 0.f, acc[COLS];
 #pragma unroll
     for (int i = 0; i < COLS; ++i) acc[i] = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-        // the tiles of the head that CTA c went through, and whether this warp had a strip of the head in them
+#pragma unroll 2
+    for (int i = warp; i < records; i += 8) {
+        const int c = c0 + (i >> log_warps), from_warp = ((i & ((1 << log_warps) - 1)) << k.log_heads) + g - k.g0;
+        // the first of the head's tiles that CTA c went through, and whether it had keys for that warp
         const int from = max(stretch(total, c, ctas), u0), to = min(stretch(total, c + 1, ctas), u1);
         if (from >= to) continue;
-        const int ta = (from - units0) / s.steps, tb = (to - 1 - units0) / s.steps;
-        int strip = ta * DEC_TILE_STRIPS + warp;
-        if (strip < lo) strip += (lo - strip + DEC_TILE_STRIPS - 1) / DEC_TILE_STRIPS * DEC_TILE_STRIPS;
-        if (strip >= hi || strip / DEC_TILE_STRIPS > tb) continue;
-        const float* r = p.part + (static_cast<long long>(blockIdx.x) + c) * DEC_TILE_STRIPS * REC + warp * REC;
-        const float rm = r[D], top = fmaxf(m, rm), f0 = fast_exp2(m - top), f1 = fast_exp2(rm - top);
+        const int strip = (from - u0) / s.steps * DEC_TILE_STRIPS + from_warp;
+        if (strip >> k.log_heads >= s.groups) continue;
+        const float* r = p.part + (static_cast<long long>(blockIdx.x) + c) * DEC_TILE_STRIPS * REC + from_warp * REC;
+        const float rm = r[D], top = fmaxf(m, rm), f0 = m > -INFINITY ? fast_exp2(m - top) : 0.f, f1 = fast_exp2(rm - top);
         m = top;
         l = l * f0 + r[D + 1] * f1;
 #pragma unroll
         for (int q = 0; q < COLS; ++q) acc[q] = acc[q] * f0 + r[q * 32 + lane] * f1;
     }
-    if (lane == 0) { sh_m[warp] = m; sh_l[warp] = l; }
+    if (lane == 0) { sh_m[warp] = m; sh_l[warp] = l; }            // a warp without records leaves -inf, 0 and zeros
 #pragma unroll
     for (int q = 0; q < COLS; ++q) sh_y[warp][q * 32 + lane] = acc[q];
     __syncthreads();
@@ -786,7 +877,7 @@ __global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant_
     wait_for_previous_kernel();
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const int tiles0 = p.tile_base[b] + kv * s.tiles;
-    const int step = e / DEC_KEYS, col = e % DEC_KEYS, per_head = s.per_head / DEC_TILE_STRIPS;
+    const int step = e / DEC_KEYS, col = e % DEC_KEYS, per_head = block_tiles(1, s.groups);
     float share = 0.f;
     for (int g = 0; g < p.G; ++g) {
         const float lse = p.lse[b * p.Hq + kv * p.G + g];
