@@ -14,25 +14,28 @@ import torch
 
 from . import _cuda_kernels as _ck
 from ._cabi import lib
-from ._norm_rotate import (_NO_STRIDES, _TYPE, _check_heads, _check_table, _descriptors, _head_rows, _on_gpu, _scale,
-                           rotary_table)
+from ._norm_rotate import _TYPE, _check_heads, _check_table, _forward_descriptors, _head_rows, _on_gpu, _scale
 
 _BF16 = torch.bfloat16
 _POOLS = ("R", "S", "Vr", "Vs")
 
 
+_NEW = ("R", "S", "Vr", "Vs", "Q")
+_NONE = (0, 0, 0)
+
+
 def _check_pools(who, pools):
-    pools = tuple(pools)
     if len(pools) != 4:
         raise RuntimeError(f"{who}: pools are the four tensors R, S, Vr, Vs, got {len(pools)}")
+    first = pools[0]
     for name, p in zip(_POOLS, pools):
         if not isinstance(p, torch.Tensor) or p.dim() != 4 or p.dtype != _BF16 or not p.is_contiguous():
             raise RuntimeError(f"{who}: pool {name} must be a contiguous bf16 [pages,page_size,Hkv,D] tensor")
-        if p.shape != pools[0].shape or p.device != pools[0].device:
+        if p.shape != first.shape or p.device != first.device:
             raise RuntimeError(f"{who}: the pools must share one shape and device")
-        if p.numel() == 0:
-            raise RuntimeError(f"{who}: pool {name} is empty")
-    return pools
+    if first.numel() == 0:
+        raise RuntimeError(f"{who}: the pools are empty")
+    return first
 
 
 def _check_table_of_pages(who, page_table, lengths, device, name="page_table", B=None):
@@ -81,40 +84,41 @@ def gather_cache_append(pools, page_table, lengths, R, S, Vr, Vs, *, counts=None
     No two sequences may write the same slot of a page.  A slot behind the page table's end, or on a page that the pool
     does not have, is left out and reported by `device_status()`."""
     who = "gather_cache_append"
-    pools = _check_pools(who, pools)
-    new = (R, S, Vr, Vs) + ((Q,) if Q is not None else ())
-    B, T, D = _check_heads(who, new, ("R", "S", "Vr", "Vs", "Q"))
-    dev = pools[0].device
-    if R.device != dev or D != pools[0].shape[3] or any(x.shape[2] != pools[0].shape[2] for x in new[:4]):
-        raise RuntimeError(f"{who}: new rows must be [B,T,{pools[0].shape[2]},{pools[0].shape[3]}] on the pools' device")
+    pool = _check_pools(who, pools)
+    new = (R, S, Vr, Vs) if Q is None else (R, S, Vr, Vs, Q)
+    B, T, D = _check_heads(who, new, _NEW)
+    dev = pool.device
+    Hkv = pool.shape[2]
+    if R.device != dev or D != pool.shape[3] or not (R.shape[2] == S.shape[2] == Vr.shape[2] == Vs.shape[2] == Hkv):
+        raise RuntimeError(f"{who}: new rows must be [B,T,{Hkv},{pool.shape[3]}] on the pools' device")
     _check_table_of_pages(who, page_table, lengths, dev, B=B)
     if counts is not None:
         _check_ints(who, "counts", counts, B, dev)
     if positions is not None:
         _check_ints(who, "positions", positions, B, dev)
-    _check_mass(who, mass, pools[0])
+    _check_mass(who, mass, pool)
     ws = (None,) * 3 if weights is None else tuple(weights)
     if len(ws) != 3:
         raise RuntimeError(f"{who}: weights are three scales, of Q, R and S")
     _no_grad(who, *new, *ws)
     wq, wr, wsc = (_scale(w, who, f"weight {k}", D, dev) for k, w in enumerate(ws))
     table, rows, rot = _check_table(who, table, D, dev)
-    if not float(eps) >= 0:
+    eps = float(eps)
+    if not eps >= 0:
         raise RuntimeError(f"{who}: eps must not be negative, got {eps}")
-    _on_gpu(who, pools[0])
-    new = [_head_rows(x) for x in new]
-    with torch.cuda.device(dev):
-        turn = rot > 0
-        desc = [(x, w, r, pool, _NO_STRIDES, None, None, None)
-                for x, w, r, pool in zip(new[:4], (wr, wsc, None, None), (turn, turn, False, False), pools)]
+    _on_gpu(who, pool)
+    with _ck._on_device(dev):
+        turn = 1 if rot else 0
+        desc = [(_head_rows(R), wr, turn, pools[0], _NONE), (_head_rows(S), wsc, turn, pools[1], _NONE),
+                (_head_rows(Vr), None, 0, pools[2], _NONE), (_head_rows(Vs), None, 0, pools[3], _NONE)]
         out = None
         if Q is not None:
             Hq = Q.shape[2]
             out = torch.empty((B, T, Hq, D), dtype=_BF16, device=dev)
-            desc.append((new[4], wq, turn, out, (T * Hq * D, Hq * D, D), None, None, None))
-        _ck._call(lib.att3_gather_cache_append, _descriptors(desc), len(desc), _TYPE[R.dtype], _ck._ptr(table), rows, rot,
-                  int(interleaved), _ck._ptr(positions), _pages(page_table, pools[0]), lengths.data_ptr(),
-                  _ck._ptr(counts), _ck._ptr(mass), B, T, D, float(eps), _ck._stream(pools[0]))
+            desc.append((_head_rows(Q), wq, turn, out, (T * Hq * D, Hq * D, D)))
+        _ck._call(lib.att3_gather_cache_append, _forward_descriptors(desc), len(desc), _TYPE[R.dtype], _ck._ptr(table), rows, rot,
+                  1 if interleaved else 0, _ck._ptr(positions), _pages(page_table, pool), lengths.data_ptr(),
+                  _ck._ptr(counts), _ck._ptr(mass), B, T, D, eps, _ck._raw_stream(dev))
     return out
 
 
@@ -131,8 +135,7 @@ def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, ma
     key head's query heads of half the probability of the pairs that hold the slot as j plus half of those that hold it
     as k, 1 in all for every sequence and key head.  No two sequences of a call with masses may share a page."""
     who = "single_gather_decode"
-    pools = _check_pools(who, pools)
-    pool = pools[0]
+    pool = _check_pools(who, pools)
     if not isinstance(Q, torch.Tensor) or Q.dim() != 3 or not Q.is_floating_point():
         raise RuntimeError(f"{who}: Q must be a [B,Hq,D] tensor")
     B, Hq, D = Q.shape
@@ -159,7 +162,7 @@ def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, ma
     q = Q.to(_BF16).contiguous()
     if q.data_ptr() % 16:
         q = q.clone()
-    with torch.cuda.device(Q.device):
+    with _ck._on_device(Q.device):
         y = torch.empty((B, Hq, D), dtype=_BF16, device=Q.device)
         if B == 0:
             return y.to(Q.dtype)
@@ -168,7 +171,7 @@ def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, ma
         ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
         _ck._call(lib.att3_sg_decode, q.data_ptr(), *(p.data_ptr() for p in pools), _ck._ptr(mass), y.data_ptr(),
                   _pages(page_table, pool), lengths.data_ptr(), B, Hq, Hkv, D, window, sinks, ws.data_ptr(), nbytes,
-                  _ck._stream(Q))
+                  _ck._raw_stream(Q.device))
     return y.to(Q.dtype)
 
 
@@ -181,8 +184,7 @@ def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recen
 
     Returns (kept int32 [B,Hkv,keep], the slots that stayed, -1 behind the last; new lengths int32 [B])."""
     who = "gather_cache_evict"
-    pools = _check_pools(who, pools)
-    pool = pools[0]
+    pool = _check_pools(who, pools)
     Hkv, D = pool.shape[2:]
     if D not in (16, 32, 64, 128):
         raise RuntimeError(f"{who}: head dim must be 16, 32, 64 or 128, got {D}")
@@ -200,11 +202,11 @@ def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recen
         if out_table.shape[1] * pool.shape[1] < min(keep, slots):
             raise RuntimeError(f"{who}: out_table has no room for {min(keep, slots)} slots")
     _on_gpu(who, pool)
-    with torch.cuda.device(pool.device):
+    with _ck._on_device(pool.device):
         kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=pool.device)
         left = torch.empty(B, dtype=torch.int32, device=pool.device)
         if B:
             _ck._call(lib.att3_gather_cache_evict, *(p.data_ptr() for p in pools), mass.data_ptr(), _pages(page_table, pool),
                       _pages(out_table if out_table is not None else page_table, pool), lengths.data_ptr(), left.data_ptr(),
-                      kept.data_ptr(), B, Hkv, D, keep, sinks, recent, _ck._stream(pool))
+                      kept.data_ptr(), B, Hkv, D, keep, sinks, recent, _ck._raw_stream(pool.device))
     return kept, left

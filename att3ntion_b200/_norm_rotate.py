@@ -17,7 +17,6 @@ from . import _cuda_kernels as _ck
 from ._cabi import lib
 
 _TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_NO_STRIDES = (0, 0, 0)
 _HEAD_DIMS = (16, 32, 64, 128)
 
 
@@ -33,46 +32,53 @@ def rotary_table(length: int, dim: int, base: float = 10000.0, device=None) -> t
 
 def _head_rows(t: torch.Tensor) -> torch.Tensor:
     """`t` [B,N,H,D] if the kernels can read its rows where they lie (16-byte aligned, contiguous), else a copy."""
-    step = 16 // t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % step == 0 for n, s in zip(t.shape[:3], t.stride()) if n > 1):
-        return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():                            # D is a multiple of 16: every row is aligned
+            return t
+        step = 16 // t.element_size()
+        if t.stride(3) == 1 and all(s % step == 0 for n, s in zip(t.shape[:3], t.stride()) if n > 1):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor):
-    # a dimension of one entry may carry any stride
-    return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()))
+    a, b, c, _ = t.stride()
+    return a, b, c
 
 
 def _scale(w, who: str, name: str, D: int, device):
     if w is None:
         return None
-    if not isinstance(w, torch.Tensor) or w.shape != (D,) or w.dtype not in _TYPE:
+    if not isinstance(w, torch.Tensor) or w.dim() != 1 or w.shape[0] != D or w.dtype not in _TYPE:
         raise RuntimeError(f"{who}: {name} must be a [{D}] tensor of bf16, fp16 or fp32")
     if w.device != device:
         raise RuntimeError(f"{who}: {name} must be on the inputs' device")
-    w = w.detach()
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.detach().clone(memory_format=torch.contiguous_format)
 
 
 def _check_heads(who: str, xs, names):
     """Common shape contract of [B,N,heads,D] tensors; returns (B, N, D)."""
     x0 = xs[0]
+    if not isinstance(x0, torch.Tensor) or x0.dim() != 4:
+        raise RuntimeError(f"{who}: {names[0]} must be a [B,N,heads,D] tensor")
+    B, N, _, D = x0.shape
+    dtype, dev = x0.dtype, x0.device
     for name, x in zip(names, xs):
         if not isinstance(x, torch.Tensor) or x.dim() != 4:
             raise RuntimeError(f"{who}: {name} must be a [B,N,heads,D] tensor")
-        if x.dtype not in _TYPE or x.dtype != x0.dtype:
+        if x.dtype != dtype or dtype not in _TYPE:
             raise RuntimeError(f"{who}: all inputs must share one type of bf16, fp16 and fp32")
-        if x.shape[:2] != x0.shape[:2] or x.shape[3] != x0.shape[3]:
+        b, n, h, d = x.shape
+        if b != B or n != N or d != D:
             raise RuntimeError(f"{who}: {name} is {tuple(x.shape)}, expected batch, length and head dim of {names[0]} "
                                f"{tuple(x0.shape)}")
-        if x.device != x0.device:
+        if x.device != dev:
             raise RuntimeError(f"{who}: all inputs must be on one device")
-        if x.shape[2] < 1:
+        if h < 1:
             raise RuntimeError(f"{who}: {name} has no heads")
-    if x0.shape[3] not in _HEAD_DIMS:
-        raise RuntimeError(f"{who}: head dim must be 16, 32, 64 or 128, got {x0.shape[3]}")
-    return x0.shape[0], x0.shape[1], x0.shape[3]
+    if D not in _HEAD_DIMS:
+        raise RuntimeError(f"{who}: head dim must be 16, 32, 64 or 128, got {D}")
+    return B, N, D
 
 
 def _check_table(who: str, table, D: int, device):
@@ -101,8 +107,8 @@ def _check_positions(who: str, positions, B: int, N: int, device):
         raise RuntimeError(f"{who}: positions must be [{N}] or [{B},{N}], got {tuple(positions.shape)}")
     if positions.device != device:
         raise RuntimeError(f"{who}: positions must be on the inputs' device")
-    p = positions.expand(B, N)
-    return positions, positions.element_size(), p.stride(0), p.stride(1)
+    along = positions.stride(-1) if N > 1 else 0
+    return positions, positions.element_size(), positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0, along
 
 
 def _on_gpu(who: str, t: torch.Tensor) -> None:
@@ -110,39 +116,42 @@ def _on_gpu(who: str, t: torch.Tensor) -> None:
         raise RuntimeError(f"{who}: inputs must be CUDA tensors")
 
 
-def _descriptors(rows):
-    """att3_head_rows array from (x, w, rotate, y, y strides, dy, dx, dw) per tensor."""
+_ZEROS = (0,) * 9
+_NAMES = tuple(f"input {k}" for k in range(5))
+
+
+def _forward_descriptors(rows):
+    """att3_head_rows array from (x, w, rotate, y, y strides) per tensor."""
     words = []
-    for x, w, rotate, y, y_strides, dy, dx, dw in rows:
-        words.append(x.data_ptr() if x is not None else 0)
-        words += _strides(x) if x is not None else _NO_STRIDES
-        words += (w.data_ptr(), _TYPE[w.dtype]) if w is not None else (0, 0)
-        words.append(1 if rotate else 0)
-        words.append(y.data_ptr() if y is not None else 0)
-        words += y_strides
-        words.append(dy.data_ptr() if dy is not None else 0)
-        words += _strides(dy) if dy is not None else _NO_STRIDES
-        words.append(dx.data_ptr() if dx is not None else 0)
-        words += _strides(dx) if dx is not None else _NO_STRIDES
-        words.append(dw.data_ptr() if dw is not None else 0)
-        words.append((x if x is not None else dx).shape[2])
+    for x, w, rotate, y, y_strides in rows:
+        words += (x.data_ptr(), *_strides(x), w.data_ptr() if w is not None else 0, _TYPE[w.dtype] if w is not None else 0,
+                  rotate, y.data_ptr(), *y_strides, *_ZEROS, x.shape[2])
+    return (C.c_int64 * len(words))(*words)
+
+
+def _backward_descriptors(rows):
+    """The same from (x, w, dy, dx, dw)."""
+    words = []
+    for x, w, dy, dx, dw in rows:
+        words += (x.data_ptr(), *_strides(x), w.data_ptr() if w is not None else 0, _TYPE[w.dtype] if w is not None else 0,
+                  1, 0, 0, 0, 0, dy.data_ptr(), *_strides(dy), dx.data_ptr(), *_strides(dx),
+                  dw.data_ptr() if dw is not None else 0, x.shape[2])
     return (C.c_int64 * len(words))(*words)
 
 
 def _forward(xs, ws, table, positions, eps, interleaved, heads_first):
     who = "norm_rotate"
-    B, N, D = _check_heads(who, xs, [f"input {k}" for k in range(len(xs))])
-    dev = xs[0].device
-    ws = [_scale(w, who, f"weight {k}", D, dev) for k, w in enumerate(ws)]
+    B, N, D = _check_heads(who, xs, _NAMES)
+    dev, dtype = xs[0].device, xs[0].dtype
+    ws = [_scale(w, who, f"weight {k}", D, dev) if w is not None else None for k, w in enumerate(ws)]
     table, rows, rot = _check_table(who, table, D, dev)
     positions, pos_bytes, pos_b, pos_n = _check_positions(who, positions, B, N, dev)
     if positions is None and table is not None and N > rows:
         raise RuntimeError(f"{who}: {N} positions and a table of {rows}")
-    if not float(eps) >= 0:
+    if not eps >= 0:
         raise RuntimeError(f"{who}: eps must not be negative, got {eps}")
     _on_gpu(who, xs[0])
-    xs = [_head_rows(x.detach()) for x in xs]
-    with torch.cuda.device(dev):
+    with _ck._on_device(dev):
         ys, desc = [], []
         for x, w in zip(xs, ws):
             H = x.shape[2]
@@ -153,9 +162,9 @@ def _forward(xs, ws, table, positions, eps, interleaved, heads_first):
                 y = torch.empty((B, N, H, D), dtype=torch.bfloat16, device=dev)
                 strides = (N * H * D, H * D, D)
             ys.append(y)
-            desc.append((x, w, True, y, strides, None, None, None))
-        _ck._call(lib.att3_norm_rotate_forward, _descriptors(desc), len(xs), _TYPE[xs[0].dtype], _ck._ptr(table), rows, rot,
-                  int(interleaved), _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, float(eps), _ck._stream(xs[0]))
+            desc.append((_head_rows(x), w, 1, y, strides))
+        _ck._call(lib.att3_norm_rotate_forward, _forward_descriptors(desc), len(xs), _TYPE[dtype], _ck._ptr(table), rows, rot,
+                  interleaved, _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, eps, _ck._raw_stream(dev))
     return ys
 
 
@@ -179,22 +188,24 @@ class _NormRotateFn(Function):
         scales = [_scale(w, who, "weight", D, dev) for w in ws]
         table, rows, rot = _check_table(who, table, D, dev)
         positions, pos_bytes, pos_b, pos_n = _check_positions(who, positions, B, N, dev)
-        with torch.cuda.device(dev):
+        with _ck._on_device(dev):
+            # the scales' gradients and this call's scratch; a captured graph keeps them in its own pool
+            nbytes = lib.att3_norm_rotate_workspace_bytes(ctx.n, D)
+            sums = torch.empty(ctx.n * D + nbytes // 4, dtype=torch.float32, device=dev)
             desc, dxs, dws = [], [], []
-            for x, w, dy in zip(xs, scales, dys):
+            for k, (x, w, dy) in enumerate(zip(xs, scales, dys)):
                 dy = _head_rows(dy.transpose(1, 2) if ctx.heads_first else dy)
+                x = _head_rows(x)
                 dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-                dw = torch.empty(D, dtype=torch.float32, device=dev) if w is not None else None
-                desc.append((_head_rows(x.detach()), w, True, None, _NO_STRIDES, dy, dx, dw))
+                dw = sums[k * D: k * D + D] if w is not None else None
+                desc.append((x, w, dy, dx, dw))
                 dxs.append(dx)
                 dws.append(dw)
-            nbytes = lib.att3_norm_rotate_workspace_bytes(ctx.n, D)
-            # scratch of this call alone: a captured graph keeps it in its own pool
-            ws_buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            _ck._call(lib.att3_norm_rotate_backward, _descriptors(desc), ctx.n, _TYPE[xs[0].dtype], _ck._ptr(table), rows, rot,
-                      int(ctx.interleaved), _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, float(ctx.eps),
-                      ws_buf.data_ptr(), nbytes, _ck._stream(xs[0]))
-        dws = [None if w is None else dw.to(w.dtype) for w, dw in zip(ws, dws)]
+            _ck._call(lib.att3_norm_rotate_backward, _backward_descriptors(desc), ctx.n, _TYPE[xs[0].dtype], _ck._ptr(table), rows,
+                      rot, ctx.interleaved, _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, ctx.eps,
+                      sums.data_ptr() + ctx.n * D * 4, nbytes, _ck._raw_stream(dev))
+        # a slice of its own for a scale that is kept in FP32 would keep the scratch alive with it
+        dws = [None if w is None else dw.to(w.dtype, copy=True) for w, dw in zip(ws, dws)]
         return (None,) * 6 + (*dxs, *dws)
 
 
@@ -217,6 +228,7 @@ def norm_rotate(xs, weights=None, table=None, positions=None, *, eps=1e-6, inter
     ws = (None,) * len(xs) if weights is None else (weights,) if isinstance(weights, torch.Tensor) else tuple(weights)
     if len(ws) != len(xs):
         raise RuntimeError(f"norm_rotate: {len(xs)} tensors and {len(ws)} weights")
+    eps, interleaved, heads_first = float(eps), int(bool(interleaved)), bool(heads_first)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (*xs, *ws)):
         ys = _NormRotateFn.apply(len(xs), table, positions, eps, interleaved, heads_first, *xs, *ws)
     else:
