@@ -36,14 +36,15 @@ def _head_rows(t: torch.Tensor) -> torch.Tensor:
         if t.is_contiguous():                            # D is a multiple of 16: every row is aligned
             return t
         step = 16 // t.element_size()
-        if t.stride(3) == 1 and all(s % step == 0 for n, s in zip(t.shape[:3], t.stride()) if n > 1):
+        if t.stride(3) == 1 and all(s % step == 0 for n, s in zip(t.shape[:3], t.stride()) if n > 1) and max(_strides(t)[1:]) < 1 << 31:
             return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor):
-    a, b, c, _ = t.stride()
-    return a, b, c
+    # a dimension of one entry may carry any stride
+    (B, N, H, _), (a, b, c, _) = t.shape, t.stride()
+    return a if B > 1 else 0, b if N > 1 else 0, c if H > 1 else 0
 
 
 def _scale(w, who: str, name: str, D: int, device):
@@ -88,8 +89,8 @@ def _check_table(who: str, table, D: int, device):
     if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.float32 or table.shape[0] < 1:
         raise RuntimeError(f"{who}: table must be FP32 [positions, rotated columns] with at least one position")
     rot = table.shape[1]
-    if rot > D or rot < 8 or (rot % 16 and rot != 8):
-        raise RuntimeError(f"{who}: rotated columns must be 8 or a multiple of 16 up to the head dim {D}, got {rot}")
+    if not 8 <= rot <= D or rot % 8:
+        raise RuntimeError(f"{who}: rotated columns must be a multiple of 8 up to the head dim {D}, got {rot}")
     if table.device != device:
         raise RuntimeError(f"{who}: table must be on the inputs' device")
     if not table.is_contiguous() or table.data_ptr() % 16:
@@ -173,7 +174,7 @@ class _NormRotateFn(Function):
     def forward(ctx, n, table, positions, eps, interleaved, heads_first, *tensors):
         xs, ws = tensors[:n], tensors[n:]
         ys = _forward(xs, ws, table, positions, eps, interleaved, heads_first)
-        ctx.save_for_backward(table, positions, *tensors)
+        ctx.save_for_backward(table, positions, *tensors)        # checked by now: the backward takes them as they are
         ctx.n, ctx.eps, ctx.interleaved, ctx.heads_first = n, eps, interleaved, heads_first
         return tuple(ys)
 
@@ -185,27 +186,24 @@ class _NormRotateFn(Function):
         who = "norm_rotate"
         B, N, _, D = xs[0].shape
         dev = xs[0].device
-        scales = [_scale(w, who, "weight", D, dev) for w in ws]
         table, rows, rot = _check_table(who, table, D, dev)
         positions, pos_bytes, pos_b, pos_n = _check_positions(who, positions, B, N, dev)
         with _ck._on_device(dev):
-            # the scales' gradients and this call's scratch; a captured graph keeps them in its own pool
+            # scratch of this call alone: a captured graph keeps it in its own pool
             nbytes = lib.att3_norm_rotate_workspace_bytes(ctx.n, D)
-            sums = torch.empty(ctx.n * D + nbytes // 4, dtype=torch.float32, device=dev)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             desc, dxs, dws = [], [], []
-            for k, (x, w, dy) in enumerate(zip(xs, scales, dys)):
+            for x, w, dy in zip(xs, ws, dys):
                 dy = _head_rows(dy.transpose(1, 2) if ctx.heads_first else dy)
-                x = _head_rows(x)
                 dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-                dw = sums[k * D: k * D + D] if w is not None else None
-                desc.append((x, w, dy, dx, dw))
+                dw = torch.empty(D, dtype=torch.float32, device=dev) if w is not None else None
+                desc.append((_head_rows(x), _scale(w, who, "weight", D, dev), dy, dx, dw))
                 dxs.append(dx)
                 dws.append(dw)
             _ck._call(lib.att3_norm_rotate_backward, _backward_descriptors(desc), ctx.n, _TYPE[xs[0].dtype], _ck._ptr(table), rows,
                       rot, ctx.interleaved, _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, ctx.eps,
-                      sums.data_ptr() + ctx.n * D * 4, nbytes, _ck._raw_stream(dev))
-        # a slice of its own for a scale that is kept in FP32 would keep the scratch alive with it
-        dws = [None if w is None else dw.to(w.dtype, copy=True) for w, dw in zip(ws, dws)]
+                      scratch.data_ptr(), nbytes, _ck._raw_stream(dev))
+        dws = [dw if w is None or w.dtype == torch.float32 else dw.to(w.dtype) for w, dw in zip(ws, dws)]
         return (None,) * 6 + (*dxs, *dws)
 
 
@@ -214,7 +212,7 @@ def norm_rotate(xs, weights=None, table=None, positions=None, *, eps=1e-6, inter
 
     xs: [B,N,heads,D] tensors (heads may differ; any strides) of one type of bf16, fp16 and fp32, D in {16,32,64,128};
     a single tensor is taken too.  weights: a [D] scale or None for each, or None; a tensor without a scale is not
-    normed.  table: FP32 [positions, rot], see `rotary_table`; the first `rot` columns (8 or a multiple of 16) of every
+    normed.  table: FP32 [positions, rot], see `rotary_table`; the first `rot` columns (a multiple of 8) of every
     row are turned by its position's angles, pairing columns (d, d + rot/2), or (2d, 2d + 1) with interleaved=True; None:
     no rotation.  positions: int32 or int64 [N] or [B,N], None for 0 .. N-1.  A position outside the table is read as
     position 0 and reported by `device_status()`.

@@ -50,64 +50,51 @@ inline Pages make_pages(const int* table, long long stride, long long per_seq, l
     return Pages{table, stride, static_cast<int>(per_seq), static_cast<int>(count), static_cast<int>(size), shift};
 }
 
-// Eight consecutive elements of a 16-bit or 32-bit type, as FP32.
-template <typename T> struct Eight;
-template <> struct Eight<__nv_bfloat16> {
-    uint4 v;
-    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    }
-    static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&f)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+// Division of numbers below 2^31 by a divisor known to the host: q = (high word of n * mul, plus n) >> shift
+// (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+struct Divide {
+    unsigned mul, shift;
+    __device__ __forceinline__ int operator()(int n) const {
+        return static_cast<int>((__umulhi(static_cast<unsigned>(n), mul) + static_cast<unsigned>(n)) >> shift);
     }
 };
-template <> struct Eight<__half> {
-    uint4 v;
-    __device__ __forceinline__ void load(const __half* p) { v = *reinterpret_cast<const uint4*>(p); }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            f[2 * i] = t.x;
-            f[2 * i + 1] = t.y;
-        }
-    }
-    static __device__ __forceinline__ void store(__half* p, const float (&f)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+inline Divide make_divide(int by) {
+    unsigned l = 0;
+    while ((1ull << l) < static_cast<unsigned long long>(by)) ++l;
+    return Divide{static_cast<unsigned>(((1ull << 32) * ((1ull << l) - by)) / by + 1), l};
+}
+
+// Four consecutive elements of a 16-bit or 32-bit type, as FP32.
+template <typename T> struct Four {
+    uint2 v;                                     // 16-bit types
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ void get(float* f) const;
+    static __device__ __forceinline__ void store(T* p, const float* f);
 };
-template <> struct Eight<float> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const float* p) {
-        a = *reinterpret_cast<const float4*>(p);
-        b = *reinterpret_cast<const float4*>(p + 4);
-    }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    }
-    static __device__ __forceinline__ void store(float* p, const float (&f)[8]) {
+template <> __device__ __forceinline__ void Four<__nv_bfloat16>::get(float* f) const {
+    f[0] = __uint_as_float(v.x << 16);
+    f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+    f[2] = __uint_as_float(v.y << 16);
+    f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+}
+template <> __device__ __forceinline__ void Four<__nv_bfloat16>::store(__nv_bfloat16* p, const float* f) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+template <> __device__ __forceinline__ void Four<__half>::get(float* f) const {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
+}
+template <> __device__ __forceinline__ void Four<__half>::store(__half* p, const float* f) {
+    const __half2 a = __floats2half2_rn(f[0], f[1]), b = __floats2half2_rn(f[2], f[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+template <> struct Four<float> {
+    float4 v;
+    __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void get(float* f) const { f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w; }
+    static __device__ __forceinline__ void store(float* p, const float* f) {
         *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-        *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
     }
 };
 

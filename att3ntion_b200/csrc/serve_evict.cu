@@ -8,7 +8,8 @@
 // In place, rank r comes from slot s >= r.  A block owns one pool's rows of one (sequence, key head), or a slice of
 // their columns, and goes through the ranks in ascending chunks: all loads of a chunk, a barrier, all stores.  Stores
 // of ranks [a, b) reach slots below b, which later ranks no longer read, so nothing is overwritten early.  The same
-// order serves fresh pages.  Rows that stay where they are cost nothing.
+// order serves fresh pages.  Rows that stay where they are cost nothing.  While a chunk's rows are on their way, the
+// next chunk's places are looked up (kept slot, page, row: three dependent loads), one thread a row.
 //
 // The move is bound by memory traffic (16 D + 4 bytes read and written per kept token and key head).
 #include <algorithm>
@@ -21,8 +22,8 @@ namespace {
 constexpr int SEL_THREADS = 1024;
 constexpr int BINS = 2048;
 constexpr int SEL_SMEM_KEYS = 49152;        // 192 KB of keys; longer sequences read the mass again in every pass
-constexpr int MOVE_THREADS = 512;
-constexpr int MOVE_UNROLL = 8;
+constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_UNROLL = 8;              // 16-byte pieces a thread has in flight
 
 struct Params {
     uint4* pool[4];
@@ -151,39 +152,56 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
 }
 
 // blockIdx.x: (sequence, key head); blockIdx.y: pool * slices + slice, the last one the mass.
-__global__ void __launch_bounds__(MOVE_THREADS) move_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_constant__ Params p) {
+    constexpr int MOST = MOVE_THREADS * MOVE_UNROLL;                   // rows of a chunk: that many of masses, fewer of pools
+    __shared__ int from[2][MOST / 2], to[2][MOST / 2];
     const int h = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
     const int n = p.src.length(p.lengths, b, p.status, false);
     const int left = min(n, p.keep);
     const int* kept = p.kept + static_cast<long long>(blockIdx.x) * p.keep;
     const bool is_mass = static_cast<int>(blockIdx.y) == 4 * p.slices;
-    const int width = is_mass ? 1 : p.row16 / p.slices;                // pieces a row here
+    const int width = is_mass ? 2 : p.row16 / p.slices;                // threads a row (two share a mass: the first moves it)
     const int at = is_mass ? 0 : (blockIdx.y % p.slices) * width + threadIdx.x % width;
-    const int rows = MOVE_THREADS / width, mine = threadIdx.x / width;
+    const int rows = MOVE_THREADS / width, mine = threadIdx.x / width, chunk = rows * MOVE_UNROLL;
+    const bool idle = is_mass && threadIdx.x % width != 0;
     uint4* pool = is_mass ? nullptr : p.pool[blockIdx.y / p.slices];
-    for (int base = 0; base < left; base += rows * MOVE_UNROLL) {
+    // places of a chunk's rows: source row, target row; the source is -1 where nothing moves
+    auto look = [&](int base, int buf) {
+        for (int i = threadIdx.x; i < chunk && base + i < left; i += MOVE_THREADS) {
+            int s = p.src.row(b, __ldg(kept + base + i));
+            const int d = p.dst.row(b, base + i);
+            if (s < 0 || d < 0) { serve::report(p.status, serve::ST_PAGE); s = -1; }
+            from[buf][i] = s == d ? -1 : s;
+            to[buf][i] = d;
+        }
+    };
+    asm volatile("griddepcontrol.wait;" ::: "memory");                 // the kept slots
+    look(0, 0);
+    __syncthreads();
+    int buf = 0;
+    for (int base = 0; base < left; base += chunk, buf ^= 1) {
         uint4 v[MOVE_UNROLL];
-        long long to[MOVE_UNROLL];
 #pragma unroll
         for (int u = 0; u < MOVE_UNROLL; ++u) {
-            const int r = base + u * rows + mine;
-            to[u] = -1;
-            if (r >= left) continue;
-            const int s = p.src.row(b, __ldg(kept + r)), d = p.dst.row(b, r);
-            if (s < 0 || d < 0) { serve::report(p.status, serve::ST_PAGE); continue; }
-            if (s == d) continue;
-            const long long from = static_cast<long long>(s) * p.Hkv + h;
-            to[u] = static_cast<long long>(d) * p.Hkv + h;
-            if (is_mass) v[u].x = __float_as_uint(p.mass[from]);
-            else { v[u] = pool[from * p.row16 + at]; to[u] = to[u] * p.row16 + at; }
+            const int i = u * rows + mine;
+            if (idle || base + i >= left) continue;
+            const int s = from[buf][i];
+            if (s < 0) continue;
+            const long long row = static_cast<long long>(s) * p.Hkv + h;
+            if (is_mass) v[u].x = __float_as_uint(p.mass[row]);
+            else v[u] = pool[row * p.row16 + at];
         }
+        look(base + chunk, buf ^ 1);
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < MOVE_UNROLL; ++u) {
-            if (to[u] < 0) continue;
-            if (is_mass) p.mass[to[u]] = __uint_as_float(v[u].x);
-            else pool[to[u]] = v[u];
+            const int i = u * rows + mine;
+            if (idle || base + i >= left || from[buf][i] < 0) continue;
+            const long long row = static_cast<long long>(to[buf][i]) * p.Hkv + h;
+            if (is_mass) p.mass[row] = __uint_as_float(v[u].x);
+            else pool[row * p.row16 + at] = v[u];
         }
+        __syncthreads();                                               // the buffer is looked up into again
     }
 }
 
@@ -247,7 +265,16 @@ extern "C" int att3_gather_cache_evict(void* R, void* S, void* Vr, void* Vs, flo
     cudaError_t e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_SMEM_KEYS * 4);
     if (e != cudaSuccess) return att3::set_cuda_error(e, who);
     select_kernel<<<B * Hkv, SEL_THREADS, smem, st>>>(p);
-    move_kernel<<<dim3(B * Hkv, 4 * p.slices + 1), MOVE_THREADS, 0, st>>>(p);
-    e = cudaGetLastError();
+    // the second kernel may be set up while the first runs out; it waits for its end itself
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(B * Hkv, 4 * p.slices + 1);
+    cfg.blockDim = dim3(MOVE_THREADS);
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, move_kernel, p);
     return e == cudaSuccess ? ATT3_OK : att3::set_cuda_error(e, who);
 }

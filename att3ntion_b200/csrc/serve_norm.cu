@@ -11,29 +11,31 @@
 // rows are neither.
 //
 // Both directions are bound by memory traffic: a row is read once and written once, everything between stays in
-// registers.  D / 8 neighbouring lanes hold a row (16 bytes a lane and 16-bit element), so the mean is a few shuffles
-// and the rotation's partner one shuffle away.  Such a group takes up to four heads of one token: four loads in
-// flight a lane, and the token's angles are fetched once for them.  All of a call's tensors go in one launch, each
-// with its own range of blocks.  The backward keeps the columns of dw that a lane owns in registers over all rows
-// that it visits; blocks write their sums to a plane each, which a second kernel adds in a fixed order, so that
-// repeated calls agree to the bit.
+// registers.  D / 8 neighbouring lanes hold a row, eight columns a lane.  Which eight follows the rotation: four of the
+// first half of the rotated columns and their four partners, or neighbours; so a lane turns its pairs by itself with
+// four angles, and only the mean needs the row's other lanes.  (Eight neighbouring columns a lane, the partner's fetched
+// by shuffles, took 394 instructions a row and direction and 2.3 TB/s in the backward.)  A group of lanes takes
+// several heads of one token, whose angles are fetched once for them, or the heads of several tokens where there are
+// few.  All of a call's tensors go in one launch, each with its own range of blocks.  The backward keeps the columns of
+// dw that a lane owns in registers over all rows that it visits and has the next rows on their way while it works;
+// blocks write their sums to a plane each, which a second kernel adds in a fixed order, so that repeated calls agree to
+// the bit.
 #include <algorithm>
 
 #include "att3_abi_internal.h"
 #include "serve_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace {
 
-using serve::Eight;
+using serve::Four;
 
 __device__ int g_serve_status = 0;
 
 constexpr int THREADS = 256;
-constexpr int HEADS_PER_ITEM = 4;
+constexpr int FWD_ROWS = 4, BWD_ROWS = 2;           // rows of an item, the unit of work of D / 8 lanes
 constexpr int MAX_TENSORS = 5;
-constexpr int BWD_BLOCKS_PER_SM = 4;
-
-enum RotMode { ROT_NONE = 0, ROT_LANES = 1, ROT_IN_LANE = 2, ROT_NEIGHBOURS = 3 };
+constexpr int FWD_BLOCKS_PER_SM = 16, BWD_BLOCKS_PER_SM = 6;       // at most; a block then takes several items a group
 
 struct Tensor {
     const void* x;
@@ -42,8 +44,12 @@ struct Tensor {
     void* dx;
     const void* w;
     float* dw;
-    long long xs[3], ys[3], dys[3], dxs[3];
-    int w_type, rotate, heads, items, block0, blocks;      // items: groups of up to four heads in a token
+    long long xb, yb, dyb, dxb;                    // strides of the batch, then of the position and the head, in elements
+    int xn, xh, yn, yh, dyn, dyh, dxn, dxh;
+    int w_type, rotate, heads, block0, blocks;
+    int per_token, tokens_per;                     // items of a token, or tokens of an item
+    serve::Divide by_per_token;
+    int items;                                     // in all
 };
 
 struct Params {
@@ -52,8 +58,9 @@ struct Params {
     const float* table;
     const void* positions;
     long long pos_b, pos_n;
-    int pos_bytes, table_rows, rot, mode;
-    int B, N;
+    int pos_bytes, table_rows, rot, interleaved;
+    int B, N, tokens;
+    serve::Divide by_N;
     float eps;
     float* partial;                                // backward: [blocks][D]
     // append
@@ -65,68 +72,81 @@ struct Params {
     int* status;
 };
 
-__device__ __forceinline__ void load_scale(const Tensor& t, int col, float (&w)[8]) {
-    if (t.w_type == 0) { Eight<__nv_bfloat16> v; v.load(static_cast<const __nv_bfloat16*>(t.w) + col); v.get(w); }
-    else if (t.w_type == 1) { Eight<__half> v; v.load(static_cast<const __half*>(t.w) + col); v.get(w); }
-    else { Eight<float> v; v.load(static_cast<const float*>(t.w) + col); v.get(w); }
+// A lane's eight columns: four from `a` on, four from `b` on.  Of the rotated columns lane l has the pairs with the
+// angles 4 l .. 4 l + 3.
+struct Columns { int a, b; bool turns; };
+__device__ __forceinline__ Columns columns_of(const Params& p, int lane_in_row) {
+    const bool turns = lane_in_row * 8 < p.rot;
+    if (turns && !p.interleaved) return Columns{lane_in_row * 4, (p.rot >> 1) + lane_in_row * 4, true};
+    return Columns{lane_in_row * 8, lane_in_row * 8 + 4, turns};
 }
 
-// A lane's eight cosines and signed sines: y'[k] = y[k] c[k] + partner[k] s[k].
-__device__ __forceinline__ void load_angles(const Params& p, int pos, int lane_in_row, float (&c)[8], float (&s)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) { c[k] = 1.f; s[k] = 0.f; }
-    if (p.mode == ROT_NONE || lane_in_row * 8 >= p.rot) return;
-    const int half = p.rot >> 1;
-    const float* row = p.table + static_cast<long long>(pos) * p.rot;
-    if (p.mode == ROT_LANES) {
-        const bool first = lane_in_row * 8 < half;
-        const int at = lane_in_row * 8 - (first ? 0 : half);
-        const float4 c0 = __ldg(reinterpret_cast<const float4*>(row + at)), c1 = __ldg(reinterpret_cast<const float4*>(row + at + 4));
-        const float4 s0 = __ldg(reinterpret_cast<const float4*>(row + half + at)), s1 = __ldg(reinterpret_cast<const float4*>(row + half + at + 4));
-        c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w; c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
-        s[0] = s0.x; s[1] = s0.y; s[2] = s0.z; s[3] = s0.w; s[4] = s1.x; s[5] = s1.y; s[6] = s1.z; s[7] = s1.w;
-        if (first) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) s[k] = -s[k];
-        }
-    } else {
-        // four angles: of the pairs (k, k + 4) of the only rotated lane, or of the neighbours (2k, 2k + 1)
-        const int at = p.mode == ROT_IN_LANE ? 0 : lane_in_row * 4;
-        const float4 c4 = __ldg(reinterpret_cast<const float4*>(row + at));
-        const float4 s4 = __ldg(reinterpret_cast<const float4*>(row + half + at));
-        if (p.mode == ROT_IN_LANE) {
-            c[0] = c[4] = c4.x; c[1] = c[5] = c4.y; c[2] = c[6] = c4.z; c[3] = c[7] = c4.w;
-            s[4] = s4.x; s[5] = s4.y; s[6] = s4.z; s[7] = s4.w;
-            s[0] = -s4.x; s[1] = -s4.y; s[2] = -s4.z; s[3] = -s4.w;
-        } else {
-            c[0] = c[1] = c4.x; c[2] = c[3] = c4.y; c[4] = c[5] = c4.z; c[6] = c[7] = c4.w;
-            s[1] = s4.x; s[3] = s4.y; s[5] = s4.z; s[7] = s4.w;
-            s[0] = -s4.x; s[2] = -s4.y; s[4] = -s4.z; s[6] = -s4.w;
-        }
+template <typename T>
+struct Row8 {
+    Four<T> a, b;
+    __device__ __forceinline__ void load(const T* p, const Columns& c) { a.load(p + c.a); b.load(p + c.b); }
+    __device__ __forceinline__ void get(float (&f)[8]) const { a.get(f); b.get(f + 4); }
+    static __device__ __forceinline__ void store(T* p, const Columns& c, const float (&f)[8]) {
+        Four<T>::store(p + c.a, f);
+        Four<T>::store(p + c.b, f + 4);
     }
+};
+
+__device__ __forceinline__ void load_scale(const Tensor& t, const Columns& c, float (&w)[8]) {
+    if (t.w_type == 0) { Row8<__nv_bfloat16> v; v.load(static_cast<const __nv_bfloat16*>(t.w), c); v.get(w); }
+    else if (t.w_type == 1) { Row8<__half> v; v.load(static_cast<const __half*>(t.w), c); v.get(w); }
+    else { Row8<float> v; v.load(static_cast<const float*>(t.w), c); v.get(w); }
 }
 
-// In place: y c + partner s (sign = 1), or the transposed rotation (sign = -1).  Every lane of the warp calls it.
-template <int LANES>
-__device__ __forceinline__ void rotate(int mode, int rot, int lane_in_row, float (&y)[8], const float (&c)[8],
-                                       const float (&s)[8], float sign) {
-    if (mode == ROT_NONE) return;
-    float o[8];
-    if (mode == ROT_LANES) {
-        const int shift = rot >> 4;                                    // lanes in half of the rotated columns
-        int from = lane_in_row < shift ? lane_in_row + shift : lane_in_row - shift;
-        if (lane_in_row * 8 >= rot) from = lane_in_row;
+// Two FP32 at a time: f[k] * by[k] of eight, and sums of eight products.
+__device__ __forceinline__ void scale8(float (&f)[8], const float (&by)[8]) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = __shfl_sync(0xFFFFFFFFu, y[k], from, LANES);
-    } else if (mode == ROT_IN_LANE) {
+    for (int k = 0; k < 8; k += 2) sm100::unpair_f32(sm100::mul_f32x2(sm100::pair_f32(f[k], f[k + 1]), sm100::pair_f32(by[k], by[k + 1])), f[k], f[k + 1]);
+}
+__device__ __forceinline__ void scale8(float (&f)[8], float by) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = y[k ^ 4];
+    for (int k = 0; k < 8; k += 2) sm100::unpair_f32(sm100::mul_f32x2(sm100::pair_f32(f[k], f[k + 1]), sm100::pair_f32(by, by)), f[k], f[k + 1]);
+}
+__device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
+    uint64_t s = sm100::mul_f32x2(sm100::pair_f32(a[0], a[1]), sm100::pair_f32(b[0], b[1]));
+#pragma unroll
+    for (int k = 2; k < 8; k += 2) s = sm100::fma_f32x2(sm100::pair_f32(a[k], a[k + 1]), sm100::pair_f32(b[k], b[k + 1]), s);
+    float x, y;
+    sm100::unpair_f32(s, x, y);
+    return x + y;
+}
+
+// A lane's four angles (cosines 1, sines 0 where it turns nothing).
+struct Angles { float4 c, s; };
+__device__ __forceinline__ Angles load_angles(const Params& p, int pos, int lane_in_row, bool turns) {
+    Angles t{make_float4(1.f, 1.f, 1.f, 1.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    if (turns) {
+        const float* row = p.table + static_cast<long long>(pos) * p.rot + lane_in_row * 4;
+        t.c = __ldg(reinterpret_cast<const float4*>(row));
+        t.s = __ldg(reinterpret_cast<const float4*>(row + (p.rot >> 1)));
+    }
+    return t;
+}
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+    const float x = a * c - b * s;
+    b = b * c + a * s;
+    a = x;
+}
+// Rot y (sign = 1) or Rot^T y (sign = -1), in place.
+__device__ __forceinline__ void rotate(bool interleaved, float (&y)[8], const Angles& t, float sign) {
+    const float c[4] = {t.c.x, t.c.y, t.c.z, t.c.w}, s[4] = {sign * t.s.x, sign * t.s.y, sign * t.s.z, sign * t.s.w};
+    if (interleaved) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) turn(y[2 * k], y[2 * k + 1], c[k], s[k]);
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = y[k ^ 1];
+        for (int k = 0; k < 4; k += 2) {
+            const uint64_t a = sm100::pair_f32(y[k], y[k + 1]), b = sm100::pair_f32(y[k + 4], y[k + 5]);
+            const uint64_t cc = sm100::pair_f32(c[k], c[k + 1]), ss = sm100::pair_f32(s[k], s[k + 1]), minus = sm100::pair_f32(-s[k], -s[k + 1]);
+            sm100::unpair_f32(sm100::fma_f32x2(b, minus, sm100::mul_f32x2(a, cc)), y[k], y[k + 1]);
+            sm100::unpair_f32(sm100::fma_f32x2(a, ss, sm100::mul_f32x2(b, cc)), y[k + 4], y[k + 5]);
+        }
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = y[k] * c[k] + sign * (o[k] * s[k]);
 }
 
 template <int LANES>
@@ -144,6 +164,26 @@ __device__ __forceinline__ int find_tensor(const Params& p) {
     return ti;
 }
 
+// The first row of an item and how many it has; row u is the next head, or the head of the next token.
+struct Place { int b, n, head, rows; };
+template <int ROWS>
+__device__ __forceinline__ Place place_of(const Params& p, int heads, int per_token, const serve::Divide& by_per_token, int tokens_per, int item) {
+    Place at;
+    int token;
+    if (tokens_per > 1) {
+        token = item * tokens_per;
+        at.head = 0;
+        at.rows = min(tokens_per, p.tokens - token);
+    } else {
+        token = by_per_token(item);
+        at.head = (item - token * per_token) * ROWS;
+        at.rows = token < p.tokens ? min(ROWS, heads - at.head) : 0;
+    }
+    at.b = p.by_N(token);
+    at.n = token - at.b * p.N;
+    return at;
+}
+
 __device__ __forceinline__ int position_of(const Params& p, int b, int n) {
     long long pos = n;
     if (p.positions) {
@@ -151,157 +191,194 @@ __device__ __forceinline__ int position_of(const Params& p, int b, int n) {
         pos = p.pos_bytes == 8 ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
     }
     if (pos < 0 || pos >= p.table_rows) {
-        if (p.mode != ROT_NONE) serve::report(p.status, serve::ST_POSITION);
+        serve::report(p.status, serve::ST_POSITION);
         pos = 0;
     }
     return static_cast<int>(pos);
 }
 
-// One group of D / 8 lanes takes up to four heads of one token.  PAGED: the results of all tensors but the fifth (the
-// queries) go to the cache rows of slot lengths[b] + n, and that slot is the position unless `positions` names the
-// position of the first new token.
+// PAGED: the results of all tensors but the fifth (the queries) go to the cache rows of slot lengths[b] + n, and that
+// slot is the position unless `positions` names the position of the first new token.
 template <typename XT, int D, bool PAGED>
-__global__ void __launch_bounds__(THREADS) norm_rotate_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 4 : 3) norm_rotate_kernel(const __grid_constant__ Params p) {
     constexpr int LANES = D / 8;
     const int ti = find_tensor(p);
     const Tensor& t = p.t[ti];
-    const int lr = threadIdx.x % LANES;
-    const long long item = static_cast<long long>(blockIdx.x - t.block0) * (THREADS / LANES) + threadIdx.x / LANES;
-    const long long tokens = static_cast<long long>(p.B) * p.N;
-    const long long token = item / t.items;
-    const int head0 = static_cast<int>(item - token * t.items) * HEADS_PER_ITEM;
-    const bool live = token < tokens;
-    const int b = live ? static_cast<int>(token / p.N) : 0, n = live ? static_cast<int>(token - static_cast<long long>(b) * p.N) : 0;
+    const int lr = threadIdx.x % LANES, tokens_per = t.tokens_per, heads = t.heads, per_token = t.per_token, items = t.items;
+    const serve::Divide by_per_token = t.by_per_token;
+    const Columns cols = columns_of(p, lr);
+    const bool several = tokens_per > 1;
+    const bool turns = t.rotate && cols.turns, normed = t.w != nullptr, interleaved = p.interleaved != 0;
+    const bool to_cache = PAGED && ti < 4;
+    const float eps = p.eps;
+    const XT* const x0 = static_cast<const XT*>(t.x);
+    __nv_bfloat16* const y0 = static_cast<__nv_bfloat16*>(t.y);
+    const long long xb = t.xb, yb = t.yb;
+    const int xn = t.xn, xh = t.xh, yn = t.yn, step = to_cache ? D : t.yh;
+    float w[8];
+    if (normed) load_scale(t, cols, w);
 
-    Eight<XT> raw[HEADS_PER_ITEM];
-    const XT* x = static_cast<const XT*>(t.x) + b * t.xs[0] + n * t.xs[1] + lr * 8;
+    // the next token's batch and position
+    auto after = [&](int& b, int& n) { if (++n == p.N) { n = 0; ++b; } };
+    const int stride = t.blocks * (THREADS / LANES);
+    // every lane of a warp makes the same number of turns: the shuffles want all of them
+    for (int base = (blockIdx.x - t.block0) * (THREADS / LANES); base < items; base += stride) {
+        const int item = base + threadIdx.x / LANES;
+        Place at{0, 0, 0, 0};
+        if (item < items) at = place_of<FWD_ROWS>(p, heads, per_token, by_per_token, tokens_per, item);
+        Row8<XT> raw[FWD_ROWS];
+        {
+            int b = at.b, n = at.n;
+            const XT* x = x0 + b * xb + static_cast<long long>(n) * xn + static_cast<long long>(at.head) * xh;
 #pragma unroll
-    for (int u = 0; u < HEADS_PER_ITEM; ++u)
-        if (live && head0 + u < t.heads) raw[u].load(x + (head0 + u) * t.xs[2]);
-
-    long long dst = -1;                                                 // element offset of (row, head 0, column of this lane)
-    int pos = 0;
-    if (live) {
-        if (PAGED) {
-            const int slot = __ldg(p.lengths + b) + n;
-            if (p.mode != ROT_NONE && t.rotate) {
-                long long at = p.positions ? static_cast<long long>(static_cast<const int*>(p.positions)[b]) + n : slot;
-                if (at < 0 || at >= p.table_rows) { serve::report(p.status, serve::ST_POSITION); at = 0; }
-                pos = static_cast<int>(at);
+            for (int u = 0; u < FWD_ROWS; ++u) {
+                if (u < at.rows) raw[u].load(x, cols);
+                if (several) {
+                    after(b, n);
+                    x = x0 + b * xb + static_cast<long long>(n) * xn;
+                } else x += xh;
             }
-            if (ti < 4) {
-                if (!p.counts || n < __ldg(p.counts + b)) {
-                    const int row = p.pages.row(b, slot);
-                    if (row < 0) serve::report(p.status, serve::ST_PAGE);
-                    else dst = static_cast<long long>(row) * p.Hkv * D + lr * 8;
-                    if (ti == 0 && p.mass && row >= 0 && lr == 0)
-                        for (int u = 0; u < HEADS_PER_ITEM; ++u)
-                            if (head0 + u < t.heads) p.mass[static_cast<long long>(row) * p.Hkv + head0 + u] = 0.f;
+        }
+        Angles angles;
+        __nv_bfloat16* dst = nullptr;                                   // where the row goes, or nowhere
+        int b = at.b, n = at.n;
+#pragma unroll
+        for (int u = 0; u < FWD_ROWS; ++u) {
+            if (several ? u >= tokens_per : u >= heads) break;          // the same for the whole block
+            if (u == 0 || several) {
+                int pos = 0;
+                dst = nullptr;
+                if (u < at.rows) {
+                    if (PAGED) {
+                        const int slot = __ldg(p.lengths + b) + n;
+                        if (turns) {
+                            long long q = p.positions ? static_cast<long long>(static_cast<const int*>(p.positions)[b]) + n : slot;
+                            if (q < 0 || q >= p.table_rows) { serve::report(p.status, serve::ST_POSITION); q = 0; }
+                            pos = static_cast<int>(q);
+                        }
+                        if (!to_cache) dst = y0 + b * yb + static_cast<long long>(n) * yn;
+                        else if (!p.counts || n < __ldg(p.counts + b)) {
+                            const int row = p.pages.row(b, slot);
+                            if (row < 0) serve::report(p.status, serve::ST_PAGE);
+                            else dst = y0 + static_cast<long long>(row) * p.Hkv * D;
+                        }
+                    } else {
+                        if (turns) pos = position_of(p, b, n);
+                        dst = y0 + b * yb + static_cast<long long>(n) * yn;
+                    }
+                    if (dst && !several) dst += static_cast<long long>(at.head) * step;
                 }
-            } else {
-                dst = b * t.ys[0] + n * t.ys[1] + lr * 8;
+                angles = load_angles(p, pos, lr, turns);
+                if (several) after(b, n);
             }
-        } else {
-            if (t.rotate) pos = position_of(p, b, n);
-            dst = b * t.ys[0] + n * t.ys[1] + lr * 8;
+            float y[8];
+            if (u < at.rows) raw[u].get(y);
+            else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = 0.f;
+            }
+            if (normed) {
+                const float r = rsqrtf(row_sum<LANES>(dot8(y, y)) * (1.f / D) + eps);
+                scale8(y, r);
+                scale8(y, w);
+            }
+            if (turns) rotate(interleaved, y, angles, 1.f);
+            if (u < at.rows && dst) {
+                Row8<__nv_bfloat16>::store(dst, cols, y);
+                if (PAGED && ti == 0 && p.mass && lr == 0) p.mass[(dst - y0) / D] = 0.f;
+            }
+            if (!several && dst) dst += step;
         }
-    }
-    const long long step = PAGED && ti < 4 ? D : t.ys[2];
-    float c[8], s[8], w[8];
-    if (t.rotate) load_angles(p, pos, lr, c, s);
-    if (t.w) load_scale(t, lr * 8, w);
-#pragma unroll
-    for (int u = 0; u < HEADS_PER_ITEM; ++u) {
-        if (u >= t.heads) break;                                        // the same for the whole block
-        float y[8];
-        const bool here = live && head0 + u < t.heads;
-        if (here) raw[u].get(y);
-        else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = 0.f;
-        }
-        if (t.w) {
-            float ss = 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) ss += y[k] * y[k];
-            const float r = 1.f / sqrtf(row_sum<LANES>(ss) * (1.f / D) + p.eps);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = y[k] * r * w[k];
-        }
-        if (t.rotate) rotate<LANES>(p.mode, p.rot, lr, y, c, s, 1.f);
-        if (here && dst >= 0) Eight<__nv_bfloat16>::store(static_cast<__nv_bfloat16*>(t.y) + dst + (head0 + u) * step, y);
     }
 }
 
 template <typename XT, int D>
-__global__ void __launch_bounds__(THREADS) norm_rotate_backward_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 3 : 2) norm_rotate_backward_kernel(const __grid_constant__ Params p) {
     constexpr int LANES = D / 8, GROUPS = THREADS / LANES;
     __shared__ float sums[GROUPS][D];
     const int ti = find_tensor(p);
     const Tensor& t = p.t[ti];
     const int lr = threadIdx.x % LANES, group = threadIdx.x / LANES;
-    const long long tokens = static_cast<long long>(p.B) * p.N, items = tokens * t.items;
+    const int heads = t.heads, per_token = t.per_token, items = t.items;
+    const serve::Divide by_per_token = t.by_per_token;
+    const bool several = t.tokens_per > 1, normed = t.w != nullptr;
+    const Columns cols = columns_of(p, lr);
+    const bool turns = t.rotate && cols.turns, interleaved = p.interleaved != 0;
+    const float eps = p.eps;
+    const XT* const x0 = static_cast<const XT*>(t.x);
+    const __nv_bfloat16* const dy0 = static_cast<const __nv_bfloat16*>(t.dy);
+    XT* const dx0 = static_cast<XT*>(t.dx);
     float w[8], dw[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) { w[k] = 1.f; dw[k] = 0.f; }
-    if (t.w) load_scale(t, lr * 8, w);
+    if (normed) load_scale(t, cols, w);
 
-    // every lane of a warp makes the same number of turns: the shuffles want all of them
-    for (long long base = static_cast<long long>(blockIdx.x - t.block0) * GROUPS; base < items;
-         base += static_cast<long long>(t.blocks) * GROUPS) {
-        const long long item = base + group;
-        const bool live = item < items;
-        const long long token = live ? item / t.items : 0;
-        const int head0 = live ? static_cast<int>(item - token * t.items) * HEADS_PER_ITEM : 0;
-        const int b = static_cast<int>(token / p.N), n = static_cast<int>(token - static_cast<long long>(b) * p.N);
-        const XT* x = static_cast<const XT*>(t.x) + b * t.xs[0] + n * t.xs[1] + lr * 8;
-        const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(t.dy) + b * t.dys[0] + n * t.dys[1] + lr * 8;
-        XT* dx = static_cast<XT*>(t.dx) + b * t.dxs[0] + n * t.dxs[1] + lr * 8;
-        Eight<XT> rx[HEADS_PER_ITEM];
-        Eight<__nv_bfloat16> rg[HEADS_PER_ITEM];
+    struct Fetched { Row8<XT> x; Row8<__nv_bfloat16> g; int pos; XT* dx; };
+    auto fetch = [&](int item, Fetched (&f)[BWD_ROWS]) {
+        Place at{0, 0, 0, 0};
+        if (item < items) at = place_of<BWD_ROWS>(p, heads, per_token, by_per_token, several ? BWD_ROWS : 1, item);
 #pragma unroll
-        for (int u = 0; u < HEADS_PER_ITEM; ++u)
-            if (live && head0 + u < t.heads) {
-                rg[u].load(dy + (head0 + u) * t.dys[2]);
-                if (t.w) rx[u].load(x + (head0 + u) * t.xs[2]);
+        for (int u = 0; u < BWD_ROWS; ++u) {
+            f[u].dx = nullptr;
+            if (u < at.rows) {
+                const int h = several ? 0 : at.head + u;
+                f[u].g.load(dy0 + at.b * t.dyb + static_cast<long long>(at.n) * t.dyn + static_cast<long long>(h) * t.dyh, cols);
+                if (normed) f[u].x.load(x0 + at.b * t.xb + static_cast<long long>(at.n) * t.xn + static_cast<long long>(h) * t.xh, cols);
+                f[u].dx = dx0 + at.b * t.dxb + static_cast<long long>(at.n) * t.dxn + static_cast<long long>(h) * t.dxh;
+                if (u == 0 || several) f[u].pos = turns ? position_of(p, at.b, at.n) : 0;
             }
-        float c[8], s[8];
-        if (t.rotate) load_angles(p, live ? position_of(p, b, n) : 0, lr, c, s);
+            if (several && ++at.n == p.N) { at.n = 0; ++at.b; }
+        }
+    };
+    // every lane of a warp makes the same number of turns: the shuffles want all of them
+    const int stride = t.blocks * GROUPS;
+    Fetched next[BWD_ROWS];
+    int base = (blockIdx.x - t.block0) * GROUPS;
+    fetch(base + group, next);
+    for (; base < items; base += stride) {
+        Fetched now[BWD_ROWS];
 #pragma unroll
-        for (int u = 0; u < HEADS_PER_ITEM; ++u) {
-            if (u >= t.heads) break;
-            const bool here = live && head0 + u < t.heads;
+        for (int u = 0; u < BWD_ROWS; ++u) now[u] = next[u];
+        fetch(base + stride + group, next);
+        Angles angles;
+#pragma unroll
+        for (int u = 0; u < BWD_ROWS; ++u) {
             float g[8], v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) g[k] = v[k] = 0.f;
-            if (here) {
-                rg[u].get(g);
-                if (t.w) rx[u].get(v);
+            if (now[u].dx) {
+                now[u].g.get(g);
+                if (normed) now[u].x.get(v);
+                if (u == 0 || several) angles = load_angles(p, now[u].pos, lr, turns);
+                if (turns) rotate(interleaved, g, angles, -1.f);
             }
-            if (t.rotate) rotate<LANES>(p.mode, p.rot, lr, g, c, s, -1.f);
-            if (t.w) {
-                float ss = 0.f, m = 0.f;
+            if (normed) {
+                float wg[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    ss += v[k] * v[k];
-                    m += v[k] * (w[k] * g[k]);
-                }
-                ss = row_sum<LANES>(ss);
-                m = row_sum<LANES>(m);
-                const float r = 1.f / sqrtf(ss * (1.f / D) + p.eps);
-                const float f = r * r * (m * r) * (1.f / D);
+                for (int k = 0; k < 8; ++k) wg[k] = g[k];
+                scale8(wg, w);
+                const float ss = row_sum<LANES>(dot8(v, v)), m = row_sum<LANES>(dot8(v, wg));
+                const float q = rsqrtf(ss * (1.f / D) + eps);
+                const uint64_t qq = sm100::pair_f32(q, q);
+                const float f1 = -q * q * (m * q) * (1.f / D);
+                const uint64_t ff = sm100::pair_f32(f1, f1);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    dw[k] += g[k] * (v[k] * r);
-                    g[k] = r * (w[k] * g[k]) - v[k] * f;
+                for (int k = 0; k < 8; k += 2) {
+                    const uint64_t vv = sm100::pair_f32(v[k], v[k + 1]);
+                    sm100::unpair_f32(sm100::fma_f32x2(sm100::pair_f32(g[k], g[k + 1]), sm100::mul_f32x2(vv, qq), sm100::pair_f32(dw[k], dw[k + 1])),
+                                      dw[k], dw[k + 1]);
+                    sm100::unpair_f32(sm100::fma_f32x2(vv, ff, sm100::mul_f32x2(qq, sm100::pair_f32(wg[k], wg[k + 1]))), g[k], g[k + 1]);
                 }
             }
-            if (here) Eight<XT>::store(dx + (head0 + u) * t.dxs[2], g);
+            if (now[u].dx) Row8<XT>::store(now[u].dx, cols, g);
         }
     }
-    if (!t.w) return;
+    if (!normed) return;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sums[group][lr * 8 + k] = dw[k];
+    for (int k = 0; k < 4; ++k) {
+        sums[group][cols.a + k] = dw[k];
+        sums[group][cols.b + k] = dw[k + 4];
+    }
     __syncthreads();
     if (threadIdx.x < D) {
         float a = 0.f;
@@ -334,31 +411,33 @@ size_t element(int type) { return type == 2 ? 4 : 2; }
 bool aligned(const void* ptr, const int64_t* strides, int type) {
     if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return false;
     for (int k = 0; strides && k < 3; ++k)
-        if (strides[k] * static_cast<int64_t>(element(type)) % 16 != 0) return false;
+        if ((k > 0 && (strides[k] > 0x7FFFFFFFll || strides[k] < 0)) || strides[k] * static_cast<int64_t>(element(type)) % 16 != 0) return false;
     return true;
 }
 
-// Checks and fills what forward, backward and append have in common.  Blocks of a tensor: one group per item, or
-// (persistent) a share of `budget` blocks in proportion to its rows.
+// Checks and fills what forward, backward and append have in common.  Blocks of a tensor: one group per item, but no
+// more than its share of `budget` blocks in proportion to its rows.
 int fill(Params& p, const char* who, const att3_head_rows* t, int n, int x_type, const float* table, int table_rows,
-         int rot, int interleaved, int B, int N, int D, float eps, int budget) {
+         int rot, int interleaved, int B, int N, int D, float eps, int rows_per_item, int budget) {
     if (!t || n < 1 || n > MAX_TENSORS) return att3::set_error(ATT3_ERR_INVALID, "%s: 1 to %d tensors, got %d", who, MAX_TENSORS, n);
     if (D != 16 && D != 32 && D != 64 && D != 128)
         return att3::set_error(ATT3_ERR_INVALID, "%s: head dim must be 16, 32, 64 or 128, got %d", who, D);
     if (B < 0 || N < 0) return att3::set_error(ATT3_ERR_INVALID, "%s: negative batch or length", who);
     if (x_type < 0 || x_type > 2) return att3::set_error(ATT3_ERR_INVALID, "%s: unknown element type %d", who, x_type);
     if (!(eps >= 0.f)) return att3::set_error(ATT3_ERR_INVALID, "%s: eps must not be negative", who);
-    if (rot < 0 || rot > D || (rot % 16 != 0 && rot != 8))
-        return att3::set_error(ATT3_ERR_INVALID, "%s: rotated columns must be 0, 8 or a multiple of 16 up to the head dim %d, got %d", who, D, rot);
+    if (rot < 0 || rot > D || rot % 8 != 0)
+        return att3::set_error(ATT3_ERR_INVALID, "%s: rotated columns must be a multiple of 8 up to the head dim %d, got %d", who, D, rot);
     if (rot && (!table || table_rows < 1 || reinterpret_cast<uintptr_t>(table) % 16 != 0))
         return att3::set_error(ATT3_ERR_INVALID, "%s: the rotation needs a 16-byte aligned table with at least one row", who);
     p.n = n;
     p.table = table;
     p.table_rows = table_rows;
     p.rot = rot;
-    p.mode = rot == 0 ? ROT_NONE : interleaved ? ROT_NEIGHBOURS : rot == 8 ? ROT_IN_LANE : ROT_LANES;
+    p.interleaved = interleaved != 0;
     p.B = B;
     p.N = N;
+    p.by_N = serve::make_divide(std::max(1, N));
+    p.tokens = static_cast<int>(std::min<long long>(static_cast<long long>(B) * N, 0x7FFFFFFFll));
     p.eps = eps;
     const long long groups = THREADS / (D / 8);
     long long rows = 0, blocks = 0;
@@ -371,16 +450,24 @@ int fill(Params& p, const char* who, const att3_head_rows* t, int n, int x_type,
         o.x = t[k].x; o.y = t[k].y; o.dy = t[k].dy; o.dx = t[k].dx; o.w = t[k].w; o.dw = t[k].dw;
         o.w_type = static_cast<int>(t[k].w_type);
         o.rotate = t[k].rotate != 0;
-        for (int q = 0; q < 3; ++q) {
-            o.xs[q] = t[k].x_stride[q]; o.ys[q] = t[k].y_stride[q]; o.dys[q] = t[k].dy_stride[q]; o.dxs[q] = t[k].dx_stride[q];
-        }
+        o.xb = t[k].x_stride[0]; o.yb = t[k].y_stride[0]; o.dyb = t[k].dy_stride[0]; o.dxb = t[k].dx_stride[0];
+        o.xn = static_cast<int>(t[k].x_stride[1]); o.xh = static_cast<int>(t[k].x_stride[2]);
+        o.yn = static_cast<int>(t[k].y_stride[1]); o.yh = static_cast<int>(t[k].y_stride[2]);
+        o.dyn = static_cast<int>(t[k].dy_stride[1]); o.dyh = static_cast<int>(t[k].dy_stride[2]);
+        o.dxn = static_cast<int>(t[k].dx_stride[1]); o.dxh = static_cast<int>(t[k].dx_stride[2]);
         if (o.w && (o.w_type < 0 || o.w_type > 2)) return att3::set_error(ATT3_ERR_INVALID, "%s: unknown element type of scale %d", who, k);
         if (o.w && reinterpret_cast<uintptr_t>(o.w) % 16 != 0) return att3::set_error(ATT3_ERR_INVALID, "%s: scale %d must be 16-byte aligned", who, k);
         o.heads = static_cast<int>(t[k].heads);
-        o.items = (o.heads + HEADS_PER_ITEM - 1) / HEADS_PER_ITEM;
-        const long long items = static_cast<long long>(B) * N * o.items;
+        // one head: several tokens an item; more heads: several heads of one token
+        o.tokens_per = o.heads == 1 ? rows_per_item : 1;
+        o.per_token = o.tokens_per > 1 ? 1 : (o.heads + rows_per_item - 1) / rows_per_item;
+        o.by_per_token = serve::make_divide(o.per_token);
+        const long long tokens = static_cast<long long>(B) * N;
+        const long long items = o.tokens_per > 1 ? (tokens + o.tokens_per - 1) / o.tokens_per : tokens * o.per_token;
+        if (tokens * std::max(4, o.heads) > 0x3FFFFFFFll) return att3::set_error(ATT3_ERR_INVALID, "%s: more than 2^30 rows in a tensor", who);
+        o.items = static_cast<int>(items);
         long long nb = (items + groups - 1) / groups;
-        if (budget) nb = std::min(nb, std::max<long long>(1, budget * static_cast<long long>(o.heads) / rows));
+        nb = std::min(nb, std::max<long long>(1, budget * static_cast<long long>(o.heads) / rows));
         o.block0 = static_cast<int>(blocks);
         o.blocks = static_cast<int>(nb);
         blocks += nb;
@@ -441,13 +528,13 @@ extern "C" int att3_norm_rotate_forward(const att3_head_rows* tensors, int n, in
                                         int64_t pos_n, int B, int N, int D, float eps, void* stream) {
     const char* who = "att3_norm_rotate_forward";
     Params p = {};
-    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, N, D, eps, 0)) return rc;
+    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, N, D, eps, FWD_ROWS, att3::sm_count() * FWD_BLOCKS_PER_SM)) return rc;
     if (positions && pos_bytes != 4 && pos_bytes != 8) return att3::set_error(ATT3_ERR_INVALID, "%s: positions are 4 or 8 bytes wide", who);
     if (B == 0 || N == 0) return ATT3_OK;
     for (int k = 0; k < n; ++k) {
         if (!tensors[k].x || !tensors[k].y) return att3::set_error(ATT3_ERR_INVALID, "%s: null tensor %d", who, k);
         if (!aligned(tensors[k].x, tensors[k].x_stride, x_type) || !aligned(tensors[k].y, tensors[k].y_stride, 0))
-            return att3::set_error(ATT3_ERR_INVALID, "%s: rows of tensor %d must be 16-byte aligned", who, k);
+            return att3::set_error(ATT3_ERR_INVALID, "%s: rows of tensor %d must be 16-byte aligned, with strides below 2^31", who, k);
     }
     if (!att3::require_sm100(who)) return ATT3_ERR_UNSUPPORTED;
     p.positions = positions; p.pos_bytes = pos_bytes; p.pos_b = pos_b; p.pos_n = pos_n;
@@ -468,7 +555,7 @@ extern "C" int att3_norm_rotate_backward(const att3_head_rows* tensors, int n, i
     const char* who = "att3_norm_rotate_backward";
     Params p = {};
     const int budget = att3::sm_count() * BWD_BLOCKS_PER_SM;
-    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, N, D, eps, budget)) return rc;
+    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, N, D, eps, BWD_ROWS, budget)) return rc;
     if (positions && pos_bytes != 4 && pos_bytes != 8) return att3::set_error(ATT3_ERR_INVALID, "%s: positions are 4 or 8 bytes wide", who);
     const bool rows = B > 0 && N > 0;
     bool scaled = false;
@@ -515,7 +602,7 @@ extern "C" int att3_gather_cache_append(const att3_head_rows* tensors, int n, in
     const char* who = "att3_gather_cache_append";
     Params p = {};
     if (n != 4 && n != 5) return att3::set_error(ATT3_ERR_INVALID, "%s: R, S, Vr, Vs and optionally Q, got %d tensors", who, n);
-    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, T, D, eps, 0)) return rc;
+    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, T, D, eps, FWD_ROWS, att3::sm_count() * FWD_BLOCKS_PER_SM)) return rc;
     if (B == 0 || T == 0) return ATT3_OK;
     if (int rc = att3::check_gather_pages(pages, who)) return rc;
     if (!lengths) return att3::set_error(ATT3_ERR_INVALID, "%s: null lengths", who);

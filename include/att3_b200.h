@@ -303,7 +303,7 @@ typedef struct att3_head_rows {
 } att3_head_rows;
 
 /* y = Rot(w o x / sqrt(mean(x^2) + eps)) for up to five tensors in one pass.  Rot turns pairs of the first `rot`
- * columns (0, 8 or a multiple of 16), (d, d + rot/2) or with `interleaved` (2d, 2d + 1), by the angles of the row's
+ * columns (a multiple of 8), (d, d + rot/2) or with `interleaved` (2d, 2d + 1), by the angles of the row's
  * position: table is FP32 [table_rows, rot], the cosines of a position and then its sines.  positions: 4 or 8 byte
  * integers with strides pos_b, pos_n, or NULL for 0 .. N-1. */
 int att3_norm_rotate_forward(const att3_head_rows* tensors, int n, int x_type, const float* table, int table_rows,
