@@ -14,18 +14,26 @@ CPU baselines outside the kernel path and are not provided.
 import sys
 from importlib import import_module
 
-for _name in ("_cuda_kernels", "_autograd", "_custom_op", "_single_gather", "_single_gather_shared"):
+for _name in ("_cuda_kernels", "_autograd", "_custom_op", "_single_gather", "_single_gather_shared", "_norm_rotate",
+              "_gather_cache"):
     _mod = import_module(f"att3ntion_b200.{_name}")
     sys.modules[f"{__name__}.{_name}"] = _mod
     globals()[_name] = _mod
 
 from att3ntion_b200 import (  # noqa: E402
+    GatherCache,
     HypergraphAttention,
     QuickGELU,
+    gather_cache_append,
+    gather_cache_evict,
+    norm_rotate,
+    rotary_table,
     single_gather_attention,
+    single_gather_decode,
     single_gather_shared_attention,
     window_mask,
 )
 
-__all__ = ["HypergraphAttention", "QuickGELU", "single_gather_attention", "single_gather_shared_attention",
+__all__ = ["GatherCache", "HypergraphAttention", "QuickGELU", "gather_cache_append", "gather_cache_evict", "norm_rotate",
+           "rotary_table", "single_gather_attention", "single_gather_decode", "single_gather_shared_attention",
            "window_mask"]

@@ -20,6 +20,7 @@ _EXPORTS = {
     "gather_cache_append": "._gather_cache",
     "gather_cache_evict": "._gather_cache",
     "single_gather_decode": "._gather_cache",
+    "GatherCache": "._gather_cache",
 }
 
 __all__ = sorted(_EXPORTS)

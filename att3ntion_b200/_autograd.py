@@ -8,6 +8,10 @@ with QuickGELU, heads split from ``d_model``, inputs cast to BF16 at the kernel
 boundary and the sequence padded to a multiple of 16 with the padding invisible.
 ``gather_mode=1`` keeps only the Q-anchored gather and, for head sizes 64 and 128,
 routes to ``single_gather_attention`` (optionally windowed).
+
+Beyond the reference, keyword arguments add per-head RMS norms of Q, R and S (``qk_norm``), the position rotation of
+the same rows (``rotary_base``), and first keys that stay visible outside the window (``sinks``); a windowed layer is
+served from a ``GatherCache`` with ``prefill`` and ``decode``.
 """
 from __future__ import annotations
 
@@ -18,6 +22,7 @@ import torch.nn as nn
 from torch.autograd import Function
 
 from . import _custom_op  # noqa: F401  (registers torch.ops.att3ntion.hypergraph_{forward,backward})
+from ._norm_rotate import norm_rotate, rotary_table
 from ._single_gather import single_gather_attention, single_gather_heads_last, window_mask
 
 TILE = 16
@@ -102,9 +107,14 @@ class QuickGELU(nn.Module):
 
 
 class HypergraphAttention(nn.Module):
-    """Three-way hypergraph attention layer on the sm_100a kernels."""
+    """Three-way hypergraph attention layer on the sm_100a kernels.
 
-    def __init__(self, d_model, n_heads, dropout_rate=0, scatter=False, gather_mode=0, window=0):
+    qk_norm: RMS norms with learned scales over the heads of Q, R and S.  rotary_base: rotates those rows by their
+    position's angles (see `rotary_table`; pairs of columns half a head apart).  sinks (with a window): the first `sinks`
+    keys stay visible to every later query."""
+
+    def __init__(self, d_model, n_heads, dropout_rate=0, scatter=False, gather_mode=0, window=0, *, qk_norm=False,
+                 rotary_base=None, sinks=0, norm_eps=1e-6):
         super().__init__()
         if d_model % n_heads != 0:
             raise ValueError(f"d_model ({d_model}) must be divisible by n_heads ({n_heads})")
@@ -114,7 +124,12 @@ class HypergraphAttention(nn.Module):
             raise ValueError("scatter requires all three gathers (gather_mode=0)")
         if window and gather_mode != 1:
             raise ValueError("window requires the Q-anchored gather only (gather_mode=1)")
+        if sinks < 0 or (sinks and not window):
+            raise ValueError("sinks are first keys that stay visible outside a window: they need window > 0")
         self.d_model, self.n_heads, self.head_dim = d_model, n_heads, d_model // n_heads
+        if (qk_norm or rotary_base) and self.head_dim not in (16, 32, 64, 128):
+            raise ValueError(f"qk_norm and rotary_base need a head dim of 16, 32, 64 or 128, got {self.head_dim}")
+        self.sinks, self.rotary_base, self.norm_eps = sinks, rotary_base, norm_eps
         self.scatter, self.gather_mode, self.window = scatter, gather_mode, window
         inner = n_heads * self.head_dim
         self.Wq = nn.Linear(d_model, inner, bias=False)
@@ -128,6 +143,9 @@ class HypergraphAttention(nn.Module):
         self.Wo = nn.Linear(inner, d_model, bias=True)
         self.dropout = nn.Dropout(dropout_rate)
         self.gelu = QuickGELU()
+        self.q_norm, self.r_norm, self.s_norm = (nn.Parameter(torch.ones(self.head_dim)) if qk_norm else None
+                                                 for _ in range(3))
+        self._tables = []
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
                               error_msgs):
@@ -150,6 +168,28 @@ class HypergraphAttention(nn.Module):
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
                                       error_msgs)
 
+    def _rotary(self, length, device):
+        """The angle table, at least `length` positions long, or None.  It grows by doubling, and the shorter ones are kept:
+        a captured graph may still read them."""
+        if not self.rotary_base:
+            return None
+        for t in reversed(self._tables):
+            if t.device == device and t.shape[0] >= length:
+                return t
+        most = max((t.shape[0] for t in self._tables if t.device == device), default=256)
+        self._tables.append(rotary_table(max(length, 2 * most), self.head_dim, self.rotary_base, device))
+        return self._tables[-1]
+
+    def _qrs(self, x, heads_first):
+        """The score operands of every position, [B,N,H,D] or [B,H,N,D]: projected, and normed and rotated in one pass
+        (then bf16) if the layer has either."""
+        b, n, _ = x.shape
+        qrs = [w(x).view(b, n, self.n_heads, self.head_dim) for w in (self.Wq, self.Wr, self.Ws)]
+        if self.q_norm is None and not self.rotary_base:
+            return [t.permute(0, 2, 1, 3) for t in qrs] if heads_first else qrs
+        return norm_rotate(qrs, (self.q_norm, self.r_norm, self.s_norm), self._rotary(n, x.device), eps=self.norm_eps,
+                           heads_first=heads_first)
+
     def _heads(self, t, width=None):
         b, n, _ = t.shape
         return t.reshape(b, n, self.n_heads, width or self.head_dim).permute(0, 2, 1, 3)
@@ -158,6 +198,8 @@ class HypergraphAttention(nn.Module):
         if rotary_emb is not None:
             raise ValueError("CUDA HypergraphAttention does not support rotary embeddings")
         b, n, _ = x.shape
+        if self.q_norm is not None or self.rotary_base or self.sinks:
+            return self._extended(x, mask)
         Q, R, S = self.Wq(x), self.Wr(x), self.Ws(x)
         window_only = bool(self.window) and mask is None      # then the kernels derive the window from indices
         if self.window:
@@ -179,6 +221,10 @@ class HypergraphAttention(nn.Module):
             y = self.gelu(y).permute(0, 2, 1, 3).contiguous().view(b, n, self.n_heads * self.head_dim)
             return self.Wo(y)
 
+        return self._three_gather(x, self._heads(Q), self._heads(R), self._heads(S), mask)
+
+    def _three_gather(self, x, Q, R, S, mask):
+        b, n, _ = x.shape
         if self.scatter:
             Vq_1, Vq_2 = self._heads(self.Wv_q(x), 2 * self.head_dim).split(self.head_dim, dim=-1)
             Vr_1, Vr_2 = self._heads(self.Wv_r(x), 2 * self.head_dim).split(self.head_dim, dim=-1)
@@ -189,7 +235,7 @@ class HypergraphAttention(nn.Module):
             Vq_2, Vr_2, Vs_2 = torch.zeros_like(Vq_1), torch.zeros_like(Vr_1), torch.zeros_like(Vs_1)
 
         Y_q, Y_r, Y_s, Y_q_, Y_r_, Y_s_ = _HypergraphAttentionAutograd.apply(
-            self._heads(Q), self._heads(R), self._heads(S), Vq_1, Vq_2, Vr_1, Vr_2, Vs_1, Vs_2, mask,
+            Q, R, S, Vq_1, Vq_2, Vr_1, Vr_2, Vs_1, Vs_2, mask,
             self.dropout.p, self.scatter, self.gather_mode)
         y = self.gelu(Y_q)
         if self.gather_mode == 0:
@@ -198,3 +244,77 @@ class HypergraphAttention(nn.Module):
             y = y + self.gelu(Y_q_) + self.gelu(Y_r_) + self.gelu(Y_s_)
         y = y.permute(0, 2, 1, 3).contiguous().view(b, n, self.n_heads * self.head_dim)
         return self.Wo(y)
+
+    # ------------------------------------------------------------------ norms, rotation, sinks
+
+    def _gather(self, x, Q, R, S, Vr, Vs, mask, last):
+        """The Q-anchored gather and its output projection; operands [B,N,H,D] if `last`, else [B,H,N,D]."""
+        b, n, _ = x.shape
+        if last:
+            y = single_gather_heads_last(Q, R, S, Vr, Vs, min(self.window, n), act=True)
+        else:
+            y = single_gather_attention(Q, R, S, Vr, Vs, mask, 0 if self.sinks else min(self.window, n))
+            y = self.gelu(y.to(x.dtype)).permute(0, 2, 1, 3)
+        return self.Wo(y.to(x.dtype).reshape(b, n, self.n_heads * self.head_dim))
+
+    def _reads_in_place(self, n, mask):
+        """Whether the windowed kernels take the projections where they lie, [B,N,H,D]."""
+        return mask is None and not self.sinks and 0 < self.window <= 128 and n % TILE == 0
+
+    def _extended(self, x, mask):
+        b, n, _ = x.shape
+        last = self.gather_mode == 1 and self.head_dim in (64, 128) and self._reads_in_place(n, mask)
+        Q, R, S = self._qrs(x, heads_first=not last)
+        if self.window and not last and (mask is not None or self.sinks):
+            win = window_mask(n, self.window, x.device, self.sinks)
+            mask = win if mask is None else mask.to(device=x.device, dtype=torch.bool) & win
+        if self.gather_mode == 1 and self.head_dim in (64, 128):
+            split = lambda t: t.view(b, n, self.n_heads, self.head_dim) if last else self._heads(t)
+            return self._gather(x, Q, R, S, split(self.Wv_r(x)), split(self.Wv_s(x)), mask, last)
+        if self.window and mask is None:
+            mask = window_mask(n, self.window, x.device)
+        # the gather's outputs come in the operands' type, which is the kernels' own here
+        return self._three_gather(x, *(t.to(x.dtype) for t in (Q, R, S)), mask)
+
+    # ------------------------------------------------------------------ serving
+
+    def _check_serving(self, who, x, cache):
+        if self.gather_mode != 1 or not self.window or self.head_dim not in (64, 128):
+            raise ValueError(f"{who}: needs gather_mode=1, a window and a head dim of 64 or 128")
+        if x.dim() != 3 or x.shape[0] != cache.sequences:
+            raise ValueError(f"{who}: x must be [{cache.sequences},length,{self.d_model}], got {tuple(x.shape)}")
+
+    @torch.no_grad()
+    def prefill(self, x, cache, counts=None):
+        """The layer over the prompts x [B,N,d_model] of empty sequences, storing their rows in `cache`.  counts (a list of
+        ints): the prompts' lengths, right-padded to N; what comes back behind a prompt's end means nothing."""
+        self._check_serving("prefill", x, cache)
+        if any(cache.host_lengths):
+            raise ValueError("prefill: the cache's sequences must be empty")
+        b, n, _ = x.shape
+        # a window of causal keys: the padding behind a prompt is never seen by its own positions
+        last = self._reads_in_place(n, None)
+        Q, R, S = self._qrs(x, heads_first=not last)
+        vr, vs = self.Wv_r(x), self.Wv_s(x)
+        split = lambda t: t.view(b, n, self.n_heads, self.head_dim)
+        side = (lambda t: t) if last else (lambda t: t.transpose(1, 2))
+        mask = window_mask(n, self.window, x.device, self.sinks) if self.sinks else None
+        vr, vs = split(vr), split(vs)
+        R_, S_ = side(R), side(S)
+        cache.append(R_, S_, vr.to(R_.dtype), vs.to(R_.dtype), counts=counts)
+        return self._gather(x, Q, R, S, side(vr), side(vs), mask, last)
+
+    @torch.no_grad()
+    def decode(self, x, cache):
+        """The layer over one new token of every sequence, x [B,1,d_model], after storing its rows in `cache`: the last
+        `window` cached tokens and the first `sinks` are visible."""
+        self._check_serving("decode", x, cache)
+        if x.shape[1] != 1:
+            raise ValueError(f"decode: one token a sequence, got {x.shape[1]}")
+        b = x.shape[0]
+        split = lambda t: t.view(b, 1, self.n_heads, self.head_dim)
+        table = self._rotary(max(cache.host_positions, default=0) + 1, x.device)
+        q = cache.append(split(self.Wr(x)), split(self.Ws(x)), split(self.Wv_r(x)), split(self.Wv_s(x)), Q=split(self.Wq(x)),
+                         weights=(self.q_norm, self.r_norm, self.s_norm), table=table, eps=self.norm_eps)
+        y = self.gelu(cache.decode(q[:, 0], window=self.window, sinks=self.sinks).to(x.dtype))
+        return self.Wo(y.reshape(b, 1, self.n_heads * self.head_dim))

@@ -210,3 +210,102 @@ def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recen
                       _pages(out_table if out_table is not None else page_table, pool), lengths.data_ptr(), left.data_ptr(),
                       kept.data_ptr(), B, Hkv, D, keep, sinks, recent, _ck._raw_stream(pool.device))
     return kept, left
+
+
+class GatherCache:
+    """A paged gather cache of a batch of sequences that move together: pools, page table and lengths on the device, and
+    the book-keeping of pages on the host.
+
+    sequences: rows of the page table.  pages: pages of `page_size` slots in each pool.  slots: the most that a sequence
+    may hold.  track_mass: add up every token's share of the attention in `decode`, for `evict`.
+
+    Pages are handed out in Python when a call needs them, so these methods are not for capture into a graph: a captured
+    step calls the functions above on tensors of its own (or this cache's), which read lengths and tables as they are."""
+
+    def __init__(self, sequences, n_kv_heads, head_dim, *, pages, slots, page_size=64, track_mass=False, device="cuda"):
+        if min(sequences, n_kv_heads, pages, slots, page_size) < 1:
+            raise ValueError("GatherCache: sequences, heads, pages, slots and page_size must be positive")
+        if head_dim not in (64, 128):
+            raise ValueError(f"GatherCache: head_dim must be 64 or 128, got {head_dim}")
+        self.sequences, self.page_size, self.slots = sequences, page_size, slots
+        shape = (pages, page_size, n_kv_heads, head_dim)
+        self.pools = [torch.zeros(shape, dtype=_BF16, device=device) for _ in range(4)]
+        self.mass = torch.zeros(shape[:3], dtype=torch.float32, device=device) if track_mass else None
+        self._book = torch.full((sequences, -(-slots // page_size)), -1, dtype=torch.int32)      # the host's page table
+        self.page_table = self._book.to(device)
+        # slots in use and tokens seen (which stay apart once tokens have been evicted), one tensor so that one add moves both
+        self._counters = torch.zeros((2, sequences), dtype=torch.int32, device=device)
+        self.lengths, self.positions = self._counters[0], self._counters[1]
+        self.host_lengths, self.host_positions = [0] * sequences, [0] * sequences
+        self._free = list(range(pages - 1, -1, -1))
+
+    def _counts(self, counts, T):
+        if counts is None:
+            return [T] * self.sequences
+        counts = [int(c) for c in counts]
+        if len(counts) != self.sequences or any(not 0 <= c <= T for c in counts):
+            raise ValueError(f"GatherCache: counts must be {self.sequences} numbers of 0 .. {T}")
+        return counts
+
+    def reserve(self, counts):
+        """Hands out the pages that `counts[b]` more slots of every sequence need."""
+        want = []
+        for b, c in enumerate(counts):
+            n = self.host_lengths[b] + c
+            if n > self.slots:
+                raise RuntimeError(f"GatherCache: sequence {b} would hold {n} slots, at most {self.slots}")
+            have, need = -(-self.host_lengths[b] // self.page_size), -(-n // self.page_size)
+            want += [(b, k) for k in range(have, need) if int(self._book[b, k]) < 0]
+        if len(want) > len(self._free):
+            raise RuntimeError(f"GatherCache: {len(want)} pages needed, {len(self._free)} free")
+        for b, k in want:
+            self._book[b, k] = self._free.pop()
+        if want:
+            self.page_table.copy_(self._book)
+
+    def append(self, R, S, Vr, Vs, *, counts=None, Q=None, weights=None, table=None, eps=1e-6, interleaved=False):
+        """`gather_cache_append` at the sequences' ends (R .. [B,T,Hkv,D]; counts: a list of ints, all T by default);
+        rotations go by the number of tokens seen, evicted ones included.  Returns Q's rows, if given."""
+        T = R.shape[1]
+        host = self._counts(counts, T)
+        self.reserve(host)
+        device = self.page_table.device
+        on_device = None if counts is None else torch.tensor(host, dtype=torch.int32, device=device)
+        q = gather_cache_append(self.pools, self.page_table, self.lengths, R, S, Vr, Vs, counts=on_device, Q=Q, weights=weights,
+                                table=table, positions=self.positions, mass=self.mass, eps=eps, interleaved=interleaved)
+        self._counters.add_(T if on_device is None else on_device)
+        for b, c in enumerate(host):
+            self.host_lengths[b] += c
+            self.host_positions[b] += c
+        return q
+
+    def decode(self, Q, *, window=0, sinks=0):
+        """`single_gather_decode` of Q [B,Hq,D] over the cached rows, adding to the masses if they are tracked."""
+        return single_gather_decode(Q, self.pools, self.page_table, self.lengths, window=window, sinks=sinks, mass=self.mass)
+
+    def evict(self, keep, *, sinks=0, recent=0):
+        """`gather_cache_evict` in place; the pages behind the kept slots become free.  Returns the slots that stayed,
+        int32 [B,Hkv,keep]."""
+        if self.mass is None:
+            raise RuntimeError("GatherCache.evict: the cache does not track masses (track_mass=True)")
+        kept, left = gather_cache_evict(self.pools, self.mass, self.page_table, self.lengths, keep, sinks=sinks, recent=recent)
+        self.lengths.copy_(left)
+        for b in range(self.sequences):
+            self.host_lengths[b] = min(self.host_lengths[b], int(keep))
+            self._release(b, -(-self.host_lengths[b] // self.page_size))
+        self.page_table.copy_(self._book)
+        return kept
+
+    def _release(self, b, first):
+        for k in range(first, self._book.shape[1]):
+            page = int(self._book[b, k])
+            if page >= 0:
+                self._free.append(page)
+                self._book[b, k] = -1
+
+    def clear(self, sequence):
+        """Empties one sequence and frees its pages."""
+        self._release(sequence, 0)
+        self.host_lengths[sequence] = self.host_positions[sequence] = 0
+        self._counters[:, sequence] = 0
+        self.page_table.copy_(self._book)

@@ -29,10 +29,12 @@ def _pad_rows(t: torch.Tensor, n_pad: int) -> torch.Tensor:
     return torch.nn.functional.pad(t, (0, 0, 0, n_pad)) if n_pad else t
 
 
-def window_mask(n: int, window: int, device) -> torch.Tensor:
-    """[n,n] bool: query i sees key j iff i - window < j <= i (window >= n: causal)."""
+def window_mask(n: int, window: int, device, sinks: int = 0) -> torch.Tensor:
+    """[n,n] bool: query i sees key j iff i - window < j <= i (window >= n: causal), or j <= i is one of the first
+    `sinks` keys."""
     i = torch.arange(n, device=device)
-    return (i[None, :] <= i[:, None]) & (i[None, :] > i[:, None] - window)
+    near = i[None, :] > i[:, None] - window
+    return (i[None, :] <= i[:, None]) & (near | (i[None, :] < sinks) if sinks else near)
 
 
 def _prepare_mask(mask, batch: int, n: int, n_pad: int, device):

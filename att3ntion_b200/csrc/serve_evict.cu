@@ -213,7 +213,8 @@ int check_gather_pages(const att3_gather_pages* g, const char* who) {
     if (!g || !g->table) return set_error(ATT3_ERR_INVALID, "%s: null page table", who);
     if (g->page_size < 1 || g->pages < 1 || g->per_sequence < 1)
         return set_error(ATT3_ERR_INVALID, "%s: page size, pages and table width must be positive", who);
-    if (g->pages * g->page_size > 0x7FFFFFFFll || g->per_sequence * g->page_size > 0x7FFFFFFFll)
+    constexpr int64_t most = 0x7FFFFFFFll;
+    if (g->pages > most || g->page_size > most || g->per_sequence > most || g->pages * g->page_size > most || g->per_sequence * g->page_size > most)
         return set_error(ATT3_ERR_INVALID, "%s: a pool or a sequence of more than 2^31 - 1 slots", who);
     return ATT3_OK;
 }

@@ -461,3 +461,140 @@ def test_captured_step_follows_the_lengths():
     for p, t in zip(pools, twin):
         assert torch.equal(p, t)
     ck.device_status()
+
+
+# --------------------------------------------------------------------------- the layer
+
+@pytest.mark.parametrize("kw", [dict(window=128, qk_norm=True, rotary_base=10000.0), dict(window=16, qk_norm=True),
+                                dict(window=33, rotary_base=500.0, sinks=3), dict(window=200, qk_norm=True, rotary_base=1e4),
+                                dict(window=64)])
+@pytest.mark.parametrize("head_dim,dtype", [(64, torch.float32), (128, torch.bfloat16)])
+def test_layer_prefill_and_decode_follow_its_forward(kw, head_dim, dtype):
+    """Prompts of different lengths, then tokens one by one, against the forward pass over the whole sequences.  The two
+    round at different places, so they are held to the gate that the forward itself is held to (relative 0.03 in the
+    2-norm; the forward rounds Q o R, the decode does not)."""
+    from att3ntion_b200 import GatherCache, HypergraphAttention
+    torch.manual_seed(3)
+    B, N, H = 3, 150, 2
+    layer = HypergraphAttention(H * head_dim, H, gather_mode=1, **kw).cuda().to(dtype)
+    x = torch.randn(B, N, H * head_dim, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        want = layer(x)
+    prompts = [140, 1, 97]
+    cache = GatherCache(B, H, head_dim, pages=40, slots=N, page_size=16)
+    y = layer.prefill(x[:, :140], cache, counts=prompts)
+    base = layer.Wo.bias.detach().double()
+    # The layer's results hold the output bias too and are rounded with it: each by half a step of its type, relative to
+    # the whole value.  With the bias an order of magnitude above the rest (0.06 against 0.002 here) that is no part of
+    # the 0.03 above but comes on top, once for either side.
+    half_step = torch.finfo(dtype).eps / 2
+
+    def near(a, b):
+        a, b = a.detach().double(), b.detach().double()
+        tol = 0.03 * (b - base).norm() + half_step * (a.norm() + b.norm())
+        assert torch.isfinite(a).all() and (a - b).norm() <= tol, (float((a - b).norm()), float(tol))
+    for b, n in enumerate(prompts):
+        near(y[b, :n], want[b, :n])
+    for _ in range(10):
+        at = cache.host_lengths
+        step = torch.stack([x[b, at[b]] for b in range(B)])[:, None]
+        where = list(at)
+        y = layer.decode(step, cache)
+        for b in range(B):
+            near(y[b, 0], want[b, where[b]])
+    assert cache.lengths.tolist() == cache.host_lengths == [n + 10 for n in prompts]
+
+
+def test_layer_trains_with_norms_and_rotation():
+    """Gradients of the extended layer against central differences of its own loss in the direction of the gradient."""
+    from att3ntion_b200 import HypergraphAttention
+    torch.manual_seed(4)
+    for mode, window in ((1, 16), (1, 0), (0, 0)):
+        layer = HypergraphAttention(64, 1, gather_mode=mode, window=window, qk_norm=True, rotary_base=100.0).cuda()
+        x = torch.randn(1, 32, 64, device="cuda")
+        dy = torch.randn(1, 32, 64, device="cuda")
+        layer(x).backward(dy)
+        for name in ("q_norm", "r_norm", "s_norm", "Wq.weight", "Ws.weight"):
+            p = dict(layer.named_parameters())[name]
+            assert p.grad is not None and torch.isfinite(p.grad).all() and p.grad.norm() > 0, name
+            # The loss is a sum of N D terms of BF16 results: 2^-9 rms each, so 2^-9 |dy o y| in all; a step that moves the
+            # loss by 30 times that leaves the difference quotient good to a tenth.
+            with torch.no_grad():
+                direction = p.grad / p.grad.norm()
+                noise = float((dy * layer(x)).norm()) * 2.0 ** -9
+                h = max(0.05, 30 * noise / float(p.grad.norm()))
+                if h > 0.3 * float(p.norm()):
+                    continue                                    # a gradient too small to be seen through the rounding
+                p.add_(direction, alpha=h)
+                up = float((layer(x).double() * dy.double()).sum())
+                p.add_(direction, alpha=-2 * h)
+                down = float((layer(x).double() * dy.double()).sum())
+                p.add_(direction, alpha=h)
+            assert abs((up - down) / (2 * h) - float(p.grad.norm())) <= 0.25 * float(p.grad.norm()), (mode, name)
+
+
+def test_cache_run_append_decode_evict_decode():
+    """A cache that tracks masses through steps, an eviction and further steps, against the definitions in 64 bits."""
+    from att3ntion_b200 import GatherCache, rotary_table
+    g = torch.Generator().manual_seed(21)
+    B, Hq, Hkv, D, page = 2, 4, 2, 64, 8
+    cache = GatherCache(B, Hkv, D, pages=24, slots=80, page_size=page, track_mass=True)
+    table = rotary_table(200, D)
+    ws = [1 + 0.2 * torch.randn(D, generator=g) for _ in range(3)]
+    kept_rows = [[[[] for _ in range(4)] for _ in range(Hkv)] for _ in range(B)]     # what each head's slots must hold
+    share = [[[] for _ in range(Hkv)] for _ in range(B)]
+    seen = [0, 0]
+
+    def step(T, counts):
+        new = [rand(g, B, T, Hkv, D) for _ in range(4)]
+        q = rand(g, B, T, Hq, D)
+        got = cache.append(*[t.cuda() for t in new], counts=counts, Q=q.cuda(), weights=[w.cuda() for w in ws], table=table.cuda())
+        for b in range(B):
+            for t in range(T if counts is None else counts[b]):
+                pos = torch.tensor([[seen[b]]])
+                rows = [x[b: b + 1, t: t + 1].double() for x in new]
+                for k in (0, 1):
+                    rows[k] = ref.norm_rotate(rows[k], ws[k + 1].double(), table.double(), pos, 1e-6, False)
+                for h in range(Hkv):
+                    for k in range(4):
+                        kept_rows[b][h][k].append(rows[k][0, 0, h])
+                    share[b][h].append(0.0)
+                seen[b] += 1
+        return got
+
+    def check(q):
+        y = cache.decode(q)
+        for b in range(B):
+            for h in range(Hq):
+                k = h // (Hq // Hkv)
+                R, S, Vr, Vs = (torch.stack(t) for t in kept_rows[b][k])
+                x = (q[b, h].double().cpu() * R) @ S.T / 8.0
+                p = torch.softmax(x.flatten(), 0).view_as(x)
+                Y, A = ((p @ Vs) * Vr).sum(0), ((p @ Vs.abs()) * Vr.abs()).sum(0)
+                # R and S were rounded to BF16 on the way in: each factor of a score by 2^-8 at most, so a score by 2^-7 of
+                # its sum of magnitudes, and the probabilities by twice that
+                slack = 2.0 ** -7 * float(((q[b, h].double().cpu().abs() * R.abs()) @ S.abs().T / 8.0).max()) * 2
+                assert ((y[b, h].double().cpu() - Y).abs() <= 3 * HALF * (Y.abs() + A) + slack * A).all()
+                part = (p.sum(0) + p.sum(1)) / (2 * (Hq // Hkv))
+                share[b][k] = [a + float(v) for a, v in zip(share[b][k], part)]
+
+    step(30, [30, 17])
+    for _ in range(4):
+        check(step(1, None)[:, 0])
+    kept = cache.evict(20, sinks=2, recent=5)
+    assert cache.lengths.tolist() == cache.host_lengths == [20, 20] and cache.positions.tolist() == seen == [34, 21]
+    for b in range(B):
+        for h in range(Hkv):
+            slots = kept[b, h].tolist()
+            assert slots == sorted(set(slots)) and slots[:2] == [0, 1] and slots[-5:] == list(range(seen[b] - 5, seen[b]))
+            # what left had no more mass than what stayed (up to the rounding of R and S)
+            out = [share[b][h][e] for e in range(seen[b]) if e not in slots]
+            mid = [share[b][h][e] for e in slots[2:-5]]
+            assert max(out) <= min(mid) * 1.2
+            kept_rows[b][h] = [[t[e] for e in slots] for t in kept_rows[b][h]]
+            share[b][h] = [share[b][h][e] for e in slots]
+    assert len(cache._free) == 24 - 2 * 3
+    for _ in range(6):
+        check(step(1, None)[:, 0])
+    cache.clear(0)
+    assert cache.lengths.tolist() == [0, 26] and len(cache._free) == 24 - 4
