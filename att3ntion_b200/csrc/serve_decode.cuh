@@ -404,21 +404,30 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         // are free between a segment's last score product and the next segment's first: Vr waits in the value tile for
         // the collapse, the next segment's R in the residual tile for the build, which replaces it in place.
         const uint32_t tiles_at = smem_u32(tile_hi);
-        auto fetch = [&](const __nv_bfloat16* pool, const Walk<MASS>& at, uint32_t tile, int from_row, int rows) {
+        auto fetch = [&](const __nv_bfloat16* pool, const Walk<MASS>& at, uint32_t tile, int from_row) {
             const char* src = reinterpret_cast<const char*>(pool + static_cast<size_t>(at.head) * D + chunk * 8);
             const uint32_t pitch = p.Hkv * D * 2;
-#pragma unroll 4
-            for (int i = 0; i < PASSES; ++i) {
-                const int in = i * RPP + sub;
-                const uint32_t from = __shfl_sync(0xFFFFFFFFu, from_row, in);
-                if (in < rows) copy16(tile + sw128_offset<128>(wq * 32 + in, chunk), src + static_cast<uint64_t>(from) * pitch);
+            // rows of a batch first, then its copies: a shuffle's result is not waited for before every copy.  A row behind
+            // the last key repeats row 0's place of the lane's shuffle; the build and the collapse leave it out.
+            constexpr int BATCH = 8;
+            const uint32_t at0 = tile + sw128_offset<128>(wq * 32 + sub, chunk);
+#pragma unroll 1
+            for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
+                uint32_t from[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) from[i] = __shfl_sync(0xFFFFFFFFu, from_row, (i0 + i) * RPP + sub);
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i)            // RPP rows further on: the swizzle's row bits come round every 8 rows
+                    copy16(RPP * (i0 + i) % 8 == 0 ? at0 + RPP * (i0 + i) * 128 : tile + sw128_offset<128>(wq * 32 + (i0 + i) * RPP + sub, chunk),
+                           src + static_cast<uint64_t>(from[i]) * pitch);
             }
             copy_commit();
         };
         uint4 q = make_uint4(0, 0, 0, 0);
         auto prepare = [&](const Walk<MASS>& at) {
             look(at);
-            fetch(p.R, at, tiles_at + L::TILE, row, valid);
+            if (valid > 0) fetch(p.R, at, tiles_at + L::TILE, row);
+            else copy_commit();
             q = *reinterpret_cast<const uint4*>(p.Q + (static_cast<size_t>(at.b) * p.Hq + at.head * p.G + g) * D + chunk * 8);
         };
         while (go && !w.live(p, half)) go = w.next(p);
@@ -428,19 +437,25 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             // ---- operand tiles: value and residual of q o R
             copy_wait<0>();
             __syncwarp();
-#pragma unroll 4
-            for (int i = 0; i < PASSES; ++i) {
+            auto build = [&](int i, bool all) {
                 const int in = i * RPP + sub;
                 const uint32_t at = sw128_offset<128>(wq * 32 + in, chunk);
-                uint4 r = *reinterpret_cast<const uint4*>(tile_hi + L::TILE + at), hi, lo;
-                if (in >= valid) r = make_uint4(0, 0, 0, 0);
+                const uint4 r = *reinterpret_cast<const uint4*>(tile_hi + L::TILE + at);
+                uint4 hi, lo;
                 hi.x = mul_bf16x2(q.x, r.x); hi.y = mul_bf16x2(q.y, r.y);
                 hi.z = mul_bf16x2(q.z, r.z); hi.w = mul_bf16x2(q.w, r.w);
                 lo.x = residual_bf16x2(q.x, r.x, hi.x); lo.y = residual_bf16x2(q.y, r.y, hi.y);
                 lo.z = residual_bf16x2(q.z, r.z, hi.z); lo.w = residual_bf16x2(q.w, r.w, hi.w);
-                if (in >= valid) hi = lo = make_uint4(0, 0, 0, 0);
+                if (!all && in >= valid) hi = lo = make_uint4(0, 0, 0, 0);         // rows behind the last key
                 st_shared_v4(tile_hi + at, hi.x, hi.y, hi.z, hi.w);
                 st_shared_v4(tile_hi + L::TILE + at, lo.x, lo.y, lo.z, lo.w);
+            };
+            if (valid == DEC_STRIP) {
+#pragma unroll 8
+                for (int i = 0; i < PASSES; ++i) build(i, true);
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < PASSES; ++i) build(i, false);
             }
             fence_async_smem();
             warp_arrive(&bars[DB_A_FULL0 + half], lane);
@@ -452,7 +467,10 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 ok = pipe_wait(&bars[DB_S_FULL0 + half], n & 1, fail, 2);
                 if (!ok) break;
                 tc_fence_after();
-                if (k + 1 == w.k1) fetch(p.Vr, w, tiles_at, row, valid);          // the tiles' last reader is done
+                if (k + 1 == w.k1) {                       // the tiles' last reader is done
+                    if (valid > 0) fetch(p.Vr, w, tiles_at, row);
+                    else copy_commit();
+                }
                 float col[4] = {0.f, 0.f, 0.f, 0.f};       // with masses: this warp's sums of columns c * 32 + lane
                 // Raises the strip's reference to the maximum over its rows if a row exceeds it by 2^8; what was summed so
                 // far follows.  (The products issued so far are complete: this step's scores came after them.)
@@ -626,20 +644,34 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     uint32_t o[2][16];
                     tmem_ld_16x256b_x4(tO + c * 32, o[0]);
                     tmem_ld_16x256b_x4(tO + (16u << 16) + c * 32, o[1]);
-                    tmem_wait_ld();
                     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    // the row's swizzle is the lane's own: rows eight apart share it
+                    const int r7 = (lane >> 2) & 7;
+                    const uint8_t* rows = tile_hi + (wq * 32 + (lane >> 2)) * 128 + (c >> 1) * 128 * 128 + (lane & 3) * 4;
+                    uint32_t u[4][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int in = (lane >> 2) + 8 * i;
-                        if (in >= valid_now) continue;     // rows behind the last key
+                    for (int k = 0; k < 4; ++k) {
+                        const uint8_t* piece = rows + ((((c & 1) * 4 + k) ^ r7) << 4);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t u = *reinterpret_cast<const uint32_t*>(tile_hi + sw128_offset<128>(wq * 32 + in, c * 4 + k) + (lane & 3) * 4);
-                            const float2 f = unpack_bf16x2(u);
+                        for (int i = 0; i < 4; ++i) u[i][k] = *reinterpret_cast<const uint32_t*>(piece + i * 1024);
+                    }
+                    tmem_wait_ld();
+                    if (valid_now < DEC_STRIP) {           // rows behind the last key
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if ((lane >> 2) + 8 * i >= valid_now) {
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) u[i][k] = o[i >> 1][k * 4 + (i & 1) * 2] = o[i >> 1][k * 4 + (i & 1) * 2 + 1] = 0u;
+                            }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = unpack_bf16x2(u[i][k]);
                             v[2 * k] += f.x * __uint_as_float(o[i >> 1][k * 4 + (i & 1) * 2]);
                             v[2 * k + 1] += f.y * __uint_as_float(o[i >> 1][k * 4 + (i & 1) * 2 + 1]);
                         }
-                    }
                     // v[2 k + e]: column 8 k + 2 (lane % 4) + e.  Bits 4, 3, 2 of the lane choose k's bits and e.
 #pragma unroll
                     for (int st = 0; st < 3; ++st) {
