@@ -493,82 +493,88 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     }
                 };
                 const uint64_t scale = pair_f32(p.c2, p.c2);
-                if (valid > 0 && w.s.seen - k * DEC_KEYS >= DEC_KEYS) {
-                    // a full step: 128 scores in registers
-                    uint32_t x[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, x[c]);
-                    tmem_wait_ld();
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[c][i]));
-                    renew(mx);
-                    // rows behind the last key contribute nothing: their exponent is -inf throughout
+                const int cols = w.s.seen - k * DEC_KEYS, chunks = w.chunks(k);          // visible columns of this step
+                // Exponentials of 32 scores relative to the reference: their sum, their BF16 pairs to tensor memory (P of
+                // chunk c covers score columns 16 c .. 16 c + 15, which are read by then), with masses the column sums.
+                // Rows behind the last key contribute nothing: their exponent is -inf throughout.
+                uint64_t s0 = pair_f32(0.f, 0.f), s1 = s0;
+                auto exponentials = [&](const uint32_t (&x)[32], int c) {
                     const float shift1 = lane < valid ? -ref : -INFINITY;
                     const uint64_t shift = pair_f32(shift1, shift1);
-                    uint64_t s0 = pair_f32(0.f, 0.f), s1 = s0;
+                    float v[32];
+                    uint32_t packed[16];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float v[32];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            float a, b;
-                            unpair_f32(fma_f32x2(pair_b32(x[c][i], x[c][i + 1]), scale, shift), a, b);
-                            v[i] = fast_exp2(a);
-                            v[i + 1] = fast_exp2(b);
-                            if (i & 2) s1 = add_f32x2(s1, pair_f32(v[i], v[i + 1]));
-                            else s0 = add_f32x2(s0, pair_f32(v[i], v[i + 1]));
-                            x[c >> 1][(c & 1) * 16 + i / 2] = pack_bf16x2(v[i], v[i + 1]);
-                        }
-                        if (MASS) col[c] = sgring::warp_transpose_sum(v, lane);
+                    for (int i = 0; i < 32; i += 2) {
+                        float a, b;
+                        unpair_f32(fma_f32x2(pair_b32(x[i], x[i + 1]), scale, shift), a, b);
+                        v[i] = fast_exp2(a);
+                        v[i + 1] = fast_exp2(b);
+                        if (i & 2) s1 = add_f32x2(s1, pair_f32(v[i], v[i + 1]));
+                        else s0 = add_f32x2(s0, pair_f32(v[i], v[i + 1]));
+                        packed[i / 2] = pack_bf16x2(v[i], v[i + 1]);
                     }
-                    tmem_st32(tS, x[0]);
-                    tmem_st32(tS + 32, x[1]);
-                    tmem_wait_st();
-                    float a, b;
-                    unpair_f32(add_f32x2(s0, s1), a, b);
-                    sum += a + b;
+                    tmem_st16(tS + c * 16, packed);
+                    if (MASS) {
+                        const float t = sgring::warp_transpose_sum(v, lane);
+                        col[0] = c == 0 ? t : col[0]; col[1] = c == 1 ? t : col[1];
+                        col[2] = c == 2 ? t : col[2]; col[3] = c == 3 ? t : col[3];
+                    }
+                };
+                // Two passes over the scores, the maximum and the exponentials, 64 columns at a time (the last step: 32), the
+                // scores read twice from tensor memory: with all 128 of them in registers and everything unrolled the code
+                // spills and outgrows the instruction cache, which holds all roles' code; with 32 at a time throughout, a
+                // step takes 2950 cycles.
+                if (valid > 0 && cols >= DEC_KEYS) {
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < 4; c += 2) {
+                        uint32_t x[2][32];
+                        tmem_ld32(tS + c * 32, x[0]);
+                        tmem_ld32(tS + c * 32 + 32, x[1]);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(x[0][i]), __uint_as_float(x[1][i])));
+                    }
+                    renew(mx);
+#pragma unroll 1
+                    for (int c = 0; c < 4; c += 2) {
+                        uint32_t x[2][32];
+                        tmem_ld32(tS + c * 32, x[0]);
+                        tmem_ld32(tS + c * 32 + 32, x[1]);
+                        tmem_wait_ld();
+                        exponentials(x[0], c);
+                        exponentials(x[1], c + 1);
+                    }
                 } else if (valid > 0) {
-                    // the last step: the chunks of 32 columns that hold keys, one after the other.  P of chunk c covers
-                    // score columns 16 c .. 16 c + 15, which are read by then.
-                    const int cols = w.s.seen - k * DEC_KEYS, chunks = w.chunks(k);
+                    auto load = [&](int c, uint32_t (&x)[32]) {
+                        tmem_ld32(tS + c * 32, x);
+                        tmem_wait_ld();
+                        if (c * 32 + 32 > cols) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) x[i] = c * 32 + i < cols ? x[i] : 0xFF800000u;          // -inf
+                        }
+                    };
                     float mx = -INFINITY;
 #pragma unroll 1
                     for (int c = 0; c < chunks; ++c) {
                         uint32_t x[32];
-                        tmem_ld32(tS + c * 32, x);
-                        tmem_wait_ld();
+                        load(c, x);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, c * 32 + i < cols ? __uint_as_float(x[i]) : -INFINITY);
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
                     }
                     renew(mx);
-                    const float shift1 = lane < valid ? -ref : -INFINITY;
-                    const uint64_t shift = pair_f32(shift1, shift1);
 #pragma unroll 1
                     for (int c = 0; c < chunks; ++c) {
-                        uint32_t x[32], packed[16];
-                        tmem_ld32(tS + c * 32, x);
-                        tmem_wait_ld();
-                        float v[32];
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            float a, b;
-                            unpair_f32(fma_f32x2(pair_b32(x[i], x[i + 1]), scale, shift), a, b);
-                            v[i] = c * 32 + i < cols ? fast_exp2(a) : 0.f;
-                            v[i + 1] = c * 32 + i + 1 < cols ? fast_exp2(b) : 0.f;
-                            sum += v[i] + v[i + 1];
-                            packed[i / 2] = pack_bf16x2(v[i], v[i + 1]);
-                        }
-                        tmem_st16(tS + c * 16, packed);
-                        if (MASS) {
-                            const float s = sgring::warp_transpose_sum(v, lane);
-                            col[0] = c == 0 ? s : col[0]; col[1] = c == 1 ? s : col[1];
-                            col[2] = c == 2 ? s : col[2]; col[3] = c == 3 ? s : col[3];
-                        }
+                        uint32_t x[32];
+                        load(c, x);
+                        exponentials(x, c);
                     }
+                }
+                if (valid > 0) {
                     tmem_wait_st();
+                    float a, b;
+                    unpair_f32(add_f32x2(s0, s1), a, b);
+                    sum += a + b;
                 }
                 tc_fence_before();
                 warp_arrive(&bars[DB_P_FULL0 + half], lane);
