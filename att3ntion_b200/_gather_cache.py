@@ -9,31 +9,36 @@ device, so captured graphs follow them; an entry outside its table is never foll
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
 from . import _cuda_kernels as _ck
 from ._cabi import lib
-from ._norm_rotate import _TYPE, _check_heads, _check_table, _forward_descriptors, _head_rows, _on_gpu, _scale
+from ._norm_rotate import _TYPE, _ZEROS, _Rows, _check_heads, _check_table, _on_gpu, _read, _scale
 
 _BF16 = torch.bfloat16
 _POOLS = ("R", "S", "Vr", "Vs")
 
 
 _NEW = ("R", "S", "Vr", "Vs", "Q")
-_NONE = (0, 0, 0)
 
 
 def _check_pools(who, pools):
     if len(pools) != 4:
         raise RuntimeError(f"{who}: pools are the four tensors R, S, Vr, Vs, got {len(pools)}")
     first = pools[0]
+    shape = dev = None
     for name, p in zip(_POOLS, pools):
-        if not isinstance(p, torch.Tensor) or p.dim() != 4 or p.dtype != _BF16 or not p.is_contiguous():
+        if not isinstance(p, torch.Tensor) or p.dtype is not _BF16 or p.dim() != 4 or not p.is_contiguous():
             raise RuntimeError(f"{who}: pool {name} must be a contiguous bf16 [pages,page_size,Hkv,D] tensor")
-        if p.shape != first.shape or p.device != first.device:
+        if shape is None:
+            shape, dev = p.shape, p.get_device()
+        elif p.shape != shape or p.get_device() != dev:
             raise RuntimeError(f"{who}: the pools must share one shape and device")
-    if first.numel() == 0:
+        if p.data_ptr() & 15:
+            raise RuntimeError(f"{who}: pool {name} must start on a 16-byte boundary")
+    if 0 in shape:
         raise RuntimeError(f"{who}: the pools are empty")
     return first
 
@@ -66,6 +71,12 @@ def _check_mass(who, mass, pool):
 
 def _pages(page_table, pool):
     return (C.c_int64 * 5)(page_table.data_ptr(), page_table.stride(0), page_table.shape[1], pool.shape[0], pool.shape[1])
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_workspace(device_index, *sizes):
+    """att3_sg_decode_workspace_bytes of these sizes on that device (current at the call)."""
+    return lib.att3_sg_decode_workspace_bytes(*sizes)
 
 
 def _no_grad(who, *tensors):
@@ -101,7 +112,7 @@ def gather_cache_append(pools, page_table, lengths, R, S, Vr, Vs, *, counts=None
     if len(ws) != 3:
         raise RuntimeError(f"{who}: weights are three scales, of Q, R and S")
     _no_grad(who, *new, *ws)
-    wq, wr, wsc = (_scale(w, who, f"weight {k}", D, dev) for k, w in enumerate(ws))
+    (wq, wq_at, wq_kind), (wr, wr_at, wr_kind), (wsc, ws_at, ws_kind) = (_scale(w, who, f"weight {k}", D, dev) for k, w in enumerate(ws))
     table, rows, rot = _check_table(who, table, D, dev)
     eps = float(eps)
     if not eps >= 0:
@@ -109,14 +120,20 @@ def gather_cache_append(pools, page_table, lengths, R, S, Vr, Vs, *, counts=None
     _on_gpu(who, pool)
     with _ck._on_device(dev):
         turn = 1 if rot else 0
-        desc = [(_head_rows(R), wr, turn, pools[0], _NONE), (_head_rows(S), wsc, turn, pools[1], _NONE),
-                (_head_rows(Vr), None, 0, pools[2], _NONE), (_head_rows(Vs), None, 0, pools[3], _NONE)]
+        words, held = [], []                                 # copies live until the launch
+        for x, w_at, kind, t, pool_of in ((R, wr_at, wr_kind, turn, pools[0]), (S, ws_at, ws_kind, turn, pools[1]),
+                                          (Vr, 0, 0, 0, pools[2]), (Vs, 0, 0, 0, pools[3])):
+            x, at, xb, xn, xh = _read(x)
+            words += (at, xb, xn, xh, w_at, kind, t, pool_of.data_ptr(), 0, 0, 0, *_ZEROS, Hkv)
+            held.append(x)
         out = None
         if Q is not None:
             Hq = Q.shape[2]
             out = torch.empty((B, T, Hq, D), dtype=_BF16, device=dev)
-            desc.append((_head_rows(Q), wq, turn, out, (T * Hq * D, Hq * D, D)))
-        _ck._call(lib.att3_gather_cache_append, _forward_descriptors(desc), len(desc), _TYPE[R.dtype], _ck._ptr(table), rows, rot,
+            x, at, xb, xn, xh = _read(Q)
+            words += (at, xb, xn, xh, wq_at, wq_kind, turn, out.data_ptr(), T * Hq * D, Hq * D, D, *_ZEROS, Hq)
+            held.append(x)
+        _ck._call(lib.att3_gather_cache_append, _Rows[len(new)](*words), len(new), _TYPE[R.dtype], _ck._ptr(table), rows, rot,
                   1 if interleaved else 0, _ck._ptr(positions), _pages(page_table, pool), lengths.data_ptr(),
                   _ck._ptr(counts), _ck._ptr(mass), B, T, D, eps, _ck._raw_stream(dev))
     return out
@@ -159,20 +176,20 @@ def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, ma
     _on_gpu(who, Q)
     slots = page_table.shape[1] * pool.shape[1]
     window, sinks = min(window, slots), min(sinks, slots)
-    q = Q.to(_BF16).contiguous()
-    if q.data_ptr() % 16:
+    q = Q if Q.dtype is _BF16 and Q.is_contiguous() else Q.to(_BF16).contiguous()
+    if q.data_ptr() & 15:
         q = q.clone()
     with _ck._on_device(Q.device):
         y = torch.empty((B, Hq, D), dtype=_BF16, device=Q.device)
         if B == 0:
             return y.to(Q.dtype)
-        nbytes = lib.att3_sg_decode_workspace_bytes(B, Hq, Hkv, D, window, sinks, slots, int(mass is not None))
+        nbytes = _decode_workspace(Q.device.index, B, Hq, Hkv, D, window, sinks, slots, 0 if mass is None else 1)
         # scratch of this call alone: a captured graph keeps it in its own pool
         ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
         _ck._call(lib.att3_sg_decode, q.data_ptr(), *(p.data_ptr() for p in pools), _ck._ptr(mass), y.data_ptr(),
                   _pages(page_table, pool), lengths.data_ptr(), B, Hq, Hkv, D, window, sinks, ws.data_ptr(), nbytes,
                   _ck._raw_stream(Q.device))
-    return y.to(Q.dtype)
+    return y if Q.dtype is _BF16 else y.to(Q.dtype)
 
 
 def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recent=0, out_table=None):

@@ -18,6 +18,7 @@ from ._cabi import lib
 
 _TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _HEAD_DIMS = (16, 32, 64, 128)
+_BF16 = torch.bfloat16
 
 
 def rotary_table(length: int, dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
@@ -47,14 +48,30 @@ def _strides(t: torch.Tensor):
     return a if B > 1 else 0, b if N > 1 else 0, c if H > 1 else 0
 
 
+def _read(t: torch.Tensor):
+    """(tensor that the kernels read, its address, its three strides) for a checked [B,N,H,D] tensor."""
+    at = t.data_ptr()
+    if not at & 15 and t.is_contiguous():
+        _, N, H, D = t.shape
+        return t, at, N * H * D, H * D, D
+    t = _head_rows(t)
+    return (t, t.data_ptr(), *_strides(t))
+
+
 def _scale(w, who: str, name: str, D: int, device):
+    """(scale that the kernels read, its address, its type's number); address 0 without one."""
     if w is None:
-        return None
-    if not isinstance(w, torch.Tensor) or w.dim() != 1 or w.shape[0] != D or w.dtype not in _TYPE:
+        return None, 0, 0
+    kind = _TYPE.get(w.dtype) if isinstance(w, torch.Tensor) else None
+    if kind is None or w.dim() != 1 or w.shape[0] != D:
         raise RuntimeError(f"{who}: {name} must be a [{D}] tensor of bf16, fp16 or fp32")
     if w.device != device:
         raise RuntimeError(f"{who}: {name} must be on the inputs' device")
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.detach().clone(memory_format=torch.contiguous_format)
+    at = w.data_ptr()
+    if at & 15 or not w.is_contiguous():
+        w = w.detach().clone(memory_format=torch.contiguous_format)
+        at = w.data_ptr()
+    return w, at, kind
 
 
 def _check_heads(who: str, xs, names):
@@ -62,23 +79,26 @@ def _check_heads(who: str, xs, names):
     x0 = xs[0]
     if not isinstance(x0, torch.Tensor) or x0.dim() != 4:
         raise RuntimeError(f"{who}: {names[0]} must be a [B,N,heads,D] tensor")
-    B, N, _, D = x0.shape
-    dtype, dev = x0.dtype, x0.device
-    for name, x in zip(names, xs):
-        if not isinstance(x, torch.Tensor) or x.dim() != 4:
-            raise RuntimeError(f"{who}: {name} must be a [B,N,heads,D] tensor")
-        if x.dtype != dtype or dtype not in _TYPE:
-            raise RuntimeError(f"{who}: all inputs must share one type of bf16, fp16 and fp32")
-        b, n, h, d = x.shape
-        if b != B or n != N or d != D:
-            raise RuntimeError(f"{who}: {name} is {tuple(x.shape)}, expected batch, length and head dim of {names[0]} "
-                               f"{tuple(x0.shape)}")
-        if x.device != dev:
-            raise RuntimeError(f"{who}: all inputs must be on one device")
-        if h < 1:
-            raise RuntimeError(f"{who}: {name} has no heads")
+    B, N, heads, D = x0.shape
+    dtype, dev = x0.dtype, x0.get_device()
+    if dtype not in _TYPE:
+        raise RuntimeError(f"{who}: all inputs must share one type of bf16, fp16 and fp32")
     if D not in _HEAD_DIMS:
         raise RuntimeError(f"{who}: head dim must be 16, 32, 64 or 128, got {D}")
+    for name, x in zip(names, xs):
+        if x is not x0:
+            if not isinstance(x, torch.Tensor) or x.dim() != 4:
+                raise RuntimeError(f"{who}: {name} must be a [B,N,heads,D] tensor")
+            b, n, heads, d = x.shape
+            if x.dtype is not dtype:
+                raise RuntimeError(f"{who}: all inputs must share one type of bf16, fp16 and fp32")
+            if b != B or n != N or d != D:
+                raise RuntimeError(f"{who}: {name} is {tuple(x.shape)}, expected batch, length and head dim of {names[0]} "
+                                   f"{tuple(x0.shape)}")
+            if x.get_device() != dev:
+                raise RuntimeError(f"{who}: all inputs must be on one device")
+        if heads < 1:
+            raise RuntimeError(f"{who}: {name} has no heads")
     return B, N, D
 
 
@@ -119,52 +139,36 @@ def _on_gpu(who: str, t: torch.Tensor) -> None:
 
 _ZEROS = (0,) * 9
 _NAMES = tuple(f"input {k}" for k in range(5))
-
-
-def _forward_descriptors(rows):
-    """att3_head_rows array from (x, w, rotate, y, y strides) per tensor."""
-    words = []
-    for x, w, rotate, y, y_strides in rows:
-        words += (x.data_ptr(), *_strides(x), w.data_ptr() if w is not None else 0, _TYPE[w.dtype] if w is not None else 0,
-                  rotate, y.data_ptr(), *y_strides, *_ZEROS, x.shape[2])
-    return (C.c_int64 * len(words))(*words)
-
-
-def _backward_descriptors(rows):
-    """The same from (x, w, dy, dx, dw)."""
-    words = []
-    for x, w, dy, dx, dw in rows:
-        words += (x.data_ptr(), *_strides(x), w.data_ptr() if w is not None else 0, _TYPE[w.dtype] if w is not None else 0,
-                  1, 0, 0, 0, 0, dy.data_ptr(), *_strides(dy), dx.data_ptr(), *_strides(dx),
-                  dw.data_ptr() if dw is not None else 0, x.shape[2])
-    return (C.c_int64 * len(words))(*words)
+_Rows = {n: C.c_int64 * (21 * n) for n in range(1, 6)}         # att3_head_rows arrays
 
 
 def _forward(xs, ws, table, positions, eps, interleaved, heads_first):
     who = "norm_rotate"
     B, N, D = _check_heads(who, xs, _NAMES)
-    dev, dtype = xs[0].device, xs[0].dtype
-    ws = [_scale(w, who, f"weight {k}", D, dev) if w is not None else None for k, w in enumerate(ws)]
+    dev, n = xs[0].device, len(xs)
     table, rows, rot = _check_table(who, table, D, dev)
     positions, pos_bytes, pos_b, pos_n = _check_positions(who, positions, B, N, dev)
     if positions is None and table is not None and N > rows:
         raise RuntimeError(f"{who}: {N} positions and a table of {rows}")
     if not eps >= 0:
         raise RuntimeError(f"{who}: eps must not be negative, got {eps}")
+    words, ys, held = [], [], []
+    scales = [_scale(w, who, f"weight {k}", D, dev) for k, w in enumerate(ws)]
     _on_gpu(who, xs[0])
     with _ck._on_device(dev):
-        ys, desc = [], []
-        for x, w in zip(xs, ws):
+        for x, (w, w_at, kind) in zip(xs, scales):
             H = x.shape[2]
+            x, at, xb, xn, xh = _read(x)
             if heads_first:
-                y = torch.empty((B, H, N, D), dtype=torch.bfloat16, device=dev)
-                strides = (H * N * D, D, N * D)
+                y = torch.empty((B, H, N, D), dtype=_BF16, device=dev)
+                yb, yn, yh = H * N * D, D, N * D
             else:
-                y = torch.empty((B, N, H, D), dtype=torch.bfloat16, device=dev)
-                strides = (N * H * D, H * D, D)
+                y = torch.empty((B, N, H, D), dtype=_BF16, device=dev)
+                yb, yn, yh = N * H * D, H * D, D
+            words += (at, xb, xn, xh, w_at, kind, 1, y.data_ptr(), yb, yn, yh, *_ZEROS, H)
             ys.append(y)
-            desc.append((_head_rows(x), w, 1, y, strides))
-        _ck._call(lib.att3_norm_rotate_forward, _forward_descriptors(desc), len(xs), _TYPE[dtype], _ck._ptr(table), rows, rot,
+            held.append(x)                                   # copies live until the launch
+        _ck._call(lib.att3_norm_rotate_forward, _Rows[n](*words), n, _TYPE[xs[0].dtype], _ck._ptr(table), rows, rot,
                   interleaved, _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, eps, _ck._raw_stream(dev))
     return ys
 
@@ -192,15 +196,20 @@ class _NormRotateFn(Function):
             # scratch of this call alone: a captured graph keeps it in its own pool
             nbytes = lib.att3_norm_rotate_workspace_bytes(ctx.n, D)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            desc, dxs, dws = [], [], []
+            words, held, dxs, dws = [], [], [], []
             for x, w, dy in zip(xs, ws, dys):
-                dy = _head_rows(dy.transpose(1, 2) if ctx.heads_first else dy)
-                dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+                H, dtype = x.shape[2], x.dtype
+                dx = torch.empty(x.shape, dtype=dtype, device=dev)
                 dw = torch.empty(D, dtype=torch.float32, device=dev) if w is not None else None
-                desc.append((_head_rows(x), _scale(w, who, "weight", D, dev), dy, dx, dw))
+                w, w_at, kind = _scale(w, who, "weight", D, dev)
+                dy, dy_at, gb, gn, gh = _read(dy.transpose(1, 2) if ctx.heads_first else dy)
+                x, at, xb, xn, xh = _read(x)
+                words += (at, xb, xn, xh, w_at, kind, 1, 0, 0, 0, 0, dy_at, gb, gn, gh, dx.data_ptr(), N * H * D, H * D, D,
+                          dw.data_ptr() if dw is not None else 0, H)
+                held += (x, w, dy)
                 dxs.append(dx)
                 dws.append(dw)
-            _ck._call(lib.att3_norm_rotate_backward, _backward_descriptors(desc), ctx.n, _TYPE[xs[0].dtype], _ck._ptr(table), rows,
+            _ck._call(lib.att3_norm_rotate_backward, _Rows[ctx.n](*words), ctx.n, _TYPE[dtype], _ck._ptr(table), rows,
                       rot, ctx.interleaved, _ck._ptr(positions), pos_bytes, pos_b, pos_n, B, N, D, ctx.eps,
                       scratch.data_ptr(), nbytes, _ck._raw_stream(dev))
         dws = [dw if w is None or w.dtype == torch.float32 else dw.to(w.dtype) for w, dw in zip(ws, dws)]

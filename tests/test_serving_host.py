@@ -1,9 +1,11 @@
 """What the serving operators refuse, and their host-side logic: no GPU needed."""
 import ctypes as C
+import re
 
 import pytest
 import torch
 
+from conftest import REPO
 from att3ntion_b200 import (GatherCache, HypergraphAttention, _cabi, gather_cache_append, gather_cache_evict, norm_rotate,
                             rotary_table, single_gather_decode, window_mask)
 
@@ -14,9 +16,14 @@ INT = torch.int32
 def test_word_counts_of_the_structs():
     """The callers pass the structs as arrays of 64-bit integers: 21 and 5 of them."""
     from att3ntion_b200 import _gather_cache as gc, _norm_rotate as nr
-    x = torch.zeros(1, 2, 3, 64)
-    assert len(nr._forward_descriptors([(x, None, 1, x, (0, 0, 0))] * 2)) == 2 * _cabi.HEAD_ROWS_WORDS
-    assert len(nr._backward_descriptors([(x, x[0, 0, 0], x, x, x)])) == _cabi.HEAD_ROWS_WORDS
+    header = (REPO / "include" / "att3_b200.h").read_text()
+
+    def count(name):
+        body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), header, re.S).group(1), flags=re.S)
+        return sum(int(m.group(1) or 1) for m in re.finditer(r"\w+(?:\[(\d+)\])?;", body))
+
+    assert count("att3_head_rows") == _cabi.HEAD_ROWS_WORDS == len(nr._Rows[1]()) and len(nr._Rows[5]()) == 5 * _cabi.HEAD_ROWS_WORDS
+    assert count("att3_gather_pages") == _cabi.GATHER_PAGES_WORDS
     assert len(gc._pages(torch.zeros(1, 2, dtype=INT), torch.zeros(4, 16, 1, 64))) == _cabi.GATHER_PAGES_WORDS
 
 
