@@ -326,9 +326,9 @@ def single_gather_shared_backward(dY, Q, R, S, Vr, Vs, Y, m, l, mask, window=128
 
 def tc_launches():
     """Launch counters (cpp/cuda_bindings.cpp:31-41)."""
-    c = [int(lib.att3_launch_count(i)) for i in range(4)]
+    c = [int(lib.att3_launch_count(i)) for i in range(5)]
     return {"forward": c[2], "backward": c[3], "sg_forward": c[0], "sg_backward": c[1],
-            "sg_shared_forward": c[0], "sg_shared_backward": c[1]}
+            "sg_shared_forward": c[0], "sg_shared_backward": c[1], "serving": c[4]}
 
 
 def sg_dispatch():

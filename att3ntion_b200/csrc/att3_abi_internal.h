@@ -23,7 +23,7 @@ int sm_count();
 void count_launch(int which, int n = 1);
 
 // Kernel ids of att3_timing_read().
-enum KernelId { K_SG_FWD = 0, K_SG_BWD = 1, K_SG_REDUCE = 2, K_DENSE_FWD = 3, K_DENSE_BWD = 4, K_HG_AUX = 5, K_COUNT = 6 };
+enum KernelId { K_SG_FWD = 0, K_SG_BWD = 1, K_SG_REDUCE = 2, K_DENSE_FWD = 3, K_DENSE_BWD = 4, K_HG_AUX = 5, K_SERVE = 6, K_COUNT = 7 };
 
 // Brackets one kernel launch with CUDA events on its stream while timing is
 // enabled (att3_timing_enable); a no-op otherwise.

@@ -13,7 +13,7 @@
 namespace att3 {
 
 static thread_local char g_err[512] = "";
-static std::atomic<unsigned long long> g_launches[4];
+static std::atomic<unsigned long long> g_launches[5];
 
 int set_error(int code, const char* fmt, ...) {
     va_list ap;
@@ -58,7 +58,7 @@ int sm_count() {
 }
 
 void count_launch(int which, int n) {
-    if (which >= 0 && which < 4) g_launches[which] += n;
+    if (which >= 0 && which < 5) g_launches[which] += n;
 }
 
 // ---- optional per-kernel timing ------------------------------------------------
@@ -170,7 +170,7 @@ extern "C" const char* att3_last_error(void) { return att3::g_err; }
 extern "C" int att3_abi_version(void) { return 2; }
 
 extern "C" unsigned long long att3_launch_count(int which) {
-    return (which >= 0 && which < 4) ? att3::g_launches[which].load() : 0ull;
+    return (which >= 0 && which < 5) ? att3::g_launches[which].load() : 0ull;
 }
 
 // Rows and columns a windowed single-gather work item has to visit.  The

@@ -54,6 +54,8 @@ int launch(const serve::DecodeParams& p, const Layout& lay, long long max_seen, 
     constexpr int smem = serve::DecSmem<D>::BYTES;
     cudaError_t e = cudaFuncSetAttribute(serve::decode_kernel<D, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return att3::set_cuda_error(e, who);
+    att3::count_launch(4, MASS ? 3 : 2);
+    const att3::TimedLaunch timed(att3::K_SERVE, st);
     serve::decode_kernel<D, MASS><<<lay.ctas, serve::DEC_THREADS, smem, st>>>(p);
     // the joining kernels may be set up while the one before them runs out; they wait for its end themselves
     cudaLaunchAttribute early = {};

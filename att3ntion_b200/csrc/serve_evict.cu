@@ -265,6 +265,8 @@ extern "C" int att3_gather_cache_evict(void* R, void* S, void* Vr, void* Vs, flo
     const int smem = p.cached ? static_cast<int>(most) * 4 : 0;
     cudaError_t e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_SMEM_KEYS * 4);
     if (e != cudaSuccess) return att3::set_cuda_error(e, who);
+    att3::count_launch(4, 2);
+    const att3::TimedLaunch timed(att3::K_SERVE, st);
     select_kernel<<<B * Hkv, SEL_THREADS, smem, st>>>(p);
     // the second kernel may be set up while the first runs out; it waits for its end itself
     cudaLaunchAttribute early = {};

@@ -482,6 +482,8 @@ template <bool PAGED>
 int launch_forward(const Params& p, int x_type, int D, cudaStream_t st, const char* who) {
     const int blocks = total_blocks(p);
     if (blocks == 0) return ATT3_OK;
+    att3::count_launch(4);
+    const att3::TimedLaunch timed(att3::K_SERVE, st);
 #define ATT3_NR(T, DD) norm_rotate_kernel<T, DD, PAGED><<<blocks, THREADS, 0, st>>>(p)
 #define ATT3_NR_D(T) do { if (D == 16) ATT3_NR(T, 16); else if (D == 32) ATT3_NR(T, 32); else if (D == 64) ATT3_NR(T, 64); else ATT3_NR(T, 128); } while (0)
     if (x_type == 0) ATT3_NR_D(__nv_bfloat16);
@@ -576,6 +578,8 @@ extern "C" int att3_norm_rotate_backward(const att3_head_rows* tensors, int n, i
     if (!(p.status = att3::serve_status_ptr())) return att3::set_error(ATT3_ERR_CUDA, "%s: status word not resolvable", who);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int blocks = total_blocks(p);
+    att3::count_launch(4, (blocks ? 1 : 0) + (scaled ? 1 : 0));
+    const att3::TimedLaunch timed(att3::K_SERVE, st);
     if (blocks) {
 #define ATT3_NR(T, DD) norm_rotate_backward_kernel<T, DD><<<blocks, THREADS, 0, st>>>(p)
 #define ATT3_NR_D(T) do { if (D == 16) ATT3_NR(T, 16); else if (D == 32) ATT3_NR(T, 32); else if (D == 64) ATT3_NR(T, 64); else ATT3_NR(T, 128); } while (0)

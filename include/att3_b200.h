@@ -55,7 +55,8 @@ int att3_abi_version(void);
  * commit arrives on) has an iteration limit; a wait that runs out sets a sticky
  * status word on the device and the kernel leaves through its normal exit, so
  * the context stays usable.  This call synchronises `stream`, reads and clears
- * the word of the current device and returns ATT3_OK or ATT3_ERR_TIMEOUT.  The
+ * the word of the current device and returns ATT3_OK, ATT3_ERR_TIMEOUT or, where a
+ * serving call met a bad entry in one of its tables, ATT3_ERR_INVALID.  The
  * reference has no counterpart (its kernels have no device-side waits). */
 int att3_device_status(void* stream);
 
@@ -394,7 +395,7 @@ int att3_sg_set_packed(int on);
 
 /* Launch counters, the counterpart of att3_tc::State (cpp/cuda_bindings.h:18-48).
  * which: 0 single-gather forward, 1 single-gather backward, 2 three-gather
- * forward, 3 three-gather backward.  Returns kernels launched so far. */
+ * forward, 3 three-gather backward, 4 serving.  Returns kernels launched so far. */
 unsigned long long att3_launch_count(int which);
 
 /* Per-kernel device timing for benchmarks (no counterpart in the reference,
@@ -403,7 +404,8 @@ unsigned long long att3_launch_count(int which);
  * stream.  att3_timing_read waits for the recorded launches of one kernel,
  * returns their summed duration and count, and forgets them.  kernel_id:
  * 0 windowed forward, 1 windowed backward pass, 2 key-gradient reduction,
- * 3 dense forward, 4 dense backward, 5 three-gather helpers.
+ * 3 dense forward, 4 dense backward, 5 three-gather helpers, 6 serving (a call's
+ * kernels together).
  * att3_timing_enable returns the previous setting. */
 int att3_timing_enable(int on);
 int att3_timing_read(int kernel_id, double* total_ms, unsigned long long* launches);
