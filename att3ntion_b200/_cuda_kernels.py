@@ -39,28 +39,6 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-class _on_device:
-    """torch.cuda.device(dev) for the short calls of serving: does nothing where `dev` is current already."""
-    __slots__ = ("index", "previous")
-
-    def __init__(self, dev: torch.device):
-        self.index = dev.index
-
-    def __enter__(self):
-        self.previous = torch.cuda.current_device()
-        if self.previous != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.previous != self.index:
-            torch.cuda.set_device(self.previous)
-
-
-def _raw_stream(dev: torch.device) -> int:
-    """The current stream's handle without the Stream object around it."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
-
-
 def _workspace(device, nbytes: int) -> torch.Tensor:
     """Scratch buffer cached per device and stream (two streams must not share one: their kernels may
     overlap).  A buffer grows on demand; at most `_MAX_WORKSPACES` are kept, least recently used first

@@ -8,14 +8,10 @@ device, so captured graphs follow them; an entry outside its table is never foll
 """
 from __future__ import annotations
 
-import ctypes as C
-import functools
-
 import torch
 
-from . import _cuda_kernels as _ck
-from ._cabi import lib
-from ._norm_rotate import _TYPE, _ZEROS, _Rows, _check_heads, _check_table, _on_gpu, _read, _scale
+from . import _serve_native as _native
+from ._norm_rotate import _accepted, _check_eps, _check_heads, _check_scale, _check_table, _on_gpu
 
 _BF16 = torch.bfloat16
 _POOLS = ("R", "S", "Vr", "Vs")
@@ -69,16 +65,6 @@ def _check_mass(who, mass, pool):
         raise RuntimeError(f"{who}: mass must be a contiguous FP32 {tuple(pool.shape[:3])} tensor on the pools' device")
 
 
-def _pages(page_table, pool):
-    return (C.c_int64 * 5)(page_table.data_ptr(), page_table.stride(0), page_table.shape[1], pool.shape[0], pool.shape[1])
-
-
-@functools.lru_cache(maxsize=256)
-def _decode_workspace(device_index, *sizes):
-    """att3_sg_decode_workspace_bytes of these sizes on that device (current at the call)."""
-    return lib.att3_sg_decode_workspace_bytes(*sizes)
-
-
 def _no_grad(who, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{who}: has no gradient; call it under torch.no_grad()")
@@ -94,13 +80,20 @@ def gather_cache_append(pools, page_table, lengths, R, S, Vr, Vs, *, counts=None
     through the same pass and is returned as bf16, all T rows of it.  mass, if given, is zeroed at the slots written.
     No two sequences may write the same slot of a page.  A slot behind the page table's end, or on a page that the pool
     does not have, is left out and reported by `device_status()`."""
+    weights = (None,) * 3 if weights is None else weights
+    got = _accepted(_native.append, pools, page_table, lengths, R, S, Vr, Vs, counts, Q, weights, table, positions, mass, eps, interleaved)
+    if got is None:
+        _refuse_append(pools, page_table, lengths, (R, S, Vr, Vs) if Q is None else (R, S, Vr, Vs, Q), counts, weights, table, positions,
+                       mass, eps)
+    return got if Q is not None else None
+
+
+def _refuse_append(pools, page_table, lengths, new, counts, weights, table, positions, mass, eps):
     who = "gather_cache_append"
     pool = _check_pools(who, pools)
-    new = (R, S, Vr, Vs) if Q is None else (R, S, Vr, Vs, Q)
     B, T, D = _check_heads(who, new, _NEW)
-    dev = pool.device
-    Hkv = pool.shape[2]
-    if R.device != dev or D != pool.shape[3] or not (R.shape[2] == S.shape[2] == Vr.shape[2] == Vs.shape[2] == Hkv):
+    dev, Hkv = pool.device, pool.shape[2]
+    if new[0].device != dev or D != pool.shape[3] or any(x.shape[2] != Hkv for x in new[:4]):
         raise RuntimeError(f"{who}: new rows must be [B,T,{Hkv},{pool.shape[3]}] on the pools' device")
     _check_table_of_pages(who, page_table, lengths, dev, B=B)
     if counts is not None:
@@ -108,35 +101,15 @@ def gather_cache_append(pools, page_table, lengths, R, S, Vr, Vs, *, counts=None
     if positions is not None:
         _check_ints(who, "positions", positions, B, dev)
     _check_mass(who, mass, pool)
-    ws = (None,) * 3 if weights is None else tuple(weights)
-    if len(ws) != 3:
+    if len(weights) != 3:
         raise RuntimeError(f"{who}: weights are three scales, of Q, R and S")
-    _no_grad(who, *new, *ws)
-    (wq, wq_at, wq_kind), (wr, wr_at, wr_kind), (wsc, ws_at, ws_kind) = (_scale(w, who, f"weight {k}", D, dev) for k, w in enumerate(ws))
-    table, rows, rot = _check_table(who, table, D, dev)
-    eps = float(eps)
-    if not eps >= 0:
-        raise RuntimeError(f"{who}: eps must not be negative, got {eps}")
+    _no_grad(who, *new, *weights)
+    for k, w in enumerate(weights):
+        _check_scale(w, who, f"weight {k}", D, dev)
+    _check_table(who, table, D, dev)
+    _check_eps(who, eps)
     _on_gpu(who, pool)
-    with _ck._on_device(dev):
-        turn = 1 if rot else 0
-        words, held = [], []                                 # copies live until the launch
-        for x, w_at, kind, t, pool_of in ((R, wr_at, wr_kind, turn, pools[0]), (S, ws_at, ws_kind, turn, pools[1]),
-                                          (Vr, 0, 0, 0, pools[2]), (Vs, 0, 0, 0, pools[3])):
-            x, at, xb, xn, xh = _read(x)
-            words += (at, xb, xn, xh, w_at, kind, t, pool_of.data_ptr(), 0, 0, 0, *_ZEROS, Hkv)
-            held.append(x)
-        out = None
-        if Q is not None:
-            Hq = Q.shape[2]
-            out = torch.empty((B, T, Hq, D), dtype=_BF16, device=dev)
-            x, at, xb, xn, xh = _read(Q)
-            words += (at, xb, xn, xh, wq_at, wq_kind, turn, out.data_ptr(), T * Hq * D, Hq * D, D, *_ZEROS, Hq)
-            held.append(x)
-        _ck._call(lib.att3_gather_cache_append, _Rows[len(new)](*words), len(new), _TYPE[R.dtype], _ck._ptr(table), rows, rot,
-                  1 if interleaved else 0, _ck._ptr(positions), _pages(page_table, pool), lengths.data_ptr(),
-                  _ck._ptr(counts), _ck._ptr(mass), B, T, D, eps, _ck._raw_stream(dev))
-    return out
+    raise RuntimeError(f"{who}: arguments of a type or size that the kernels do not take")
 
 
 def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, mass=None):
@@ -151,6 +124,13 @@ def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, ma
     mass (FP32 [pages,page_size,Hkv]), if given, gains every visible slot's share of the attention: the mean over the
     key head's query heads of half the probability of the pairs that hold the slot as j plus half of those that hold it
     as k, 1 in all for every sequence and key head.  No two sequences of a call with masses may share a page."""
+    y = _accepted(_native.decode, Q, pools, page_table, lengths, window, sinks, mass)
+    if y is None:
+        _refuse_decode(Q, pools, page_table, lengths, window, sinks, mass)
+    return y
+
+
+def _refuse_decode(Q, pools, page_table, lengths, window, sinks, mass):
     who = "single_gather_decode"
     pool = _check_pools(who, pools)
     if not isinstance(Q, torch.Tensor) or Q.dim() != 3 or not Q.is_floating_point():
@@ -166,30 +146,14 @@ def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, ma
     if Q.device != pool.device:
         raise RuntimeError(f"{who}: Q must be on the pools' device")
     _check_table_of_pages(who, page_table, lengths, pool.device, B=B)
-    window, sinks = int(window), int(sinks)
-    if window < 0 or sinks < 0:
+    if int(window) < 0 or int(sinks) < 0:
         raise RuntimeError(f"{who}: window and sinks must not be negative, got {window}, {sinks}")
     if sinks and not window:
         raise RuntimeError(f"{who}: sinks go with a window")
     _check_mass(who, mass, pool)
     _no_grad(who, Q, *pools)
     _on_gpu(who, Q)
-    slots = page_table.shape[1] * pool.shape[1]
-    window, sinks = min(window, slots), min(sinks, slots)
-    q = Q if Q.dtype is _BF16 and Q.is_contiguous() else Q.to(_BF16).contiguous()
-    if q.data_ptr() & 15:
-        q = q.clone()
-    with _ck._on_device(Q.device):
-        y = torch.empty((B, Hq, D), dtype=_BF16, device=Q.device)
-        if B == 0:
-            return y.to(Q.dtype)
-        nbytes = _decode_workspace(Q.device.index, B, Hq, Hkv, D, window, sinks, slots, 0 if mass is None else 1)
-        # scratch of this call alone: a captured graph keeps it in its own pool
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
-        _ck._call(lib.att3_sg_decode, q.data_ptr(), *(p.data_ptr() for p in pools), _ck._ptr(mass), y.data_ptr(),
-                  _pages(page_table, pool), lengths.data_ptr(), B, Hq, Hkv, D, window, sinks, ws.data_ptr(), nbytes,
-                  _ck._raw_stream(Q.device))
-    return y if Q.dtype is _BF16 else y.to(Q.dtype)
+    raise RuntimeError(f"{who}: arguments of a type or size that the kernels do not take")
 
 
 def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recent=0, out_table=None):
@@ -200,9 +164,16 @@ def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recen
     sequence may keep different slots.
 
     Returns (kept int32 [B,Hkv,keep], the slots that stayed, -1 behind the last; new lengths int32 [B])."""
+    got = _accepted(_native.evict, pools, mass, page_table, lengths, keep, sinks, recent, out_table)
+    if got is None:
+        _refuse_evict(pools, mass, page_table, lengths, keep, sinks, recent, out_table)
+    return got
+
+
+def _refuse_evict(pools, mass, page_table, lengths, keep, sinks, recent, out_table):
     who = "gather_cache_evict"
     pool = _check_pools(who, pools)
-    Hkv, D = pool.shape[2:]
+    D = pool.shape[3]
     if D not in (16, 32, 64, 128):
         raise RuntimeError(f"{who}: head dim must be 16, 32, 64 or 128, got {D}")
     if mass is None:
@@ -210,23 +181,15 @@ def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recen
     _check_mass(who, mass, pool)
     _check_table_of_pages(who, page_table, lengths, pool.device)
     B = page_table.shape[0]
-    keep, sinks, recent = int(keep), int(sinks), int(recent)
-    if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+    if int(keep) < 1 or int(sinks) < 0 or int(recent) < 0 or int(sinks) + int(recent) > int(keep):
         raise RuntimeError(f"{who}: sinks + recent must fit in keep >= 1, got {sinks} + {recent} in {keep}")
     slots = page_table.shape[1] * pool.shape[1]
     if out_table is not None:
         _check_table_of_pages(who, out_table, None, pool.device, "out_table", B)
-        if out_table.shape[1] * pool.shape[1] < min(keep, slots):
-            raise RuntimeError(f"{who}: out_table has no room for {min(keep, slots)} slots")
+        if out_table.shape[1] * pool.shape[1] < min(int(keep), slots):
+            raise RuntimeError(f"{who}: out_table has no room for {min(int(keep), slots)} slots")
     _on_gpu(who, pool)
-    with _ck._on_device(pool.device):
-        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=pool.device)
-        left = torch.empty(B, dtype=torch.int32, device=pool.device)
-        if B:
-            _ck._call(lib.att3_gather_cache_evict, *(p.data_ptr() for p in pools), mass.data_ptr(), _pages(page_table, pool),
-                      _pages(out_table if out_table is not None else page_table, pool), lengths.data_ptr(), left.data_ptr(),
-                      kept.data_ptr(), B, Hkv, D, keep, sinks, recent, _ck._raw_stream(pool.device))
-    return kept, left
+    raise RuntimeError(f"{who}: arguments of a type or size that the kernels do not take")
 
 
 class GatherCache:
