@@ -14,9 +14,9 @@
 // registers.  D / 8 neighbouring lanes hold a row, eight columns a lane.  Which eight follows the rotation: four of the
 // first half of the rotated columns and their four partners, or neighbours; so a lane turns its pairs by itself with
 // four angles, and only the mean needs the row's other lanes.  (Eight neighbouring columns a lane, the partner's fetched
-// by shuffles, took 394 instructions a row and direction and 2.3 TB/s in the backward.)  A group of lanes takes
-// several heads of one token, whose angles are fetched once for them, or the heads of several tokens where there are
-// few.  All of a call's tensors go in one launch, each with its own range of blocks.  The backward keeps the columns of
+// by shuffles, took 394 instructions for two rows of 128 and 2.3 TB/s in the backward.)  A group of lanes takes up to
+// eight rows in a line: heads of one token, whose angles are fetched once for them, or, of a tensor with one head,
+// neighbouring tokens; so that what a row costs beyond its arithmetic is a step of a pointer.  All of a call's tensors go in one launch, each with its own range of blocks.  The backward keeps the columns of
 // dw that a lane owns in registers over all rows that it visits and has the next rows on their way while it works;
 // blocks write their sums to a plane each, which a second kernel adds in a fixed order, so that repeated calls agree to
 // the bit.
@@ -33,7 +33,8 @@ using serve::Four;
 __device__ int g_serve_status = 0;
 
 constexpr int THREADS = 256;
-constexpr int FWD_ROWS = 4, BWD_ROWS = 2;           // rows of an item, the unit of work of D / 8 lanes
+constexpr int LINE = 8;                            // rows of an item, the unit of work of D / 8 lanes
+constexpr int FWD_ROWS = 4, BWD_ROWS = 2;          // rows in flight
 constexpr int MAX_TENSORS = 5;
 constexpr int FWD_BLOCKS_PER_SM = 16, BWD_BLOCKS_PER_SM = 6;       // at most; a block then takes several items a group
 
@@ -47,9 +48,8 @@ struct Tensor {
     long long xb, yb, dyb, dxb;                    // strides of the batch, then of the position and the head, in elements
     int xn, xh, yn, yh, dyn, dyh, dxn, dxh;
     int w_type, rotate, heads, block0, blocks;
-    int per_token, tokens_per;                     // items of a token, or tokens of an item
-    serve::Divide by_per_token;
-    int items;                                     // in all
+    serve::Divide by_lines;                        // items of a token, or (one head) of a sequence
+    int lines, items;
 };
 
 struct Params {
@@ -59,7 +59,7 @@ struct Params {
     const void* positions;
     long long pos_b, pos_n;
     int pos_bytes, table_rows, rot, interleaved;
-    int B, N, tokens;
+    int B, N;
     serve::Divide by_N;
     float eps;
     float* partial;                                // backward: [blocks][D]
@@ -164,24 +164,15 @@ __device__ __forceinline__ int find_tensor(const Params& p) {
     return ti;
 }
 
-// The first row of an item and how many it has; row u is the next head, or the head of the next token.
+// The first row of an item and how many it has; the following ones are the next heads or, of a tensor with ONE head, the
+// next positions.
 struct Place { int b, n, head, rows; };
-template <int ROWS>
-__device__ __forceinline__ Place place_of(const Params& p, int heads, int per_token, const serve::Divide& by_per_token, int tokens_per, int item) {
-    Place at;
-    int token;
-    if (tokens_per > 1) {
-        token = item * tokens_per;
-        at.head = 0;
-        at.rows = min(tokens_per, p.tokens - token);
-    } else {
-        token = by_per_token(item);
-        at.head = (item - token * per_token) * ROWS;
-        at.rows = token < p.tokens ? min(ROWS, heads - at.head) : 0;
-    }
-    at.b = p.by_N(token);
-    at.n = token - at.b * p.N;
-    return at;
+template <bool ONE>
+__device__ __forceinline__ Place place_of(const Params& p, const Tensor& t, int item) {
+    const int outer = t.by_lines(item), start = (item - outer * t.lines) * LINE;
+    if (ONE) return Place{outer, start, 0, min(LINE, p.N - start)};
+    const int b = p.by_N(outer);
+    return Place{b, outer - b * p.N, start, min(LINE, t.heads - start)};
 }
 
 __device__ __forceinline__ int position_of(const Params& p, int b, int n) {
@@ -199,95 +190,169 @@ __device__ __forceinline__ int position_of(const Params& p, int b, int n) {
 
 // PAGED: the results of all tensors but the fifth (the queries) go to the cache rows of slot lengths[b] + n, and that
 // slot is the position unless `positions` names the position of the first new token.
-template <typename XT, int D, bool PAGED>
-__global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 4 : 3) norm_rotate_kernel(const __grid_constant__ Params p) {
-    constexpr int LANES = D / 8;
-    const int ti = find_tensor(p);
-    const Tensor& t = p.t[ti];
-    const int lr = threadIdx.x % LANES, tokens_per = t.tokens_per, heads = t.heads, per_token = t.per_token, items = t.items;
-    const serve::Divide by_per_token = t.by_per_token;
+template <typename XT, int D, bool PAGED, bool ONE>
+__device__ __forceinline__ void forward_rows(const Params& p, const Tensor& t, int ti) {
+    constexpr int LANES = D / 8, GROUPS = THREADS / LANES;
+    const int lr = threadIdx.x % LANES;
     const Columns cols = columns_of(p, lr);
-    const bool several = tokens_per > 1;
     const bool turns = t.rotate && cols.turns, normed = t.w != nullptr, interleaved = p.interleaved != 0;
     const bool to_cache = PAGED && ti < 4;
     const float eps = p.eps;
-    const XT* const x0 = static_cast<const XT*>(t.x);
+    const long long step_x = ONE ? t.xn : t.xh, step_y = to_cache ? D : ONE ? t.yn : t.yh;
     __nv_bfloat16* const y0 = static_cast<__nv_bfloat16*>(t.y);
-    const long long xb = t.xb, yb = t.yb;
-    const int xn = t.xn, xh = t.xh, yn = t.yn, step = to_cache ? D : t.yh;
     float w[8];
     if (normed) load_scale(t, cols, w);
-
-    // the next token's batch and position
-    auto after = [&](int& b, int& n) { if (++n == p.N) { n = 0; ++b; } };
-    const int stride = t.blocks * (THREADS / LANES);
+    const int items = t.items, stride = t.blocks * GROUPS;
     // every lane of a warp makes the same number of turns: the shuffles want all of them
-    for (int base = (blockIdx.x - t.block0) * (THREADS / LANES); base < items; base += stride) {
+    for (int base = (blockIdx.x - t.block0) * GROUPS; base < items; base += stride) {
         const int item = base + threadIdx.x / LANES;
         Place at{0, 0, 0, 0};
-        if (item < items) at = place_of<FWD_ROWS>(p, heads, per_token, by_per_token, tokens_per, item);
-        Row8<XT> raw[FWD_ROWS];
-        {
-            int b = at.b, n = at.n;
-            const XT* x = x0 + b * xb + static_cast<long long>(n) * xn + static_cast<long long>(at.head) * xh;
-#pragma unroll
-            for (int u = 0; u < FWD_ROWS; ++u) {
-                if (u < at.rows) raw[u].load(x, cols);
-                if (several) {
-                    after(b, n);
-                    x = x0 + b * xb + static_cast<long long>(n) * xn;
-                } else x += xh;
+        if (item < items) at = place_of<ONE>(p, t, item);
+        const XT* x = static_cast<const XT*>(t.x) + at.b * t.xb + static_cast<long long>(at.n) * t.xn + static_cast<long long>(at.head) * t.xh;
+        // where the rows go, and the position of the first
+        __nv_bfloat16* y = y0 + at.b * t.yb + static_cast<long long>(at.n) * t.yn + static_cast<long long>(at.head) * t.yh;
+        int slot = 0;                                      // of the first row in the cache
+        long long first = 0;
+        if (PAGED && at.rows > 0) {
+            slot = __ldg(p.lengths + at.b) + at.n;
+            first = p.positions ? static_cast<long long>(static_cast<const int*>(p.positions)[at.b]) + at.n : slot;
+            if (to_cache && p.counts) {                    // what is not stored is not read either
+                const int left = __ldg(p.counts + at.b) - at.n;
+                at.rows = ONE ? max(0, min(at.rows, left)) : left > 0 ? at.rows : 0;
             }
         }
+        auto position = [&](int u) {                       // of row u
+            if (!PAGED) return position_of(p, at.b, at.n + (ONE ? u : 0));
+            const long long q = first + (ONE ? u : 0);
+            if (q >= 0 && q < p.table_rows) return static_cast<int>(q);
+            serve::report(p.status, serve::ST_POSITION);
+            return 0;
+        };
+        auto cached = [&](int u) -> __nv_bfloat16* {       // the cache's row of token u, head `at.head`; none where it has no page
+            const int row = p.pages.row(at.b, slot + u);
+            if (row >= 0) return y0 + static_cast<long long>(row) * p.Hkv * D + at.head * D;
+            serve::report(p.status, serve::ST_PAGE);
+            return nullptr;
+        };
         Angles angles;
-        __nv_bfloat16* dst = nullptr;                                   // where the row goes, or nowhere
-        int b = at.b, n = at.n;
+        if (!ONE) {
+            angles = load_angles(p, turns && at.rows > 0 ? position(0) : 0, lr, turns);
+            if (to_cache) y = at.rows > 0 ? cached(0) : nullptr;
+        }
+        const int line = ONE ? LINE : min(LINE, t.heads);  // the same for the whole block
+#pragma unroll 1
+        for (int r = 0; r < line; r += FWD_ROWS) {
+            Row8<XT> raw[FWD_ROWS];
 #pragma unroll
-        for (int u = 0; u < FWD_ROWS; ++u) {
-            if (several ? u >= tokens_per : u >= heads) break;          // the same for the whole block
-            if (u == 0 || several) {
-                int pos = 0;
-                dst = nullptr;
-                if (u < at.rows) {
-                    if (PAGED) {
-                        const int slot = __ldg(p.lengths + b) + n;
-                        if (turns) {
-                            long long q = p.positions ? static_cast<long long>(static_cast<const int*>(p.positions)[b]) + n : slot;
-                            if (q < 0 || q >= p.table_rows) { serve::report(p.status, serve::ST_POSITION); q = 0; }
-                            pos = static_cast<int>(q);
-                        }
-                        if (!to_cache) dst = y0 + b * yb + static_cast<long long>(n) * yn;
-                        else if (!p.counts || n < __ldg(p.counts + b)) {
-                            const int row = p.pages.row(b, slot);
-                            if (row < 0) serve::report(p.status, serve::ST_PAGE);
-                            else dst = y0 + static_cast<long long>(row) * p.Hkv * D;
-                        }
-                    } else {
-                        if (turns) pos = position_of(p, b, n);
-                        dst = y0 + b * yb + static_cast<long long>(n) * yn;
-                    }
-                    if (dst && !several) dst += static_cast<long long>(at.head) * step;
+            for (int u = 0; u < FWD_ROWS; ++u)
+                if (r + u < at.rows) raw[u].load(x + (r + u) * step_x, cols);
+#pragma unroll
+            for (int u = 0; u < FWD_ROWS; ++u) {
+                const bool here = r + u < at.rows;
+                if (ONE && turns) angles = load_angles(p, here ? position(r + u) : 0, lr, true);
+                float f[8];
+                if (here) raw[u].get(f);
+                else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) f[k] = 0.f;
                 }
-                angles = load_angles(p, pos, lr, turns);
-                if (several) after(b, n);
+                if (normed) {
+                    const float q = rsqrtf(row_sum<LANES>(dot8(f, f)) * (1.f / D) + eps);
+                    scale8(f, q);
+                    scale8(f, w);
+                }
+                if (turns) rotate(interleaved, f, angles, 1.f);
+                if (!here) continue;
+                __nv_bfloat16* to = ONE && to_cache ? cached(r + u) : to_cache && !y ? nullptr : y + (r + u) * step_y;
+                if (!to) continue;
+                Row8<__nv_bfloat16>::store(to, cols, f);
+                if (PAGED && ti == 0 && p.mass && lr == 0) p.mass[(to - y0) / D] = 0.f;
             }
-            float y[8];
-            if (u < at.rows) raw[u].get(y);
-            else {
+        }
+    }
+}
+
+template <typename XT, int D, bool PAGED>
+__global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 4 : 3) norm_rotate_kernel(const __grid_constant__ Params p) {
+    const int ti = find_tensor(p);
+    const Tensor& t = p.t[ti];
+    if (t.heads == 1) forward_rows<XT, D, PAGED, true>(p, t, ti);
+    else forward_rows<XT, D, PAGED, false>(p, t, ti);
+}
+
+// Adds the rows' share of dw to `dw`, a lane its eight columns.
+template <typename XT, int D, bool ONE>
+__device__ __forceinline__ void backward_rows(const Params& p, const Tensor& t, const Columns& cols, int lr, float (&dw)[8]) {
+    constexpr int LANES = D / 8, GROUPS = THREADS / LANES;
+    const bool turns = t.rotate && cols.turns, normed = t.w != nullptr, interleaved = p.interleaved != 0;
+    const float eps = p.eps;
+    const long long step_x = ONE ? t.xn : t.xh, step_g = ONE ? t.dyn : t.dyh, step_d = ONE ? t.dxn : t.dxh;
+    float w[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = 0.f;
+    for (int k = 0; k < 8; ++k) w[k] = 1.f;
+    if (normed) load_scale(t, cols, w);
+    const int items = t.items, stride = t.blocks * GROUPS, line = ONE ? LINE : min(LINE, t.heads);
+    // every lane of a warp makes the same number of turns: the shuffles want all of them
+    for (int base = (blockIdx.x - t.block0) * GROUPS; base < items; base += stride) {
+        const int item = base + threadIdx.x / LANES;
+        Place at{0, 0, 0, 0};
+        if (item < items) at = place_of<ONE>(p, t, item);
+        const XT* x = static_cast<const XT*>(t.x) + at.b * t.xb + static_cast<long long>(at.n) * t.xn + static_cast<long long>(at.head) * t.xh;
+        const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(t.dy) + at.b * t.dyb + static_cast<long long>(at.n) * t.dyn +
+                                  static_cast<long long>(at.head) * t.dyh;
+        XT* dx = static_cast<XT*>(t.dx) + at.b * t.dxb + static_cast<long long>(at.n) * t.dxn + static_cast<long long>(at.head) * t.dxh;
+        Row8<XT> next_x[BWD_ROWS];
+        Row8<__nv_bfloat16> next_g[BWD_ROWS];
+        auto fetch = [&](int r) {
+#pragma unroll
+            for (int u = 0; u < BWD_ROWS; ++u)
+                if (r + u < at.rows) {
+                    next_g[u].load(dy + (r + u) * step_g, cols);
+                    if (normed) next_x[u].load(x + (r + u) * step_x, cols);
+                }
+        };
+        fetch(0);
+        Angles angles;
+        if (!ONE) angles = load_angles(p, turns && at.rows > 0 ? position_of(p, at.b, at.n) : 0, lr, turns);
+#pragma unroll 1
+        for (int r = 0; r < line; r += BWD_ROWS) {
+            Row8<XT> now_x[BWD_ROWS];
+            Row8<__nv_bfloat16> now_g[BWD_ROWS];
+#pragma unroll
+            for (int u = 0; u < BWD_ROWS; ++u) { now_x[u] = next_x[u]; now_g[u] = next_g[u]; }
+            fetch(r + BWD_ROWS);
+#pragma unroll
+            for (int u = 0; u < BWD_ROWS; ++u) {
+                const bool here = r + u < at.rows;
+                if (ONE && turns) angles = load_angles(p, here ? position_of(p, at.b, at.n + r + u) : 0, lr, true);
+                float g[8], v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) g[k] = v[k] = 0.f;
+                if (here) {
+                    now_g[u].get(g);
+                    if (normed) now_x[u].get(v);
+                }
+                if (turns) rotate(interleaved, g, angles, -1.f);
+                if (normed) {
+                    float wg[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) wg[k] = g[k];
+                    scale8(wg, w);
+                    const float ss = row_sum<LANES>(dot8(v, v)), m = row_sum<LANES>(dot8(v, wg));
+                    const float q = rsqrtf(ss * (1.f / D) + eps);
+                    const uint64_t qq = sm100::pair_f32(q, q);
+                    const float f1 = -q * q * (m * q) * (1.f / D);
+                    const uint64_t ff = sm100::pair_f32(f1, f1);
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {
+                        const uint64_t vv = sm100::pair_f32(v[k], v[k + 1]);
+                        sm100::unpair_f32(sm100::fma_f32x2(sm100::pair_f32(g[k], g[k + 1]), sm100::mul_f32x2(vv, qq), sm100::pair_f32(dw[k], dw[k + 1])),
+                                          dw[k], dw[k + 1]);
+                        sm100::unpair_f32(sm100::fma_f32x2(vv, ff, sm100::mul_f32x2(qq, sm100::pair_f32(wg[k], wg[k + 1]))), g[k], g[k + 1]);
+                    }
+                }
+                if (here) Row8<XT>::store(dx + (r + u) * step_d, cols, g);
             }
-            if (normed) {
-                const float r = rsqrtf(row_sum<LANES>(dot8(y, y)) * (1.f / D) + eps);
-                scale8(y, r);
-                scale8(y, w);
-            }
-            if (turns) rotate(interleaved, y, angles, 1.f);
-            if (u < at.rows && dst) {
-                Row8<__nv_bfloat16>::store(dst, cols, y);
-                if (PAGED && ti == 0 && p.mass && lr == 0) p.mass[(dst - y0) / D] = 0.f;
-            }
-            if (!several && dst) dst += step;
         }
     }
 }
@@ -296,84 +361,13 @@ template <typename XT, int D>
 __global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 3 : 2) norm_rotate_backward_kernel(const __grid_constant__ Params p) {
     constexpr int LANES = D / 8, GROUPS = THREADS / LANES;
     __shared__ float sums[GROUPS][D];
-    const int ti = find_tensor(p);
-    const Tensor& t = p.t[ti];
+    const Tensor& t = p.t[find_tensor(p)];
     const int lr = threadIdx.x % LANES, group = threadIdx.x / LANES;
-    const int heads = t.heads, per_token = t.per_token, items = t.items;
-    const serve::Divide by_per_token = t.by_per_token;
-    const bool several = t.tokens_per > 1, normed = t.w != nullptr;
     const Columns cols = columns_of(p, lr);
-    const bool turns = t.rotate && cols.turns, interleaved = p.interleaved != 0;
-    const float eps = p.eps;
-    const XT* const x0 = static_cast<const XT*>(t.x);
-    const __nv_bfloat16* const dy0 = static_cast<const __nv_bfloat16*>(t.dy);
-    XT* const dx0 = static_cast<XT*>(t.dx);
-    float w[8], dw[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) { w[k] = 1.f; dw[k] = 0.f; }
-    if (normed) load_scale(t, cols, w);
-
-    struct Fetched { Row8<XT> x; Row8<__nv_bfloat16> g; int pos; XT* dx; };
-    auto fetch = [&](int item, Fetched (&f)[BWD_ROWS]) {
-        Place at{0, 0, 0, 0};
-        if (item < items) at = place_of<BWD_ROWS>(p, heads, per_token, by_per_token, several ? BWD_ROWS : 1, item);
-#pragma unroll
-        for (int u = 0; u < BWD_ROWS; ++u) {
-            f[u].dx = nullptr;
-            if (u < at.rows) {
-                const int h = several ? 0 : at.head + u;
-                f[u].g.load(dy0 + at.b * t.dyb + static_cast<long long>(at.n) * t.dyn + static_cast<long long>(h) * t.dyh, cols);
-                if (normed) f[u].x.load(x0 + at.b * t.xb + static_cast<long long>(at.n) * t.xn + static_cast<long long>(h) * t.xh, cols);
-                f[u].dx = dx0 + at.b * t.dxb + static_cast<long long>(at.n) * t.dxn + static_cast<long long>(h) * t.dxh;
-                if (u == 0 || several) f[u].pos = turns ? position_of(p, at.b, at.n) : 0;
-            }
-            if (several && ++at.n == p.N) { at.n = 0; ++at.b; }
-        }
-    };
-    // every lane of a warp makes the same number of turns: the shuffles want all of them
-    const int stride = t.blocks * GROUPS;
-    Fetched next[BWD_ROWS];
-    int base = (blockIdx.x - t.block0) * GROUPS;
-    fetch(base + group, next);
-    for (; base < items; base += stride) {
-        Fetched now[BWD_ROWS];
-#pragma unroll
-        for (int u = 0; u < BWD_ROWS; ++u) now[u] = next[u];
-        fetch(base + stride + group, next);
-        Angles angles;
-#pragma unroll
-        for (int u = 0; u < BWD_ROWS; ++u) {
-            float g[8], v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) g[k] = v[k] = 0.f;
-            if (now[u].dx) {
-                now[u].g.get(g);
-                if (normed) now[u].x.get(v);
-                if (u == 0 || several) angles = load_angles(p, now[u].pos, lr, turns);
-                if (turns) rotate(interleaved, g, angles, -1.f);
-            }
-            if (normed) {
-                float wg[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) wg[k] = g[k];
-                scale8(wg, w);
-                const float ss = row_sum<LANES>(dot8(v, v)), m = row_sum<LANES>(dot8(v, wg));
-                const float q = rsqrtf(ss * (1.f / D) + eps);
-                const uint64_t qq = sm100::pair_f32(q, q);
-                const float f1 = -q * q * (m * q) * (1.f / D);
-                const uint64_t ff = sm100::pair_f32(f1, f1);
-#pragma unroll
-                for (int k = 0; k < 8; k += 2) {
-                    const uint64_t vv = sm100::pair_f32(v[k], v[k + 1]);
-                    sm100::unpair_f32(sm100::fma_f32x2(sm100::pair_f32(g[k], g[k + 1]), sm100::mul_f32x2(vv, qq), sm100::pair_f32(dw[k], dw[k + 1])),
-                                      dw[k], dw[k + 1]);
-                    sm100::unpair_f32(sm100::fma_f32x2(vv, ff, sm100::mul_f32x2(qq, sm100::pair_f32(wg[k], wg[k + 1]))), g[k], g[k + 1]);
-                }
-            }
-            if (now[u].dx) Row8<XT>::store(now[u].dx, cols, g);
-        }
-    }
-    if (!normed) return;
+    float dw[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (t.heads == 1) backward_rows<XT, D, true>(p, t, cols, lr, dw);
+    else backward_rows<XT, D, false>(p, t, cols, lr, dw);
+    if (!t.w) return;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         sums[group][cols.a + k] = dw[k];
@@ -418,7 +412,7 @@ bool aligned(const void* ptr, const int64_t* strides, int type) {
 // Checks and fills what forward, backward and append have in common.  Blocks of a tensor: one group per item, but no
 // more than its share of `budget` blocks in proportion to its rows.
 int fill(Params& p, const char* who, const att3_head_rows* t, int n, int x_type, const float* table, int table_rows,
-         int rot, int interleaved, int B, int N, int D, float eps, int rows_per_item, int budget) {
+         int rot, int interleaved, int B, int N, int D, float eps, int budget) {
     if (!t || n < 1 || n > MAX_TENSORS) return att3::set_error(ATT3_ERR_INVALID, "%s: 1 to %d tensors, got %d", who, MAX_TENSORS, n);
     if (D != 16 && D != 32 && D != 64 && D != 128)
         return att3::set_error(ATT3_ERR_INVALID, "%s: head dim must be 16, 32, 64 or 128, got %d", who, D);
@@ -437,7 +431,6 @@ int fill(Params& p, const char* who, const att3_head_rows* t, int n, int x_type,
     p.B = B;
     p.N = N;
     p.by_N = serve::make_divide(std::max(1, N));
-    p.tokens = static_cast<int>(std::min<long long>(static_cast<long long>(B) * N, 0x7FFFFFFFll));
     p.eps = eps;
     const long long groups = THREADS / (D / 8);
     long long rows = 0, blocks = 0;
@@ -458,13 +451,11 @@ int fill(Params& p, const char* who, const att3_head_rows* t, int n, int x_type,
         if (o.w && (o.w_type < 0 || o.w_type > 2)) return att3::set_error(ATT3_ERR_INVALID, "%s: unknown element type of scale %d", who, k);
         if (o.w && reinterpret_cast<uintptr_t>(o.w) % 16 != 0) return att3::set_error(ATT3_ERR_INVALID, "%s: scale %d must be 16-byte aligned", who, k);
         o.heads = static_cast<int>(t[k].heads);
-        // one head: several tokens an item; more heads: several heads of one token
-        o.tokens_per = o.heads == 1 ? rows_per_item : 1;
-        o.per_token = o.tokens_per > 1 ? 1 : (o.heads + rows_per_item - 1) / rows_per_item;
-        o.by_per_token = serve::make_divide(o.per_token);
-        const long long tokens = static_cast<long long>(B) * N;
-        const long long items = o.tokens_per > 1 ? (tokens + o.tokens_per - 1) / o.tokens_per : tokens * o.per_token;
-        if (tokens * std::max(4, o.heads) > 0x3FFFFFFFll) return att3::set_error(ATT3_ERR_INVALID, "%s: more than 2^30 rows in a tensor", who);
+        // one head: lines of positions; more heads: lines of a token's heads
+        o.lines = static_cast<int>((static_cast<long long>(o.heads == 1 ? N : o.heads) + LINE - 1) / LINE);
+        o.by_lines = serve::make_divide(std::max(1, o.lines));
+        const long long outer = o.heads == 1 ? B : static_cast<long long>(B) * N, items = outer * o.lines;
+        if (static_cast<long long>(B) * N * o.heads > 0x3FFFFFFFll) return att3::set_error(ATT3_ERR_INVALID, "%s: more than 2^30 rows in a tensor", who);
         o.items = static_cast<int>(items);
         long long nb = (items + groups - 1) / groups;
         nb = std::min(nb, std::max<long long>(1, budget * static_cast<long long>(o.heads) / rows));
@@ -530,7 +521,7 @@ extern "C" int att3_norm_rotate_forward(const att3_head_rows* tensors, int n, in
                                         int64_t pos_n, int B, int N, int D, float eps, void* stream) {
     const char* who = "att3_norm_rotate_forward";
     Params p = {};
-    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, N, D, eps, FWD_ROWS, att3::sm_count() * FWD_BLOCKS_PER_SM)) return rc;
+    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, N, D, eps, att3::sm_count() * FWD_BLOCKS_PER_SM)) return rc;
     if (positions && pos_bytes != 4 && pos_bytes != 8) return att3::set_error(ATT3_ERR_INVALID, "%s: positions are 4 or 8 bytes wide", who);
     if (B == 0 || N == 0) return ATT3_OK;
     for (int k = 0; k < n; ++k) {
@@ -557,7 +548,7 @@ extern "C" int att3_norm_rotate_backward(const att3_head_rows* tensors, int n, i
     const char* who = "att3_norm_rotate_backward";
     Params p = {};
     const int budget = att3::sm_count() * BWD_BLOCKS_PER_SM;
-    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, N, D, eps, BWD_ROWS, budget)) return rc;
+    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, N, D, eps, budget)) return rc;
     if (positions && pos_bytes != 4 && pos_bytes != 8) return att3::set_error(ATT3_ERR_INVALID, "%s: positions are 4 or 8 bytes wide", who);
     const bool rows = B > 0 && N > 0;
     bool scaled = false;
@@ -606,7 +597,7 @@ extern "C" int att3_gather_cache_append(const att3_head_rows* tensors, int n, in
     const char* who = "att3_gather_cache_append";
     Params p = {};
     if (n != 4 && n != 5) return att3::set_error(ATT3_ERR_INVALID, "%s: R, S, Vr, Vs and optionally Q, got %d tensors", who, n);
-    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, T, D, eps, FWD_ROWS, att3::sm_count() * FWD_BLOCKS_PER_SM)) return rc;
+    if (int rc = fill(p, who, tensors, n, x_type, table, table_rows, rot, interleaved, B, T, D, eps, att3::sm_count() * FWD_BLOCKS_PER_SM)) return rc;
     if (B == 0 || T == 0) return ATT3_OK;
     if (int rc = att3::check_gather_pages(pages, who)) return rc;
     if (!lengths) return att3::set_error(ATT3_ERR_INVALID, "%s: null lengths", who);
