@@ -9,7 +9,7 @@ namespace {
 struct Layout {
     size_t part, rows, row_ref, cols, col_ref, lse, unit_base, tile_base, bytes;
     long long units;
-    int ctas;
+    int ctas, wide;
 };
 
 // The workspace for the longest sequences that the arguments admit.
@@ -21,7 +21,10 @@ Layout layout(int B, int Hq, int Hkv, int D, int window, int sinks, long long ma
     auto block = [&](long long heads) { return (heads * groups + 7) / 8; };          // tiles of a block of heads
     const long long per_key_head = mass ? G * block(1) : G / 8 * groups + (G & 4 ? block(4) : 0) + (G & 2 ? block(2) : 0) + (G & 1 ? block(1) : 0);
     const long long tiles = static_cast<long long>(B) * Hkv * per_key_head;
-    o.units = tiles * ((seen + 127) / 128);
+    // One step of up to 192 keys a tile in place of two, where the longest needs no more (128 sequences of 8 heads at
+    // window 128 with 4 sinks: 42 us in place of 57).  The masses' column sums are laid out for steps of 128.
+    o.wide = !mass && seen > serve::DEC_KEYS && seen <= serve::DEC_WIDE;
+    o.units = tiles * (o.wide ? 1 : (seen + 127) / 128);
     o.ctas = static_cast<int>(std::max<long long>(1, std::min<long long>(att3::sm_count(), o.units)));
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
@@ -49,14 +52,14 @@ int check(const char* who, int B, int Hq, int Hkv, int D, int window, int sinks)
     return ATT3_OK;
 }
 
-template <int D, bool MASS>
+template <int D, bool MASS, bool WIDE>
 int launch(const serve::DecodeParams& p, const Layout& lay, long long max_seen, cudaStream_t st, const char* who) {
     constexpr int smem = serve::DecSmem<D>::BYTES;
-    cudaError_t e = cudaFuncSetAttribute(serve::decode_kernel<D, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(serve::decode_kernel<D, MASS, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return att3::set_cuda_error(e, who);
     att3::count_launch(4, MASS ? 3 : 2);
     const att3::TimedLaunch timed(att3::K_SERVE, st);
-    serve::decode_kernel<D, MASS><<<lay.ctas, serve::DEC_THREADS, smem, st>>>(p);
+    serve::decode_kernel<D, MASS, WIDE><<<lay.ctas, serve::DEC_THREADS, smem, st>>>(p);
     // the joining kernels may be set up while the one before them runs out; they wait for its end themselves
     cudaLaunchAttribute early = {};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -124,6 +127,7 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     p.lengths = lengths;
     p.pages = serve::make_pages(pages->table, pages->table_stride, pages->per_sequence, pages->pages, pages->page_size);
     p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.window = window; p.sinks = sinks;
+    p.wide = lay.wide;
     p.c2 = sgring::LOG2E / std::sqrt(static_cast<float>(D));
     char* ws = static_cast<char*>(workspace);
     p.part = reinterpret_cast<float*>(ws + lay.part);
@@ -137,6 +141,9 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     if (!(p.status = att3::serve_status_ptr())) return att3::set_error(ATT3_ERR_CUDA, "%s: status word not resolvable", who);
     const long long seen = window > 0 ? std::min<long long>(most, static_cast<long long>(window) + sinks) : most;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (D == 128) return mass ? launch<128, true>(p, lay, seen, st, who) : launch<128, false>(p, lay, seen, st, who);
-    return mass ? launch<64, true>(p, lay, seen, st, who) : launch<64, false>(p, lay, seen, st, who);
+    if (D == 128)
+        return mass ? launch<128, true, false>(p, lay, seen, st, who)
+                    : lay.wide ? launch<128, false, true>(p, lay, seen, st, who) : launch<128, false, false>(p, lay, seen, st, who);
+    return mass ? launch<64, true, false>(p, lay, seen, st, who)
+                : lay.wide ? launch<64, false, true>(p, lay, seen, st, who) : launch<64, false, false>(p, lay, seen, st, who);
 }

@@ -35,6 +35,11 @@
 // takes 4200 cycles as row gathers from one warp (62 an instruction), 1700 from three, 930 as boxes of 16 rows and 720
 // as boxes of 64; 16-byte asynchronous copies from three warps took 3000.  While one half exponentiates, the other
 // half's products run.
+//
+// Tensor memory: per half 128 columns of scores, over which P is written, then 128 of U.  Where no sequence shows more
+// than 192 slots (a window of 128 with a few sinks), a tile's keys are one step: its scores run on into the columns of U,
+// which nothing is in before the step's second product, and a stage of the ring holds 192 rows.  Without that, 132 visible
+// slots take two steps, the second for four columns.
 #pragma once
 
 #include "att3_abi_internal.h"
@@ -50,6 +55,7 @@ constexpr int DEC_THREADS = 384;
 constexpr int DEC_STRIP = 32;              // rows of a strip
 constexpr int DEC_TILE_STRIPS = 8;
 constexpr int DEC_KEYS = 128;              // keys of a unit of work
+constexpr int DEC_WIDE = 192;              // of the only unit of a tile, where no sequence shows more (DecodeParams::wide)
 constexpr int DEC_COPY_WARPS = 3;
 
 struct DecodeParams {
@@ -75,6 +81,7 @@ struct DecodeParams {
     // pools as [pages * page_size, Hkv * D], 64 columns of one row, or of `box` rows of a page (0: not used)
     CUtensorMap tmS, tmVs, tmS_box, tmVs_box;
     int box;
+    int wide;                              // 1: no sequence shows more than 192 slots, and a tile has one step of up to 192 keys
 };
 
 // Tiles of a block of `heads` (1, 2, 4 or 8) heads with `groups` strips each.
@@ -97,7 +104,7 @@ __device__ __forceinline__ Shape shape_of(const DecodeParams& p, int b, bool tel
     if (MASS) s.tiles = p.G * block_tiles(1, s.groups);
     else s.tiles = p.G / 8 * s.groups + (p.G & 4 ? block_tiles(4, s.groups) : 0) + (p.G & 2 ? block_tiles(2, s.groups) : 0) +
                    (p.G & 1 ? block_tiles(1, s.groups) : 0);
-    s.steps = (s.seen + DEC_KEYS - 1) / DEC_KEYS;
+    s.steps = p.wide ? min(s.seen, 1) : (s.seen + DEC_KEYS - 1) / DEC_KEYS;
     return s;
 }
 
@@ -159,11 +166,16 @@ __device__ __forceinline__ int slot_of(const DecodeParams& p, const Shape& s, in
     return p.window > 0 && e >= p.sinks ? e + s.skip : e;
 }
 
-// The stretch of CTA c: [total * c / n, total * (c + 1) / n).  The last CTA whose stretch begins at or before `unit`:
-__device__ __forceinline__ int cta_of(int unit, int total, int n) {
-    return static_cast<int>(((static_cast<long long>(unit) + 1) * n - 1) / total);
+// The stretch of CTA c of n begins at unit stretch(total, c, n): the first total % n of them have one unit more.
+__device__ __forceinline__ int stretch(int total, int c, int n) {
+    const int per = total / n;
+    return c * per + min(c, total - per * n);
 }
-__device__ __forceinline__ int stretch(int total, int c, int n) { return static_cast<int>(static_cast<long long>(total) * c / n); }
+// The CTA whose stretch holds `unit`.
+__device__ __forceinline__ int cta_of(int unit, int total, int n) {
+    const int per = total / n, more = total - per * n, head = more * (per + 1);
+    return unit < head ? unit / (per + 1) : more + (unit - head) / per;
+}
 
 // A CTA's way along its stretch, one tile's key range at a time; every role walks it by itself.
 template <bool MASS>
@@ -171,6 +183,12 @@ struct Walk {
     Shape s;
     int b, head, tile, k0, k1;             // sequence, key head, tile, key steps [k0, k1)
     int left, unit, slot;                  // units still to do, of the first step, row sums' slot
+    Block block;                           // of the tile, and the tile behind it
+    int block_end;
+    __device__ __forceinline__ void enter(const DecodeParams& p) {
+        block = block_of_tile<MASS>(p, s, tile);
+        block_end = block.tile0 + block_tiles(1 << block.log_heads, s.groups);
+    }
     __device__ __forceinline__ void start(const DecodeParams& p, int b0, int off, int count, int tile_base, int unit0) {
         b = b0;
         s = shape_of<MASS>(p, b);
@@ -183,6 +201,7 @@ struct Walk {
         unit = unit0;
         slot = tile_base + head * s.tiles + tile + blockIdx.x;
         k1 = min(s.steps, k0 + left);
+        enter(p);
     }
     // false when the stretch is done
     __device__ __forceinline__ bool next(const DecodeParams& p) {
@@ -191,23 +210,28 @@ struct Walk {
         if (left <= 0) return false;
         k0 = 0;
         ++slot;
-        if (++tile == s.tiles) {
-            tile = 0;
-            if (++head == p.Hkv) {
-                head = 0;
-                do { ++b; if (b >= p.B) return false; s = shape_of<MASS>(p, b); } while (s.seen == 0);
+        if (++tile == block_end) {
+            if (tile == s.tiles) {
+                tile = 0;
+                if (++head == p.Hkv) {
+                    head = 0;
+                    do { ++b; if (b >= p.B) return false; s = shape_of<MASS>(p, b); } while (s.seen == 0);
+                }
             }
+            enter(p);
         }
         k1 = min(s.steps, left);
         return true;
     }
     // whether a half of the tile holds any key
-    __device__ __forceinline__ bool live(const DecodeParams& p, int half) const {
-        const Block k = block_of_tile<MASS>(p, s, tile);
-        return (((tile - k.tile0) * DEC_TILE_STRIPS + half * 4) >> k.log_heads) < s.groups;
+    __device__ __forceinline__ bool live(int half) const {
+        return (((tile - block.tile0) * DEC_TILE_STRIPS + half * 4) >> block.log_heads) < s.groups;
     }
     // columns of key step k in chunks of 32 (the last step's tiles and products are cut to them)
-    __device__ __forceinline__ int chunks(int k) const { return min(4, (s.seen - k * DEC_KEYS + 31) / 32); }
+    template <bool WIDE>
+    __device__ __forceinline__ int chunks(int k) const {
+        return min((WIDE ? DEC_WIDE : DEC_KEYS) / 32, (s.seen - k * DEC_KEYS + 31) / 32);
+    }
 };
 
 template <int D>
@@ -274,7 +298,7 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-template <int D, bool MASS>
+template <int D, bool MASS, bool WIDE>
 __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_constant__ DecodeParams p) {
     using L = DecSmem<D>;
     constexpr int REC = D + 4, COLS = D / 32;
@@ -368,7 +392,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         sgring::reg_inc<208>();
         const int half = warp >> 2, wq = warp & 3;
         const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
-        const uint32_t tS = tmem + lanes + half * 128, tO = tmem + lanes + 256 + half * 128;
+        const uint32_t tS = tmem + lanes + half * 256, tO = tS + 128;
         uint8_t* tile_hi = smem + L::OFF_A + half * 2 * L::TILE;
         constexpr int CH = D / 8, RPP = 32 / CH, PASSES = DEC_STRIP / RPP;      // chunks a row, rows a pass
         const int chunk = lane % CH, sub = lane / CH;
@@ -383,7 +407,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         // own row of it in the pools (a row on no valid page reads row 0 and is reported).
         int g = 0, valid = 0, row = 0;
         auto look = [&](const Walk<MASS>& at) {
-            const Block k = block_of_tile<MASS>(p, at.s, at.tile);
+            const Block& k = at.block;
             const int strip = (at.tile - k.tile0) * DEC_TILE_STRIPS + warp, j0 = (strip >> k.log_heads) * DEC_STRIP;
             g = k.g0 + (strip & ((1 << k.log_heads) - 1));
             valid = max(0, min(DEC_STRIP, at.s.seen - j0));
@@ -430,7 +454,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             else copy_commit();
             q = *reinterpret_cast<const uint4*>(p.Q + (static_cast<size_t>(at.b) * p.Hq + at.head * p.G + g) * D + chunk * 8);
         };
-        while (go && !w.live(p, half)) go = w.next(p);
+        while (go && !w.live(half)) go = w.next(p);
         if (go) prepare(w);
 #pragma unroll 1
         while (go && ok) {
@@ -493,7 +517,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     }
                 };
                 const uint64_t scale = pair_f32(p.c2, p.c2);
-                const int cols = w.s.seen - k * DEC_KEYS, chunks = w.chunks(k);          // visible columns of this step
+                const int cols = w.s.seen - k * DEC_KEYS, chunks = w.template chunks<WIDE>(k);          // visible columns of this step
                 // Exponentials of 32 scores relative to the reference: their sum, their BF16 pairs to tensor memory (P of
                 // chunk c covers score columns 16 c .. 16 c + 15, which are read by then), with masses the column sums.
                 // Rows behind the last key contribute nothing: their exponent is -inf throughout.
@@ -524,28 +548,8 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 // scores read twice from tensor memory: with all 128 of them in registers and everything unrolled the code
                 // spills and outgrows the instruction cache, which holds all roles' code; with 32 at a time throughout, a
                 // step takes 2950 cycles.
-                if (valid > 0 && cols >= DEC_KEYS) {
-                    float mx = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < 4; c += 2) {
-                        uint32_t x[2][32];
-                        tmem_ld32(tS + c * 32, x[0]);
-                        tmem_ld32(tS + c * 32 + 32, x[1]);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(x[0][i]), __uint_as_float(x[1][i])));
-                    }
-                    renew(mx);
-#pragma unroll 1
-                    for (int c = 0; c < 4; c += 2) {
-                        uint32_t x[2][32];
-                        tmem_ld32(tS + c * 32, x[0]);
-                        tmem_ld32(tS + c * 32 + 32, x[1]);
-                        tmem_wait_ld();
-                        exponentials(x[0], c);
-                        exponentials(x[1], c + 1);
-                    }
-                } else if (valid > 0) {
+                // The 2 `pairs` first chunks have no hidden column.
+                auto passes = [&](int pairs, int all) {
                     auto load = [&](int c, uint32_t (&x)[32]) {
                         tmem_ld32(tS + c * 32, x);
                         tmem_wait_ld();
@@ -556,7 +560,16 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     };
                     float mx = -INFINITY;
 #pragma unroll 1
-                    for (int c = 0; c < chunks; ++c) {
+                    for (int c = 0; c < 2 * pairs; c += 2) {
+                        uint32_t x[2][32];
+                        tmem_ld32(tS + c * 32, x[0]);
+                        tmem_ld32(tS + c * 32 + 32, x[1]);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(x[0][i]), __uint_as_float(x[1][i])));
+                    }
+#pragma unroll 1
+                    for (int c = 2 * pairs; c < all; ++c) {
                         uint32_t x[32];
                         load(c, x);
 #pragma unroll
@@ -564,11 +577,25 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     }
                     renew(mx);
 #pragma unroll 1
-                    for (int c = 0; c < chunks; ++c) {
+                    for (int c = 0; c < 2 * pairs; c += 2) {
+                        uint32_t x[2][32];
+                        tmem_ld32(tS + c * 32, x[0]);
+                        tmem_ld32(tS + c * 32 + 32, x[1]);
+                        tmem_wait_ld();
+                        exponentials(x[0], c);
+                        exponentials(x[1], c + 1);
+                    }
+#pragma unroll 1
+                    for (int c = 2 * pairs; c < all; ++c) {
                         uint32_t x[32];
                         load(c, x);
                         exponentials(x, c);
                     }
+                };
+                if (valid > 0) {
+                    if (WIDE) passes((cols >= chunks * 32 ? chunks : chunks - 1) >> 1, chunks);
+                    else if (cols >= DEC_KEYS) passes(2, 4);
+                    else passes(0, chunks);
                 }
                 if (valid > 0) {
                     tmem_wait_st();
@@ -620,7 +647,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             // fetched while the products finish.
             const int head = w.b * p.Hq + w.head * p.G + g, valid_now = valid;
             const int rec = w.slot * DEC_TILE_STRIPS + warp;
-            do go = w.next(p); while (go && !w.live(p, half));
+            do go = w.next(p); while (go && !w.live(half));
             if (go) prepare(w);
             else copy_commit();                            // an empty group: Vr is the last but one either way
             copy_wait<1>();
@@ -705,6 +732,9 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         flush();
     } else {
         sgring::reg_dec<88>();
+        // the ring's stages: rows of a tile of S or Vs, 64 columns after the other
+        constexpr int block_bytes = (WIDE ? DEC_WIDE : DEC_KEYS) * 128, stage_bytes = block_bytes * (D / 64);
+        constexpr int stages = L::STAGES * L::TILE / stage_bytes;
         if (warp == 8 && busy) {
             // ================================================================== products
             const uint32_t issuer = elect_one();
@@ -713,40 +743,41 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             int fill = 0;                                  // stages consumed
             bool go = true, ok = true;
             auto stage_desc = [&](int f, bool mn) {
-                return make_smem_desc(smem_u32(smem + L::OFF_KV + (f % L::STAGES) * L::TILE), mn ? 128 * 128 : 16, 1024, SWIZZLE_128B);
+                return make_smem_desc(smem_u32(smem + L::OFF_KV + (f % stages) * stage_bytes), mn ? block_bytes : 16, 1024, SWIZZLE_128B);
             };
-            auto stage_wait = [&](int f) { return pipe_wait(&bars[DB_KV_FULL0 + f % L::STAGES], (f / L::STAGES) & 1, fail, 4); };
+            auto stage_wait = [&](int f) { return pipe_wait(&bars[DB_KV_FULL0 + f % stages], (f / stages) & 1, fail, 4); };
             auto scores = [&](int t, int f, int chunks) {
                 const uint32_t idesc_x = make_idesc_bf16(128, chunks * 32, 0, 0);
                 const uint64_t b = stage_desc(f, false);
-                const uint32_t tX = tmem + t * 128;
+                const uint32_t tX = tmem + t * 256;
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
                     const uint64_t a = make_smem_desc(smem_u32(smem + L::OFF_A + (2 * t + part) * L::TILE), 16, 1024, SWIZZLE_128B);
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = ((kk >> 2) * 128 * 128 + (kk & 3) * 32) / 16;
-                        umma_ss_pred(tX, a + off, b + off, idesc_x, part > 0 || kk > 0, issuer);
+                        const uint32_t off = (kk & 3) * 32 / 16;
+                        umma_ss_pred(tX, a + off + (kk >> 2) * (128 * 128 / 16), b + off + (kk >> 2) * (block_bytes / 16), idesc_x, part > 0 || kk > 0,
+                                     issuer);
                     }
                 }
                 umma_commit_pred(&bars[DB_S_FULL0 + t], issuer);
             };
 #pragma unroll 1
             while (go && ok) {
-                const bool two = w.live(p, 1);
+                const bool two = w.live(1);
                 ok = stage_wait(fill);
                 for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
                     ok = pipe_wait(&bars[DB_A_FULL0 + t], seg[t] & 1, fail, 5);
                     if (!ok) break;
                     tc_fence_after();
-                    scores(t, fill, w.chunks(w.k0));
+                    scores(t, fill, w.template chunks<WIDE>(w.k0));
                 }
                 if (!ok) break;
-                umma_commit_pred(&bars[DB_KV_EMPTY0 + fill % L::STAGES], issuer);
+                umma_commit_pred(&bars[DB_KV_EMPTY0 + fill % stages], issuer);
 #pragma unroll 1
                 for (int k = w.k0; k < w.k1 && ok; ++k) {
                     const bool more = k + 1 < w.k1;
-                    const int chunks = w.chunks(k);
+                    const int chunks = w.template chunks<WIDE>(k);
                     ok = stage_wait(fill + 1);
                     for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
                         ok = pipe_wait(&bars[DB_P_FULL0 + t], n[t] & 1, fail, 6);
@@ -755,7 +786,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                         tc_fence_after();
                         const uint64_t b = stage_desc(fill + 1, true);
                         auto product = [&](int kk) {
-                            umma_ts_pred(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, b + kk * (2048 / 16), idesc_u, k > w.k0 || kk > 0, issuer);
+                            umma_ts_pred(tmem + t * 256 + 128, tmem + t * 256 + kk * 8, b + kk * (2048 / 16), idesc_u, k > w.k0 || kk > 0, issuer);
                         };
                         if (chunks == 4) {
 #pragma unroll
@@ -768,12 +799,12 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                         else {
                             if (t == 0) ok = stage_wait(fill + 2);
                             if (!ok) break;
-                            scores(t, fill + 2, w.chunks(k + 1));
+                            scores(t, fill + 2, w.template chunks<WIDE>(k + 1));
                         }
                     }
                     if (!ok) break;
-                    umma_commit_pred(&bars[DB_KV_EMPTY0 + (fill + 1) % L::STAGES], issuer);
-                    if (more) umma_commit_pred(&bars[DB_KV_EMPTY0 + (fill + 2) % L::STAGES], issuer);
+                    umma_commit_pred(&bars[DB_KV_EMPTY0 + (fill + 1) % stages], issuer);
+                    if (more) umma_commit_pred(&bars[DB_KV_EMPTY0 + (fill + 2) % stages], issuer);
                     fill += 2;
                 }
                 ++seg[0];
@@ -792,9 +823,9 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             while (go && ok) {
 #pragma unroll 1
                 for (int k = w.k0; k < w.k1 && ok; ++k) {
-                    const bool boxes = p.box > 0 && (k + 1) * DEC_KEYS <= w.s.seen;
+                    const bool boxes = !WIDE && p.box > 0 && (k + 1) * DEC_KEYS <= w.s.seen;
                     const int rows = boxes ? p.box : 4;
-                    const int wanted = w.chunks(k) * 32;
+                    const int wanted = w.template chunks<WIDE>(k) * 32;
                     const bool any = mine * rows < wanted;
                     int row[4] = {0, 0, 0, 0};
                     if (any) {
@@ -809,20 +840,20 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     }
 #pragma unroll 1
                     for (int kind = 0; kind < 2; ++kind, ++fill) {
-                        const int st = fill % L::STAGES;
+                        const int st = fill % stages;
                         uint64_t* full = &bars[DB_KV_FULL0 + st];
-                        if (fill >= L::STAGES) ok = pipe_wait(&bars[DB_KV_EMPTY0 + st], (fill / L::STAGES - 1) & 1, fail, 8);
+                        if (fill >= stages) ok = pipe_wait(&bars[DB_KV_EMPTY0 + st], (fill / stages - 1) & 1, fail, 8);
                         if (!ok) break;
                         // one arrival, of the thread that names the bytes; other warps' bytes may come before it
                         if (warp == 9 && lane == 0) mbar_arrive_expect_tx(full, wanted * D * 2);
                         __syncwarp();
                         if (any) {
-                            uint8_t* dst = smem + L::OFF_KV + st * L::TILE + mine * rows * 128;
+                            uint8_t* dst = smem + L::OFF_KV + st * stage_bytes + mine * rows * 128;
 #pragma unroll
                             for (int h = 0; h < D / 64; ++h) {
                                 const int x = w.head * D + h * 64;
-                                if (boxes) tma_load_2d(dst + h * DEC_KEYS * 128, kind ? &p.tmVs_box : &p.tmS_box, x, row[0], full);
-                                else tma_gather4(dst + h * DEC_KEYS * 128, kind ? &p.tmVs : &p.tmS, x, row, full);
+                                if (boxes) tma_load_2d(dst + h * block_bytes, kind ? &p.tmVs_box : &p.tmS_box, x, row[0], full);
+                                else tma_gather4(dst + h * block_bytes, kind ? &p.tmVs : &p.tmS, x, row, full);
                             }
                         }
                         __syncwarp();
@@ -831,8 +862,8 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 go = go && w.next(p);
             }
             // every copy that was asked for has landed before the CTA ends
-            for (int f = max(0, fill - L::STAGES); f < fill; ++f)
-                pipe_wait(&bars[DB_KV_FULL0 + f % L::STAGES], (f / L::STAGES) & 1, fail, 9);
+            for (int f = max(0, fill - stages); f < fill; ++f)
+                pipe_wait(&bars[DB_KV_FULL0 + f % stages], (f / stages) & 1, fail, 9);
         }
     }
     tc_fence_before();

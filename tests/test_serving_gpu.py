@@ -242,6 +242,11 @@ DECODE_CASES = [
     ([77, 900, 16], 8, 8, 64, 16, 1, 3),
     ([600, 256], 4, 1, 128, 256, 300, 37),
     ([50] * 40, 8, 4, 128, 16, 33, 1),
+    # at most 192 visible slots: one step of keys a tile
+    ([192, 191, 129, 160, 161, 5, 0], 8, 2, 128, 32, 0, 0),
+    ([1000, 193, 192, 150, 40], 3, 1, 128, 16, 150, 42),
+    ([500, 133, 700], 8, 8, 64, 16, 128, 5),
+    ([140] * 30, 16, 1, 64, 64, 130, 2),
 ]
 
 
