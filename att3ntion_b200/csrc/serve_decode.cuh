@@ -940,10 +940,9 @@ __global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant_
     const int b = blockIdx.y / p.Hkv, kv = blockIdx.y % p.Hkv;
     const Shape s = shape_of<true>(p, b);
     const int e = blockIdx.x * 128 + threadIdx.x;
-    if (e >= s.seen) return;
-    const int row = p.pages.row(b, slot_of(p, s, e));
+    const int row = e < s.seen ? p.pages.row(b, slot_of(p, s, e)) : -1;
+    wait_for_previous_kernel();            // every block does, so that this kernel never ends before that one
     if (row < 0) return;
-    wait_for_previous_kernel();
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const int tiles0 = p.tile_base[b] + kv * s.tiles;
     const int step = e / DEC_KEYS, col = e % DEC_KEYS, per_head = block_tiles(1, s.groups);

@@ -211,21 +211,21 @@ __device__ __forceinline__ void forward_rows(const Params& p, const Tensor& t, i
         const XT* x = static_cast<const XT*>(t.x) + at.b * t.xb + static_cast<long long>(at.n) * t.xn + static_cast<long long>(at.head) * t.xh;
         // where the rows go, and the position of the first
         __nv_bfloat16* y = y0 + at.b * t.yb + static_cast<long long>(at.n) * t.yn + static_cast<long long>(at.head) * t.yh;
-        int slot = 0;                                      // of the first row in the cache
+        int slot = 0, told = LINE;                         // the first row's slot in the cache; positions that a count covers
         long long first = 0;
         if (PAGED && at.rows > 0) {
             slot = __ldg(p.lengths + at.b) + at.n;
             first = p.positions ? static_cast<long long>(static_cast<const int*>(p.positions)[at.b]) + at.n : slot;
-            if (to_cache && p.counts) {                    // what is not stored is not read either
-                const int left = __ldg(p.counts + at.b) - at.n;
-                at.rows = ONE ? max(0, min(at.rows, left)) : left > 0 ? at.rows : 0;
+            if (p.counts) {
+                told = __ldg(p.counts + at.b) - at.n;
+                if (to_cache) at.rows = ONE ? max(0, min(at.rows, told)) : told > 0 ? at.rows : 0;       // what is not stored is not read
             }
         }
         auto position = [&](int u) {                       // of row u
             if (!PAGED) return position_of(p, at.b, at.n + (ONE ? u : 0));
             const long long q = first + (ONE ? u : 0);
             if (q >= 0 && q < p.table_rows) return static_cast<int>(q);
-            serve::report(p.status, serve::ST_POSITION);
+            if ((ONE ? u : 0) < told) serve::report(p.status, serve::ST_POSITION);          // a query behind the count may lie anywhere
             return 0;
         };
         auto cached = [&](int u) -> __nv_bfloat16* {       // the cache's row of token u, head `at.head`; none where it has no page

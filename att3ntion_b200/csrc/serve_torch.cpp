@@ -230,6 +230,21 @@ struct NormRotate : torch::autograd::Function<NormRotate> {
     }
 };
 
+// During a capture autograd runs a leaf's accumulation on the stream that the leaf's accumulator was made on.  One that an
+// eager graph still keeps alive is of a stream outside the capture, and the backward pass would then end the capture, and
+// with it the process; so the forward pass refuses.
+void check_capture(const Tensors& leaves) {
+    if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+    for (const Tensor& t : leaves) {
+        if (!t.requires_grad() || !t.is_leaf()) continue;
+        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+        if (!accumulator) continue;
+        const auto stream = accumulator->stream();
+        if (stream && *stream != at::cuda::getCurrentCUDAStream(t.device().index()).unwrap())
+            throw std::runtime_error("norm_rotate: an autograd graph of these leaves made outside the capture is still alive; release it first");
+    }
+}
+
 py::object norm_rotate(const Tensors& xs, const std::vector<MaybeTensor>& weights, const MaybeTensor& table, const MaybeTensor& positions,
                        double eps, bool interleaved, bool heads_first) {
     if (xs.empty() || xs.size() > 5 || weights.size() != xs.size() || !are_heads(xs) || !(eps >= 0)) return py::none();
@@ -251,10 +266,11 @@ py::object norm_rotate(const Tensors& xs, const std::vector<MaybeTensor>& weight
         ws.push_back(weights[k] ? *weights[k] : Tensor());
     }
     Tensors ys;
-    if (graph && at::GradMode::is_enabled())
+    if (graph && at::GradMode::is_enabled()) {
+        check_capture(tensors);
         ys = NormRotate::apply(at::TensorList(tensors), static_cast<int64_t>(xs.size()), scaled, table, positions, eps, interleaved,
                                heads_first);
-    else
+    } else
         ys = run_forward(xs, ws, Call{table, positions, eps, interleaved, heads_first});
     py::tuple out(ys.size());
     for (size_t k = 0; k < ys.size(); ++k) out[k] = py::cast(ys[k]);

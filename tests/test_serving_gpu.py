@@ -468,6 +468,111 @@ def test_captured_step_follows_the_lengths():
     ck.device_status()
 
 
+def test_tables_that_are_part_of_a_larger_one():
+    """Page tables and lengths as slices of a server's own."""
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append, gather_cache_evict, single_gather_decode
+    c = Made(13, [100, 37, 64], 1, 64, 16, room=8)
+    pools, table, n = c.gpu()
+    wide = torch.full((5, table.shape[1] + 9), -7, dtype=torch.int32, device="cuda")
+    wide[1:4, 4: 4 + table.shape[1]] = table
+    part = wide[1:4, 4: 4 + table.shape[1]]
+    twin = [p.clone() for p in pools]
+    mass, twin_mass = c.mass.cuda(), c.mass.cuda()
+    new = [rand(c.g, 3, 2, 1, 64).cuda() for _ in range(4)]
+    Q = rand(c.g, 3, 3, 64).cuda()
+    results = []
+    for ps, m, t in ((pools, mass, part), (twin, twin_mass, table)):
+        gather_cache_append(ps, t, n, *new, mass=m)
+        y = single_gather_decode(Q, ps, t, n + 2, window=50, sinks=1, mass=m)
+        kept, left = gather_cache_evict(ps, m, t, n + 2, 40, sinks=1, recent=3)
+        results.append((y, kept, left, m, *ps))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    ck.device_status()
+
+
+def test_queries_behind_a_count_need_no_angles():
+    """A padded batch at the end of the angle table: the padding's positions lie behind it."""
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append, rotary_table
+    for Hkv, Hq in ((1, 1), (2, 4)):
+        c = Made(14, [60, 10], Hkv, 64, 16, room=8)
+        pools, table, n = c.gpu()
+        rot = rotary_table(64, 64).cuda()
+        new = [torch.randn(2, 8, Hkv, 64, device="cuda") for _ in range(4)]
+        Q = torch.randn(2, 8, Hq, 64, device="cuda")
+        counts = torch.tensor([4, 8], dtype=torch.int32, device="cuda")
+        q = gather_cache_append(pools, table, n, *new, counts=counts, Q=Q, table=rot)
+        ck.device_status()
+        assert torch.isfinite(q).all()
+        gather_cache_append(pools, table, n, *new, counts=counts + torch.tensor([1, 0], dtype=torch.int32, device="cuda"), Q=Q, table=rot)
+        with pytest.raises(RuntimeError, match="position"):
+            ck.device_status()
+
+
+def test_empty_batches():
+    from att3ntion_b200 import gather_cache_append, gather_cache_evict, single_gather_decode
+    pools = [torch.zeros(2, 16, 1, 64, device="cuda", dtype=torch.bfloat16) for _ in range(4)]
+    table, n = torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    new = [torch.zeros(0, 4, 1, 64, device="cuda") for _ in range(4)]
+    assert gather_cache_append(pools, table, n, *new) is None
+    assert gather_cache_append(pools, table, n, *new, Q=torch.zeros(0, 4, 2, 64, device="cuda")).shape == (0, 4, 2, 64)
+    assert single_gather_decode(torch.zeros(0, 2, 64, device="cuda"), pools, table, n).shape == (0, 2, 64)
+    kept, left = gather_cache_evict(pools, torch.zeros(2, 16, 1, device="cuda"), table, n, 5)
+    assert kept.shape == (0, 1, 5) and left.shape == (0,)
+    table, n = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    new = [torch.zeros(3, 0, 1, 64, device="cuda") for _ in range(4)]
+    assert gather_cache_append(pools, table, n, *new, Q=torch.zeros(3, 0, 2, 64, device="cuda")).shape == (3, 0, 2, 64)
+
+
+def test_norm_rotate_captured_with_its_backward():
+    """Forward and backward captured, replayed on new inputs; a capture beside a live eager graph of the same leaves is
+    refused where it can still be refused."""
+    from att3ntion_b200 import norm_rotate, rotary_table
+    x = torch.randn(2, 33, 3, 64, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    dy = torch.randn(2, 33, 3, 64, device="cuda").bfloat16()
+    table = rotary_table(40, 32).cuda()
+
+    def step():
+        y = norm_rotate(x, w, table)
+        return (y, *torch.autograd.grad(y, [x, w], dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        with torch.no_grad():
+            x.normal_()
+            dy.normal_()
+        graph.replay()
+        got_now = [t.detach().clone() for t in got]
+        want = step()
+        for a, b in zip(got_now, want):
+            assert torch.equal(a, b)
+        del want
+    del got                                # it kept the leaves' accumulators of the capture's stream
+    alive = norm_rotate(x, w, table)
+    other = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside the capture"):
+        with torch.cuda.graph(other):
+            step()
+    assert torch.isfinite(alive).all()
+    torch.cuda.synchronize()
+
+
+def test_norm_rotate_gradients_have_no_gradients():
+    from att3ntion_b200 import norm_rotate
+    x = torch.randn(1, 2, 1, 64, device="cuda", requires_grad=True)
+    y = norm_rotate(x, torch.ones(64, device="cuda"))
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(y.float().sum(), x, create_graph=True)
+
+
 # --------------------------------------------------------------------------- the layer
 
 @pytest.mark.parametrize("kw", [dict(window=128, qk_norm=True, rotary_base=10000.0), dict(window=16, qk_norm=True),
