@@ -9,7 +9,7 @@ namespace {
 struct Layout {
     size_t part, rows, row_ref, cols, col_ref, lse, unit_base, tile_base, bytes;
     long long units;
-    int ctas, wide;
+    int ctas, wide, brief;
 };
 
 // The workspace for the longest sequences that the arguments admit.
@@ -19,7 +19,8 @@ Layout layout(int B, int Hq, int Hkv, int D, int window, int sinks, long long ma
     const long long G = Hq / Hkv;
     const long long groups = (seen + 31) / 32;
     auto block = [&](long long heads) { return (heads * groups + 7) / 8; };          // tiles of a block of heads
-    const long long per_key_head = mass ? G * block(1) : G / 8 * groups + (G & 4 ? block(4) : 0) + (G & 2 ? block(2) : 0) + (G & 1 ? block(1) : 0);
+    o.brief = mass && seen <= serve::DEC_KEYS;
+    const long long per_key_head = mass && !o.brief ? G * block(1) : G / 8 * groups + (G & 4 ? block(4) : 0) + (G & 2 ? block(2) : 0) + (G & 1 ? block(1) : 0);
     const long long tiles = static_cast<long long>(B) * Hkv * per_key_head;
     // One step of up to 192 keys a tile in place of two, where the longest needs no more (128 sequences of 8 heads at
     // window 128 with 4 sinks: 42 us in place of 57).  The masses' column sums are laid out for steps of 128.
@@ -34,8 +35,9 @@ Layout layout(int B, int Hq, int Hkv, int D, int window, int sinks, long long ma
     if (mass) {
         o.rows = take((static_cast<size_t>(tiles) + o.ctas) * 8 * 32 * 4);
         o.row_ref = take((static_cast<size_t>(tiles) + o.ctas) * 8 * 4);
-        o.cols = take(static_cast<size_t>(o.units) * 2 * 128 * 4);
-        o.col_ref = take(static_cast<size_t>(o.units) * 2 * 4);
+        const size_t sums = static_cast<size_t>(o.units) * (o.brief ? 8 : 2);
+        o.cols = take(sums * 128 * 4);
+        o.col_ref = take(sums * 4);
         o.lse = take(static_cast<size_t>(B) * Hq * 4);
     }
     o.bytes = at;
@@ -128,6 +130,7 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     p.pages = serve::make_pages(pages->table, pages->table_stride, pages->per_sequence, pages->pages, pages->page_size);
     p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.window = window; p.sinks = sinks;
     p.wide = lay.wide;
+    p.brief = lay.brief;
     p.c2 = sgring::LOG2E / std::sqrt(static_cast<float>(D));
     char* ws = static_cast<char*>(workspace);
     p.part = reinterpret_cast<float*>(ws + lay.part);

@@ -72,8 +72,8 @@ struct DecodeParams {
     float* part;                           // [head + CTA][8 warps] records of D + 4 floats: y, m, l
     float* rows;                           // mass: [tile + CTA][8 warps][32] row sums
     float* row_ref;                        // mass: [tile + CTA][8 warps] the maximum they are relative to
-    float* cols;                           // mass: [unit][2 halves][128] column sums
-    float* col_ref;                        // mass: [unit][2]
+    float* cols;                           // mass: [unit][2 halves][128] column sums, or with `brief` [unit][8 strips][128]
+    float* col_ref;                        // mass: [unit][2] or [unit][8], the maximum they are relative to
     float* lse;                            // mass: [B,Hq] log2 of the softmax sum
     int* unit_base;                        // [B + 1]; the host admits no more than 2^31 - 1 units
     int* tile_base;                        // [B + 1]
@@ -81,6 +81,7 @@ struct DecodeParams {
     // pools as [pages * page_size, Hkv * D], 64 columns of one row, or of `box` rows of a page (0: not used)
     CUtensorMap tmS, tmVs, tmS_box, tmVs_box;
     int box;
+    int brief;                             // with masses, 1: no sequence shows more than 128 slots
     int wide;                              // 1: no sequence shows more than 192 slots, and a tile has one step of up to 192 keys
 };
 
@@ -101,7 +102,7 @@ __device__ __forceinline__ Shape shape_of(const DecodeParams& p, int b, bool tel
     s.seen = p.window > 0 ? min(s.n, p.window + p.sinks) : s.n;
     s.skip = s.n - s.seen;
     s.groups = (s.seen + DEC_STRIP - 1) / DEC_STRIP;
-    if (MASS) s.tiles = p.G * block_tiles(1, s.groups);
+    if (MASS && !p.brief) s.tiles = p.G * block_tiles(1, s.groups);
     else s.tiles = p.G / 8 * s.groups + (p.G & 4 ? block_tiles(4, s.groups) : 0) + (p.G & 2 ? block_tiles(2, s.groups) : 0) +
                    (p.G & 1 ? block_tiles(1, s.groups) : 0);
     s.steps = p.wide ? min(s.seen, 1) : (s.seen + DEC_KEYS - 1) / DEC_KEYS;
@@ -109,12 +110,14 @@ __device__ __forceinline__ Shape shape_of(const DecodeParams& p, int b, bool tel
 }
 
 // A block of query heads: `heads` of them from g0 on (inside the key head), its tiles from tile0 on.  With masses every
-// block is one head, so that a tile's column sums are one head's.
+// block is one head, so that a half's column sums are one head's and can be added up; but where a tile has one key step
+// at most (`brief`) they are kept strip by strip and heads share tiles as without masses (8 heads a key head, 128 key
+// heads: at window 16, one tile in place of eight, 66 -> 27 us, at window 128 72 -> 55).
 struct Block { int g0, log_heads, tile0; };
 
 template <bool MASS>
 __device__ __forceinline__ Block block_of_tile(const DecodeParams& p, const Shape& s, int tile) {
-    if (MASS) {
+    if (MASS && !p.brief) {
         const int per = block_tiles(1, s.groups), g = tile / per;
         return Block{g, 0, g * per};
     }
@@ -143,7 +146,7 @@ __device__ __forceinline__ Block block_of_tile(const DecodeParams& p, const Shap
 
 template <bool MASS>
 __device__ __forceinline__ Block block_of_head(const DecodeParams& p, const Shape& s, int g) {
-    if (MASS) return Block{g, 0, g * block_tiles(1, s.groups)};
+    if (MASS && !p.brief) return Block{g, 0, g * block_tiles(1, s.groups)};
     const int eights = p.G / 8;
     if (g < 8 * eights) return Block{g & ~7, 3, g / 8 * s.groups};
     Block k{8 * eights, 2, eights * s.groups};
@@ -605,7 +608,14 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 }
                 tc_fence_before();
                 warp_arrive(&bars[DB_P_FULL0 + half], lane);
-                if (MASS) {
+                if (MASS && p.brief) {
+                    const size_t at = (static_cast<size_t>(w.unit) + (k - w.k0)) * DEC_TILE_STRIPS + warp;
+                    if (valid > 0) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) p.cols[at * 128 + c * 32 + lane] = col[c];
+                        if (lane == 0) p.col_ref[at] = ref;
+                    }
+                } else if (MASS) {
                     // The half's column sums, relative to the largest of its four maxima: warps 2 and 3 hand theirs to
                     // 0 and 1, then 1 to 0.  (The first warp of a live half has keys, so that maximum is finite.)
                     float* buf = reinterpret_cast<float*>(smem + L::OFF_COL) + half * 256;
@@ -945,22 +955,36 @@ __global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant_
     if (row < 0) return;
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const int tiles0 = p.tile_base[b] + kv * s.tiles;
-    const int step = e / DEC_KEYS, col = e % DEC_KEYS, per_head = block_tiles(1, s.groups);
+    const int step = e / DEC_KEYS, col = e % DEC_KEYS;
     float share = 0.f;
     for (int g = 0; g < p.G; ++g) {
         const float lse = p.lse[b * p.Hq + kv * p.G + g];
-        const int tile = g * per_head + e / 256;
+        const Block k = block_of_head<true>(p, s, g);
+        auto strip_of = [&](int group) { return (group << k.log_heads) + g - k.g0; };
+        // as j: the row's sums, of every CTA that took a part of the tile's keys
+        const int mine = strip_of(e / DEC_STRIP), tile = k.tile0 + mine / DEC_TILE_STRIPS;
         const int u = units0 + tile * s.steps;
         const int c0 = cta_of(u, total, ctas), c1 = cta_of(u + s.steps - 1, total, ctas);
         for (int c = c0; c <= c1; ++c) {
             if (stretch(total, c, ctas) >= stretch(total, c + 1, ctas)) continue;
-            const size_t rec = static_cast<size_t>(tiles0 + tile + c) * DEC_TILE_STRIPS + (e % 256) / DEC_STRIP;
+            const size_t rec = static_cast<size_t>(tiles0 + tile + c) * DEC_TILE_STRIPS + mine % DEC_TILE_STRIPS;
             share += p.rows[rec * DEC_STRIP + e % DEC_STRIP] * fast_exp2(p.row_ref[rec] - lse);
         }
-        for (int t = 0; t < per_head; ++t) {
-            const size_t at = (static_cast<size_t>(units0) + (g * per_head + t) * s.steps + step) * 2;
-            share += p.cols[at * 128 + col] * fast_exp2(p.col_ref[at] - lse);
-            if (t * 256 + 128 < s.seen) share += p.cols[(at + 1) * 128 + col] * fast_exp2(p.col_ref[at + 1] - lse);
+        // as k: the column's sums over the head's rows
+        if (p.brief) {
+#pragma unroll 4
+            for (int group = 0; group < s.groups; ++group) {
+                const int strip = strip_of(group);
+                const size_t at = (static_cast<size_t>(units0) + k.tile0 + strip / DEC_TILE_STRIPS) * DEC_TILE_STRIPS + strip % DEC_TILE_STRIPS;
+                share += p.cols[at * 128 + col] * fast_exp2(p.col_ref[at] - lse);
+            }
+        } else {
+#pragma unroll 4
+            for (int t = 0; t < block_tiles(1, s.groups); ++t) {
+                const size_t at = (static_cast<size_t>(units0) + (k.tile0 + t) * s.steps + step) * 2;
+                share += p.cols[at * 128 + col] * fast_exp2(p.col_ref[at] - lse);
+                if (t * 256 + 128 < s.seen) share += p.cols[(at + 1) * 128 + col] * fast_exp2(p.col_ref[at + 1] - lse);
+            }
         }
     }
     p.mass[static_cast<long long>(row) * p.Hkv + kv] += share / (2.f * p.G);

@@ -242,6 +242,9 @@ DECODE_CASES = [
     ([77, 900, 16], 8, 8, 64, 16, 1, 3),
     ([600, 256], 4, 1, 128, 256, 300, 37),
     ([50] * 40, 8, 4, 128, 16, 33, 1),
+    # at most 128 visible slots, heads in blocks of 8, 4, 2 and 1
+    ([40, 3, 128, 97, 0, 31], 15, 1, 64, 16, 100, 7),
+    ([20, 1, 16], 22, 2, 128, 32, 0, 0),
     # at most 192 visible slots: one step of keys a tile
     ([192, 191, 129, 160, 161, 5, 0], 8, 2, 128, 32, 0, 0),
     ([1000, 193, 192, 150, 40], 3, 1, 128, 16, 150, 42),
