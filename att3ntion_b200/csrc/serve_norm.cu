@@ -34,9 +34,9 @@ __device__ int g_serve_status = 0;
 
 constexpr int THREADS = 256;
 constexpr int LINE = 8;                            // rows of an item, the unit of work of D / 8 lanes
-constexpr int FWD_ROWS = 4, BWD_ROWS = 2;          // rows in flight
+constexpr int FWD_ROWS = 4;                        // rows in flight
 constexpr int MAX_TENSORS = 5;
-constexpr int FWD_BLOCKS_PER_SM = 16, BWD_BLOCKS_PER_SM = 6;       // at most; a block then takes several items a group
+constexpr int FWD_BLOCKS_PER_SM = 32, BWD_BLOCKS_PER_SM = 6;       // at most; a block then takes several items a group
 
 struct Tensor {
     const void* x;
@@ -283,6 +283,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 4 : 3) norm_rotate_
 // Adds the rows' share of dw to `dw`, a lane its eight columns.
 template <typename XT, int D, bool ONE>
 __device__ __forceinline__ void backward_rows(const Params& p, const Tensor& t, const Columns& cols, int lr, float (&dw)[8]) {
+    // rows in flight: registers go further with four of 16 bits and two blocks an SM than with two and three (65 us against
+    // 77 for 32768 tokens of 10 heads of 128); FP32 rows the other way round (37 against 25 for 8188 tokens of 24 of 64)
+    constexpr int BWD_ROWS = sizeof(XT) == 2 ? 4 : 2;
     constexpr int LANES = D / 8, GROUPS = THREADS / LANES;
     const bool turns = t.rotate && cols.turns, normed = t.w != nullptr, interleaved = p.interleaved != 0;
     const float eps = p.eps;
@@ -358,7 +361,7 @@ __device__ __forceinline__ void backward_rows(const Params& p, const Tensor& t, 
 }
 
 template <typename XT, int D>
-__global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 3 : 2) norm_rotate_backward_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, 2) norm_rotate_backward_kernel(const __grid_constant__ Params p) {
     constexpr int LANES = D / 8, GROUPS = THREADS / LANES;
     __shared__ float sums[GROUPS][D];
     const Tensor& t = p.t[find_tensor(p)];
@@ -381,21 +384,23 @@ __global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 3 : 2) norm_rotate_
     }
 }
 
-// dw of one tensor a block: the planes of its blocks, added in a fixed order (a strided quarter or more each, then those).
-template <int D>
-__global__ void __launch_bounds__(1024) scale_grad_kernel(const __grid_constant__ Params p) {
-    constexpr int PARTS = 1024 / D;
-    __shared__ float sums[PARTS][D];
+// dw of 16 columns of one tensor: the planes of its blocks, added in a fixed order (64 shares, then those).  Set up while
+// the rows' kernel runs out.
+constexpr int GRAD_COLS = 16, GRAD_PARTS = 64;
+__global__ void __launch_bounds__(GRAD_COLS * GRAD_PARTS) scale_grad_kernel(const __grid_constant__ Params p, int D) {
+    __shared__ float sums[GRAD_PARTS][GRAD_COLS];
     const Tensor& t = p.t[blockIdx.x];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!t.w) return;
-    const int col = threadIdx.x % D, part = threadIdx.x / D;
+    const int c = threadIdx.x % GRAD_COLS, part = threadIdx.x / GRAD_COLS, col = blockIdx.y * GRAD_COLS + c;
     float a = 0.f;
 #pragma unroll 8
-    for (int q = part; q < t.blocks; q += PARTS) a += p.partial[static_cast<long long>(t.block0 + q) * D + col];
-    sums[part][col] = a;
+    for (int q = part; q < t.blocks; q += GRAD_PARTS) a += p.partial[static_cast<long long>(t.block0 + q) * D + col];
+    sums[part][c] = a;
     __syncthreads();
     if (part == 0) {
-        for (int q = 1; q < PARTS; ++q) a += sums[q][col];
+#pragma unroll 16
+        for (int q = 1; q < GRAD_PARTS; ++q) a += sums[q][c];
         t.dw[col] = a;
     }
 }
@@ -581,10 +586,17 @@ extern "C" int att3_norm_rotate_backward(const att3_head_rows* tensors, int n, i
 #undef ATT3_NR
     }
     if (scaled) {                                   // with no rows at all this writes the gradient's zeros
-        if (D == 16) scale_grad_kernel<16><<<n, 1024, 0, st>>>(p);
-        else if (D == 32) scale_grad_kernel<32><<<n, 1024, 0, st>>>(p);
-        else if (D == 64) scale_grad_kernel<64><<<n, 1024, 0, st>>>(p);
-        else scale_grad_kernel<128><<<n, 1024, 0, st>>>(p);
+        cudaLaunchAttribute early = {};
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(n, D / GRAD_COLS);
+        cfg.blockDim = dim3(GRAD_COLS * GRAD_PARTS);
+        cfg.stream = st;
+        cfg.attrs = &early;
+        cfg.numAttrs = 1;
+        const cudaError_t launched = cudaLaunchKernelEx(&cfg, scale_grad_kernel, p, D);
+        if (launched != cudaSuccess) return att3::set_cuda_error(launched, who);
     }
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? ATT3_OK : att3::set_cuda_error(e, who);
