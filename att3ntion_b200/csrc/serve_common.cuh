@@ -14,6 +14,26 @@
 
 namespace serve {
 
+// The serving kernels are short and follow one another, so each is launched to be set up while the kernel before it in
+// the stream runs out (programmatic dependent launch), and waits for that kernel's end itself, before it touches memory.
+// Every thread does: a kernel that ended without waiting could end before the one it depends on.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 enum Status { ST_WAIT = 1, ST_PAGE = 0x100, ST_POSITION = 0x200, ST_LENGTH = 0x400 };
 
 __device__ __forceinline__ void report(int* status, int what) { atomicOr(status, what); }

@@ -61,26 +61,10 @@ int launch(const serve::DecodeParams& p, const Layout& lay, long long max_seen, 
     if (e != cudaSuccess) return att3::set_cuda_error(e, who);
     att3::count_launch(4, MASS ? 3 : 2);
     const att3::TimedLaunch timed(att3::K_SERVE, st);
-    serve::decode_kernel<D, MASS, WIDE><<<lay.ctas, serve::DEC_THREADS, smem, st>>>(p);
-    // the joining kernels may be set up while the one before them runs out; they wait for its end themselves
-    cudaLaunchAttribute early = {};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.stream = st;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3(p.B * p.Hq);
-    cfg.blockDim = dim3(256);
-    e = cudaLaunchKernelEx(&cfg, serve::decode_join_kernel<D, MASS>, p, lay.ctas);
-    if (e != cudaSuccess) return att3::set_cuda_error(e, who);
-    if (MASS) {
-        cfg.gridDim = dim3(static_cast<unsigned>((max_seen + 127) / 128), p.B * p.Hkv);
-        cfg.blockDim = dim3(128);
-        e = cudaLaunchKernelEx(&cfg, serve::decode_mass_kernel, p, lay.ctas);
-        if (e != cudaSuccess) return att3::set_cuda_error(e, who);
-    }
-    e = cudaGetLastError();
+    e = serve::launch_early(serve::decode_kernel<D, MASS, WIDE>, dim3(lay.ctas), dim3(serve::DEC_THREADS), smem, st, p);
+    if (e == cudaSuccess) e = serve::launch_early(serve::decode_join_kernel<D, MASS>, dim3(p.B * p.Hq), dim3(256), 0, st, p, lay.ctas);
+    if (MASS && e == cudaSuccess)
+        e = serve::launch_early(serve::decode_mass_kernel, dim3(static_cast<unsigned>((max_seen + 127) / 128), p.B * p.Hkv), dim3(128), 0, st, p, lay.ctas);
     return e == cudaSuccess ? ATT3_OK : att3::set_cuda_error(e, who);
 }
 

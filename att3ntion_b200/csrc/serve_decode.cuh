@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
     constexpr float GROW = 8.f;            // a strip's reference maximum is renewed when a score exceeds it by 2^8
     extern __shared__ __align__(1024) uint8_t smem[];
     if ((smem_u32(smem) & 1023u) != 0) {   // the operand tiles' swizzle wants it; there is no room to align by hand
+        wait_for_previous_kernel();
         if (threadIdx.x == 0) report(p.status, 10);
         return;
     }
@@ -324,6 +325,19 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
     // ---- this CTA's stretch: units and tiles before every sequence, a run of sequences a thread
     int total;
     {
+        if (tid == 0) {
+            mbar_init(&bars[DB_A_FULL0], 4); mbar_init(&bars[DB_A_FULL1], 4);
+            mbar_init(&bars[DB_S_FULL0], 1); mbar_init(&bars[DB_S_FULL1], 1);
+            mbar_init(&bars[DB_P_FULL0], 4); mbar_init(&bars[DB_P_FULL1], 4);
+            mbar_init(&bars[DB_O_DONE0], 1); mbar_init(&bars[DB_O_DONE1], 1);
+            mbar_init(&bars[DB_DRAIN], 1);
+            mbar_init(&bars[DB_COL0], 4); mbar_init(&bars[DB_COL1], 4);
+            for (int x = 0; x < 8; ++x) { mbar_init(&bars[DB_KV_FULL0 + x], 1); mbar_init(&bars[DB_KV_EMPTY0 + x], 1); }
+            fence_mbar_init();
+            *fail = 0;
+        }
+        if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+        wait_for_previous_kernel();
         const int per = (p.B + DEC_THREADS - 1) / DEC_THREADS;
         const int lo = min(tid * per, p.B), hi = min(lo + per, p.B);
         int units = 0, tiles = 0;
@@ -339,18 +353,6 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             if (lane >= o) { iu += yu; it += yt; }
         }
         if (lane == 31) { sh_sum[warp][0] = iu; sh_sum[warp][1] = it; }
-        if (tid == 0) {
-            mbar_init(&bars[DB_A_FULL0], 4); mbar_init(&bars[DB_A_FULL1], 4);
-            mbar_init(&bars[DB_S_FULL0], 1); mbar_init(&bars[DB_S_FULL1], 1);
-            mbar_init(&bars[DB_P_FULL0], 4); mbar_init(&bars[DB_P_FULL1], 4);
-            mbar_init(&bars[DB_O_DONE0], 1); mbar_init(&bars[DB_O_DONE1], 1);
-            mbar_init(&bars[DB_DRAIN], 1);
-            mbar_init(&bars[DB_COL0], 4); mbar_init(&bars[DB_COL1], 4);
-            for (int x = 0; x < 8; ++x) { mbar_init(&bars[DB_KV_FULL0 + x], 1); mbar_init(&bars[DB_KV_EMPTY0 + x], 1); }
-            fence_mbar_init();
-            *fail = 0;
-        }
-        if (warp == 8) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
         __syncthreads();
         int bu = 0, bt = 0, tt = 0;
         total = 0;
@@ -883,9 +885,6 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
     if (tid == 0 && *fail) report(p.status, *fail & 0xFF);
 }
 
-// Waits for the kernel before it in the stream, which it may have been started ahead of.
-__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // The partials of one head, shared out over eight warps and added in a fixed order; a warp's lanes take the columns.
 template <int D, bool MASS>
 __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant__ DecodeParams p, int ctas) {
@@ -893,14 +892,13 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant_
     __shared__ float sh_m[8], sh_l[8], sh_y[8][D];
     const int b = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq, kv = hq / p.G, g = hq % p.G;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    wait_for_previous_kernel();
     const Shape s = shape_of<MASS>(p, b);
     __nv_bfloat16* y = p.Y + static_cast<size_t>(blockIdx.x) * D;
     if (s.seen == 0) {
-        wait_for_previous_kernel();
         if (threadIdx.x < D) y[threadIdx.x] = __float2bfloat16_rn(0.f);
         return;
     }
-    wait_for_previous_kernel();
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const Block k = block_of_head<MASS>(p, s, g);
     const int u0 = units0 + k.tile0 * s.steps, u1 = u0 + block_tiles(1 << k.log_heads, s.groups) * s.steps;
@@ -948,10 +946,10 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant_
 // Adds every visible slot's share of the attention to its mass: a thread a slot, the heads and partials in a fixed order.
 __global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant__ DecodeParams p, int ctas) {
     const int b = blockIdx.y / p.Hkv, kv = blockIdx.y % p.Hkv;
+    wait_for_previous_kernel();
     const Shape s = shape_of<true>(p, b);
     const int e = blockIdx.x * 128 + threadIdx.x;
     const int row = e < s.seen ? p.pages.row(b, slot_of(p, s, e)) : -1;
-    wait_for_previous_kernel();            // every block does, so that this kernel never ends before that one
     if (row < 0) return;
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const int tiles0 = p.tile_base[b] + kv * s.tiles;

@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
     __shared__ int hist[BINS];
     __shared__ int2 warp_sums[SEL_THREADS / 32];
     __shared__ int chosen[2];
+    serve::wait_for_previous_kernel();
     const int h = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv, tid = threadIdx.x;
     const int n = p.src.length(p.lengths, b, p.status, tid == 0 && h == 0);
     int* kept = p.kept + static_cast<long long>(blockIdx.x) * p.keep;
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
 __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_constant__ Params p) {
     constexpr int MOST = MOVE_THREADS * MOVE_UNROLL;                   // rows of a chunk: that many of masses, fewer of pools
     __shared__ int from[2][MOST / 2], to[2][MOST / 2];
+    serve::wait_for_previous_kernel();
     const int h = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
     const int n = p.src.length(p.lengths, b, p.status, false);
     const int left = min(n, p.keep);
@@ -175,7 +177,6 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
             to[buf][i] = d;
         }
     };
-    asm volatile("griddepcontrol.wait;" ::: "memory");                 // the kept slots
     look(0, 0);
     __syncthreads();
     int buf = 0;
@@ -267,17 +268,7 @@ extern "C" int att3_gather_cache_evict(void* R, void* S, void* Vr, void* Vs, flo
     if (e != cudaSuccess) return att3::set_cuda_error(e, who);
     att3::count_launch(4, 2);
     const att3::TimedLaunch timed(att3::K_SERVE, st);
-    select_kernel<<<B * Hkv, SEL_THREADS, smem, st>>>(p);
-    // the second kernel may be set up while the first runs out; it waits for its end itself
-    cudaLaunchAttribute early = {};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(B * Hkv, 4 * p.slices + 1);
-    cfg.blockDim = dim3(MOVE_THREADS);
-    cfg.stream = st;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, move_kernel, p);
+    e = serve::launch_early(select_kernel, dim3(B * Hkv), dim3(SEL_THREADS), smem, st, p);
+    if (e == cudaSuccess) e = serve::launch_early(move_kernel, dim3(B * Hkv, 4 * p.slices + 1), dim3(MOVE_THREADS), 0, st, p);
     return e == cudaSuccess ? ATT3_OK : att3::set_cuda_error(e, who);
 }

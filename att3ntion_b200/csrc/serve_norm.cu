@@ -274,6 +274,7 @@ __device__ __forceinline__ void forward_rows(const Params& p, const Tensor& t, i
 
 template <typename XT, int D, bool PAGED>
 __global__ void __launch_bounds__(THREADS, sizeof(XT) == 2 ? 4 : 3) norm_rotate_kernel(const __grid_constant__ Params p) {
+    serve::wait_for_previous_kernel();
     const int ti = find_tensor(p);
     const Tensor& t = p.t[ti];
     if (t.heads == 1) forward_rows<XT, D, PAGED, true>(p, t, ti);
@@ -364,6 +365,7 @@ template <typename XT, int D>
 __global__ void __launch_bounds__(THREADS, 2) norm_rotate_backward_kernel(const __grid_constant__ Params p) {
     constexpr int LANES = D / 8, GROUPS = THREADS / LANES;
     __shared__ float sums[GROUPS][D];
+    serve::wait_for_previous_kernel();
     const Tensor& t = p.t[find_tensor(p)];
     const int lr = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const Columns cols = columns_of(p, lr);
@@ -384,13 +386,12 @@ __global__ void __launch_bounds__(THREADS, 2) norm_rotate_backward_kernel(const 
     }
 }
 
-// dw of 16 columns of one tensor: the planes of its blocks, added in a fixed order (64 shares, then those).  Set up while
-// the rows' kernel runs out.
+// dw of 16 columns of one tensor: the planes of its blocks, added in a fixed order (64 shares, then those).
 constexpr int GRAD_COLS = 16, GRAD_PARTS = 64;
 __global__ void __launch_bounds__(GRAD_COLS * GRAD_PARTS) scale_grad_kernel(const __grid_constant__ Params p, int D) {
     __shared__ float sums[GRAD_PARTS][GRAD_COLS];
     const Tensor& t = p.t[blockIdx.x];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    serve::wait_for_previous_kernel();
     if (!t.w) return;
     const int c = threadIdx.x % GRAD_COLS, part = threadIdx.x / GRAD_COLS, col = blockIdx.y * GRAD_COLS + c;
     float a = 0.f;
@@ -480,14 +481,15 @@ int launch_forward(const Params& p, int x_type, int D, cudaStream_t st, const ch
     if (blocks == 0) return ATT3_OK;
     att3::count_launch(4);
     const att3::TimedLaunch timed(att3::K_SERVE, st);
-#define ATT3_NR(T, DD) norm_rotate_kernel<T, DD, PAGED><<<blocks, THREADS, 0, st>>>(p)
+    cudaError_t e = cudaSuccess;
+#define ATT3_NR(T, DD) e = serve::launch_early(norm_rotate_kernel<T, DD, PAGED>, dim3(blocks), dim3(THREADS), 0, st, p)
 #define ATT3_NR_D(T) do { if (D == 16) ATT3_NR(T, 16); else if (D == 32) ATT3_NR(T, 32); else if (D == 64) ATT3_NR(T, 64); else ATT3_NR(T, 128); } while (0)
     if (x_type == 0) ATT3_NR_D(__nv_bfloat16);
     else if (x_type == 1) ATT3_NR_D(__half);
     else ATT3_NR_D(float);
 #undef ATT3_NR_D
 #undef ATT3_NR
-    const cudaError_t e = cudaGetLastError();
+
     return e == cudaSuccess ? ATT3_OK : att3::set_cuda_error(e, who);
 }
 
@@ -576,8 +578,9 @@ extern "C" int att3_norm_rotate_backward(const att3_head_rows* tensors, int n, i
     const int blocks = total_blocks(p);
     att3::count_launch(4, (blocks ? 1 : 0) + (scaled ? 1 : 0));
     const att3::TimedLaunch timed(att3::K_SERVE, st);
+    cudaError_t e = cudaSuccess;
     if (blocks) {
-#define ATT3_NR(T, DD) norm_rotate_backward_kernel<T, DD><<<blocks, THREADS, 0, st>>>(p)
+#define ATT3_NR(T, DD) e = serve::launch_early(norm_rotate_backward_kernel<T, DD>, dim3(blocks), dim3(THREADS), 0, st, p)
 #define ATT3_NR_D(T) do { if (D == 16) ATT3_NR(T, 16); else if (D == 32) ATT3_NR(T, 32); else if (D == 64) ATT3_NR(T, 64); else ATT3_NR(T, 128); } while (0)
         if (x_type == 0) ATT3_NR_D(__nv_bfloat16);
         else if (x_type == 1) ATT3_NR_D(__half);
@@ -585,20 +588,9 @@ extern "C" int att3_norm_rotate_backward(const att3_head_rows* tensors, int n, i
 #undef ATT3_NR_D
 #undef ATT3_NR
     }
-    if (scaled) {                                   // with no rows at all this writes the gradient's zeros
-        cudaLaunchAttribute early = {};
-        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        early.val.programmaticStreamSerializationAllowed = 1;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(n, D / GRAD_COLS);
-        cfg.blockDim = dim3(GRAD_COLS * GRAD_PARTS);
-        cfg.stream = st;
-        cfg.attrs = &early;
-        cfg.numAttrs = 1;
-        const cudaError_t launched = cudaLaunchKernelEx(&cfg, scale_grad_kernel, p, D);
-        if (launched != cudaSuccess) return att3::set_cuda_error(launched, who);
-    }
-    const cudaError_t e = cudaGetLastError();
+    // with no rows at all this writes the gradient's zeros
+    if (e == cudaSuccess && scaled)
+        e = serve::launch_early(scale_grad_kernel, dim3(n, D / GRAD_COLS), dim3(GRAD_COLS * GRAD_PARTS), 0, st, p, D);
     return e == cudaSuccess ? ATT3_OK : att3::set_cuda_error(e, who);
 }
 
