@@ -471,6 +471,49 @@ def test_captured_step_follows_the_lengths():
     ck.device_status()
 
 
+def test_captured_on_two_streams_that_fork_and_join():
+    """Each kernel follows the ones that it reads from, whichever stream and kind of work they came from."""
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append, norm_rotate, rotary_table, single_gather_decode
+    B, Hq, Hkv, D, page = 3, 4, 2, 64, 16
+    c = Made(21, [10, 120, 63], Hkv, D, page, room=40)
+    pools, table, n = c.gpu()
+    rot = rotary_table(200, D).cuda()
+    w = torch.rand(D, device="cuda")
+    new = [torch.randn(B, 1, Hkv, D, device="cuda") for _ in range(4)]
+    Q = torch.randn(B, 1, Hq, D, device="cuda")
+    big = torch.randn(1 << 22, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step(ps, lengths):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            q = norm_rotate(Q * (1 + big.sum().tanh()), weights=w, table=rot, positions=lengths[:, None])
+        gather_cache_append(ps, table, lengths, *new, weights=[None, w, w], table=rot)
+        seen = lengths + 1
+        here.wait_stream(side)
+        y = single_gather_decode(q[:, 0], ps, table, seen, window=64)
+        return y, norm_rotate(y[:, None], weights=w)
+
+    twin = [p.clone() for p in pools]
+    want = step([p.clone() for p in pools], n)                         # warm-up outside the capture
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = step(pools, n)
+    for _ in range(5):
+        for x in (*new, Q, big):
+            x.normal_()
+        n.add_(1)
+        want = step(twin, n)
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(pools, twin))
+    ck.device_status()
+
+
 def test_tables_that_are_part_of_a_larger_one():
     """Page tables and lengths as slices of a server's own."""
     from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append, gather_cache_evict, single_gather_decode
