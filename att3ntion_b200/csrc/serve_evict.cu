@@ -11,7 +11,9 @@
 // order serves fresh pages.  Rows that stay where they are cost nothing.  While a chunk's rows are on their way, the
 // next chunk's places are looked up (kept slot, page, row: three dependent loads), one thread a row.
 //
-// The move is bound by memory traffic (16 D + 4 bytes read and written per kept token and key head).
+// The move is bound by memory traffic (16 D + 4 bytes read and written per kept token and key head): 32 sequences of
+// 8000 slots down to 4000, 4 key heads of 128: 193 us, 5.5 TB/s of rows of 256 bytes, 0.84 of a plain copy's rate; the
+// selection before it 22 us.  Two sequences of 700 down to 333 take 9 and 4 us, bound by the latency of the passes.
 #include <algorithm>
 
 #include "att3_abi_internal.h"
