@@ -160,8 +160,8 @@ def gather_cache_evict(pools, mass, page_table, lengths, keep, *, sinks=0, recen
     """Trims every sequence and key head to min(lengths[b], keep) slots: the first `sinks`, the last `recent` and, between
     them, those with the largest `mass` (equal ones: the lowest slots; NaN counts as largest).  The kept rows of all
     pools move with their mass, in order, to slots 0 .. , in place, or to the pages of `out_table`, which must then name
-    none that a sequence of the call reads.  Slots behind the last kept one are left as they are.  Key heads of a
-    sequence may keep different slots.
+    none that a sequence of the call reads; in place, no two sequences may share a page.  Slots behind the last kept one
+    are left as they are.  Key heads of a sequence may keep different slots.
 
     Returns (kept int32 [B,Hkv,keep], the slots that stayed, -1 behind the last; new lengths int32 [B])."""
     got = _accepted(_native.evict, pools, mass, page_table, lengths, keep, sinks, recent, out_table)
