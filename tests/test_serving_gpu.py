@@ -514,6 +514,36 @@ def test_captured_on_two_streams_that_fork_and_join():
     ck.device_status()
 
 
+def test_pages_past_32_bits_of_a_pool():
+    """The same rows on pages that begin 2^31 elements (2^32 bytes) into the pools give the same bits."""
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append, gather_cache_evict, rotary_table, single_gather_decode
+    Hkv, D, page = 8, 128, 64
+    c = Made(23, [300, 45], Hkv, D, page, room=1)
+    near, table, n = c.gpu()
+    count, skip = near[0].shape[0], (1 << 31) // (page * Hkv * D)
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 18 GB")
+    far = [torch.empty(skip + count, page, Hkv, D, dtype=torch.bfloat16, device="cuda") for _ in near]
+    for f, x in zip(far, near):
+        f[skip:] = x
+    moved = torch.where(table < 0, table, table + skip)
+    masses = [c.mass.cuda(), torch.zeros(skip + count, page, Hkv, device="cuda")]
+    masses[1][skip:] = masses[0]
+    new = [torch.randn(2, 1, Hkv, D, device="cuda") for _ in range(4)]
+    Q = torch.randn(2, 8, D, device="cuda", dtype=torch.bfloat16)
+    rot = rotary_table(400, D).cuda()
+    got = []
+    for pools, pages, mass in ((near, table, masses[0]), (far, moved, masses[1])):
+        gather_cache_append(pools, pages, n, *new, table=rot, mass=mass)
+        seen = n + 1
+        out = [single_gather_decode(Q, pools, pages, seen, mass=mass), single_gather_decode(Q, pools, pages, seen, window=100, sinks=2)]
+        out += [single_gather_decode(Q, pools, pages, seen)]
+        out += gather_cache_evict(pools, mass, pages, seen, 90, sinks=2, recent=10)
+        got.append(out + [p[-count:] for p in pools] + [mass[-count:]])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    ck.device_status()
+
+
 def test_tables_that_are_part_of_a_larger_one():
     """Page tables and lengths as slices of a server's own."""
     from att3ntion_b200 import _cuda_kernels as ck, gather_cache_append, gather_cache_evict, single_gather_decode
