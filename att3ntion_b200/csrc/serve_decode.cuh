@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
             mbar_init(&bars[DB_O_DONE0], 1); mbar_init(&bars[DB_O_DONE1], 1);
             mbar_init(&bars[DB_DRAIN], 1);
             mbar_init(&bars[DB_COL0], 4); mbar_init(&bars[DB_COL1], 4);
-            for (int x = 0; x < 8; ++x) { mbar_init(&bars[DB_KV_FULL0 + x], 1); mbar_init(&bars[DB_KV_EMPTY0 + x], 1); }
+            for (int x = 0; x < 8; ++x) { mbar_init(&bars[DB_KV_FULL0 + x], DEC_COPY_WARPS); mbar_init(&bars[DB_KV_EMPTY0 + x], 1); }
             fence_mbar_init();
             *fail = 0;
         }
@@ -861,8 +861,13 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                         uint64_t* full = &bars[DB_KV_FULL0 + st];
                         if (fill >= stages) ok = pipe_wait(&bars[DB_KV_EMPTY0 + st], (fill / stages - 1) & 1, fail, 8);
                         if (!ok) break;
-                        // one arrival, of the thread that names the bytes; other warps' bytes may come before it
-                        if (warp == 9 && lane == 0) mbar_arrive_expect_tx(full, wanted * D * 2);
+                        // One arrival of every copy warp, the one of warp 9 names the bytes; other warps' bytes may come before
+                        // it.  A warp without a box of its own (boxes of 64 rows and more) arrives too: a stage that went
+                        // round twice while it waits for the first would look to it as if it had not gone round at all.
+                        if (lane == 0) {
+                            if (warp == 9) mbar_arrive_expect_tx(full, wanted * D * 2);
+                            else mbar_arrive(full);
+                        }
                         __syncwarp();
                         if (any) {
                             uint8_t* dst = smem + L::OFF_KV + st * stage_bytes + mine * rows * 128;

@@ -784,3 +784,23 @@ def test_cache_run_append_decode_evict_decode():
         check(step(1, None)[:, 0])
     cache.clear(0)
     assert cache.lengths.tolist() == [0, 26] and len(cache._free) == 24 - 4
+
+
+# --------------------------------------------------------------------------- what the calls above left out
+
+@pytest.mark.parametrize("page", [64, 128, 384])
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_whole_boxes_many_times_round_the_ring(page, D):
+    """Pages whose boxes leave copy warps without work, stretches of many key steps, repeated: same bits, no wait given up."""
+    from att3ntion_b200 import _cuda_kernels as ck, single_gather_decode
+    lengths = [4000, 129, 2560]
+    c = Made(31, lengths, 2, D, page)
+    Q = rand(c.g, 3, 4, D)
+    pools, table, n = c.gpu()
+    q = Q.cuda()
+    first = single_gather_decode(q, pools, table, n)
+    for _ in range(50):
+        assert torch.equal(single_gather_decode(q, pools, table, n), first)
+    ck.device_status()
+    Y64, A, _ = ref.decode(Q[1:2], c.pools, c.table[1:2], lengths[1:2])
+    close(first[1:2], Y64, (1 + HALF) * HALF * (Y64.abs() + A) + 2e-4 * A, "Y")

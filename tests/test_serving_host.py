@@ -278,3 +278,59 @@ def test_layer_arguments():
     cache.host_lengths[0] = 3
     with pytest.raises(ValueError, match="empty"):
         layer.prefill(torch.zeros(2, 4, 128), cache)
+
+
+# --------------------------------------------------------------------------- the decode's ring of stages
+
+class Phases:
+    """An mbarrier as its waiters see it: only the parity of the running phase."""
+
+    def __init__(self, arrivals):
+        self.need, self.left, self.done = arrivals, arrivals, 0
+
+    def arrive(self):
+        self.left -= 1
+        if self.left == 0:
+            self.done, self.left = self.done + 1, self.need
+
+    def passes(self, parity):
+        return self.done % 2 != parity
+
+
+def ring_ends(arrivals, busy, fills, stages, last):
+    """Copy warps of the ring (busy[w]: it has bytes to bring) and its reader, one step at a time, warp `last` only when no
+    other can go on: whether all of them end."""
+    full, empty = [Phases(arrivals) for _ in range(stages)], [Phases(1) for _ in range(stages)]
+    landed, at, read = [0] * fills, [0] * len(busy), 0
+
+    def copy_step(w):
+        f = at[w]
+        if f == fills or (f >= stages and not empty[f % stages].passes((f // stages - 1) % 2)):
+            return False
+        if w == 0 or arrivals > 1:
+            full[f % stages].arrive()
+        landed[f] += busy[w]
+        at[w] += 1
+        return True
+
+    while True:
+        if read < fills and full[read % stages].passes((read // stages) % 2) and landed[read] == sum(busy):
+            empty[read % stages].arrive()
+            read += 1
+        elif not any(copy_step(w) for w in range(len(busy)) if w != last) and not copy_step(last):
+            return read == fills and all(a == fills for a in at)
+
+
+@pytest.mark.parametrize("stages", [3, 8])
+@pytest.mark.parametrize("busy", [(1, 0, 0), (1, 1, 0), (1, 1, 1)])
+def test_no_copy_warp_misses_a_phase_of_the_ring(stages, busy):
+    """Boxes of 128 rows leave two of the three copy warps without work, boxes of 64 one.  Whichever of them is late, the
+    ring's barriers must not go round twice meanwhile; with one arrival a stage they could."""
+    source = (REPO / "att3ntion_b200" / "csrc" / "serve_decode.cuh").read_text()
+    warps = re.search(r"DEC_COPY_WARPS = (\d+);", source).group(1)
+    count = re.search(r"mbar_init\(&bars\[DB_KV_FULL0 \+ x\], (\w+)\)", source).group(1)
+    arrivals = int(warps if count == "DEC_COPY_WARPS" else count)
+    for fills in range(1, 8 * stages):
+        for last in range(3):
+            assert ring_ends(arrivals, busy, fills, stages, last), (fills, last)
+    assert not all(ring_ends(1, (1, 0, 0), fills, stages, 1) for fills in range(1, 8 * stages))
