@@ -16,7 +16,9 @@ namespace serve {
 
 // The serving kernels are short and follow one another, so each is launched to be set up while the kernel before it in
 // the stream runs out (programmatic dependent launch), and waits for that kernel's end itself, before it touches memory.
-// Every thread does: a kernel that ended without waiting could end before the one it depends on.
+// Every thread does: a kernel that ended without waiting could end before the one it depends on.  What they read may
+// have been written while they were already being set up, so none of it goes through read-only loads (__ldg), which want
+// memory that stays as it is for a kernel's whole life.
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <typename... Params, typename... Args>
@@ -50,13 +52,13 @@ struct Pages {
     __device__ __forceinline__ int row(int b, int slot) const {
         const unsigned p = shift >= 0 ? static_cast<unsigned>(slot) >> shift : static_cast<unsigned>(slot) / static_cast<unsigned>(size);
         if (slot < 0 || p >= static_cast<unsigned>(per_seq)) return -1;
-        const int page = __ldg(table + b * stride + p);
+        const int page = table[b * stride + p];
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(count)) return -1;
         return page * size + (slot - static_cast<int>(p) * size);
     }
     // Slots in use, cut to what the table can name.
     __device__ __forceinline__ int length(const int* lengths, int b, int* status, bool tell) const {
-        const int n = __ldg(lengths + b), most = per_seq * size;
+        const int n = lengths[b], most = per_seq * size;
         if (n >= 0 && n <= most) return n;
         if (tell) report(status, ST_LENGTH);
         return n < 0 ? 0 : most;

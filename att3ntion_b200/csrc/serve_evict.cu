@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
     auto fetch = [&](int i) -> uint32_t {
         const int row = p.src.row(b, first + i);
         if (row < 0) { serve::report(p.status, serve::ST_PAGE); return 0u; }
-        return order_key(__ldg(p.mass + static_cast<long long>(row) * p.Hkv + h));
+        return order_key(p.mass[static_cast<long long>(row) * p.Hkv + h]);
     };
     auto key_of = [&](int i) -> uint32_t { return p.cached ? keys[i] : fetch(i); };
     if (p.cached) {
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
     // places of a chunk's rows: source row, target row; the source is -1 where nothing moves
     auto look = [&](int base, int buf) {
         for (int i = threadIdx.x; i < chunk && base + i < left; i += MOVE_THREADS) {
-            int s = p.src.row(b, __ldg(kept + base + i));
+            int s = p.src.row(b, kept[base + i]);
             const int d = p.dst.row(b, base + i);
             if (s < 0 || d < 0) { serve::report(p.status, serve::ST_PAGE); s = -1; }
             from[buf][i] = s == d ? -1 : s;

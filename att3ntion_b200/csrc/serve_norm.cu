@@ -125,8 +125,8 @@ __device__ __forceinline__ Angles load_angles(const Params& p, int pos, int lane
     Angles t{make_float4(1.f, 1.f, 1.f, 1.f), make_float4(0.f, 0.f, 0.f, 0.f)};
     if (turns) {
         const float* row = p.table + static_cast<long long>(pos) * p.rot + lane_in_row * 4;
-        t.c = __ldg(reinterpret_cast<const float4*>(row));
-        t.s = __ldg(reinterpret_cast<const float4*>(row + (p.rot >> 1)));
+        t.c = *reinterpret_cast<const float4*>(row);
+        t.s = *reinterpret_cast<const float4*>(row + (p.rot >> 1));
     }
     return t;
 }
@@ -217,10 +217,10 @@ __device__ __forceinline__ void forward_rows(const Params& p, const Tensor& t, i
         int slot = 0, told = LINE;                         // the first row's slot in the cache; positions that a count covers
         long long first = 0;
         if (PAGED && at.rows > 0) {
-            slot = __ldg(p.lengths + at.b) + at.n;
+            slot = p.lengths[at.b] + at.n;
             first = p.positions ? static_cast<long long>(static_cast<const int*>(p.positions)[at.b]) + at.n : slot;
             if (p.counts) {
-                told = __ldg(p.counts + at.b) - at.n;
+                told = p.counts[at.b] - at.n;
                 if (to_cache) at.rows = ONE ? max(0, min(at.rows, told)) : told > 0 ? at.rows : 0;       // what is not stored is not read
             }
         }

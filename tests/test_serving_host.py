@@ -334,3 +334,13 @@ def test_no_copy_warp_misses_a_phase_of_the_ring(stages, busy):
         for last in range(3):
             assert ring_ends(arrivals, busy, fills, stages, last), (fills, last)
     assert not all(ring_ends(1, (1, 0, 0), fills, stages, 1) for fills in range(1, 8 * stages))
+
+
+def test_kernels_set_up_early_use_no_read_only_loads():
+    """The serving kernels start while the kernel before them, which may write their inputs, still runs: loads that want
+    memory constant for the kernel's whole life are not theirs to use."""
+    sources = list((REPO / "att3ntion_b200" / "csrc").glob("serve_*.cu*"))
+    assert len(sources) >= 5
+    for path in sources:
+        code = re.sub(r"//.*", "", path.read_text())
+        assert not re.search(r"__ldg|ld\.global\.nc|__restrict__", code), path.name
