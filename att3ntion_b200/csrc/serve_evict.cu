@@ -85,26 +85,29 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
     int* kept = p.kept + static_cast<long long>(blockIdx.x) * p.keep;
     const int left = min(n, p.keep);
     if (h == 0 && tid == 0) p.new_lengths[b] = left;
-    for (int r = left + tid; r < p.keep; r += SEL_THREADS) kept[r] = -1;
+    // Counts go up to 2^31 - 1, a step beyond them would be negative: loops over ranks and slots count unsigned.
+    const unsigned keep = p.keep;
+    for (unsigned r = left + tid; r < keep; r += SEL_THREADS) kept[r] = -1;
     if (n <= p.keep) {
-        for (int r = tid; r < n; r += SEL_THREADS) kept[r] = r;
+        for (unsigned r = tid; r < static_cast<unsigned>(n); r += SEL_THREADS) kept[r] = r;
         return;
     }
     // here sinks + recent <= keep < n: the held ends do not meet
-    const int first = p.sinks, M = n - p.sinks - p.recent, want = p.keep - p.sinks - p.recent;
-    for (int r = tid; r < p.sinks; r += SEL_THREADS) kept[r] = r;
-    for (int r = tid; r < p.recent; r += SEL_THREADS) kept[p.keep - p.recent + r] = n - p.recent + r;
+    const int first = p.sinks, want = p.keep - p.sinks - p.recent;
+    const unsigned M = n - p.sinks - p.recent, recent = p.recent;
+    for (unsigned r = tid; r < static_cast<unsigned>(p.sinks); r += SEL_THREADS) kept[r] = r;
+    for (unsigned r = tid; r < recent; r += SEL_THREADS) kept[keep - recent + r] = n - recent + r;
     if (want == 0) return;
 
-    auto fetch = [&](int i) -> uint32_t {
+    auto fetch = [&](unsigned i) -> uint32_t {
         const int row = p.src.row(b, first + i);
         if (row < 0) { serve::report(p.status, serve::ST_PAGE); return 0u; }
         return order_key(p.mass[static_cast<long long>(row) * p.Hkv + h]);
     };
-    auto key_of = [&](int i) -> uint32_t { return p.cached ? keys[i] : fetch(i); };
+    auto key_of = [&](unsigned i) -> uint32_t { return p.cached ? keys[i] : fetch(i); };
     if (p.cached) {
 #pragma unroll 4
-        for (int i = tid; i < M; i += SEL_THREADS) keys[i] = fetch(i);
+        for (unsigned i = tid; i < M; i += SEL_THREADS) keys[i] = fetch(i);
     }
 
     // `prefix`: the leading bits of the want-th largest key; `more`: how many of the keys that share them still count
@@ -115,7 +118,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
         for (int i = tid; i < BINS; i += SEL_THREADS) hist[i] = 0;
         __syncthreads();
-        for (int i = tid; i < M; i += SEL_THREADS) {
+        for (unsigned i = tid; i < M; i += SEL_THREADS) {
             const uint32_t k = key_of(i);
             if ((k & done) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1u)], 1);
         }
@@ -136,9 +139,9 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
         more = chosen[1];
     }
     // keys above `prefix` stay, and the first `more` that equal it.  Each thread ranks a run of neighbouring slots.
-    const int run = (M + SEL_THREADS - 1) / SEL_THREADS, lo = min(tid * run, M), hi = min(lo + run, M);
+    const unsigned run = (M + SEL_THREADS - 1) / SEL_THREADS, lo = min(tid * run, M), hi = min(lo + run, M);
     int above = 0, equal = 0;
-    for (int i = lo; i < hi; ++i) {
+    for (unsigned i = lo; i < hi; ++i) {
         const uint32_t k = key_of(i);
         above += k > prefix;
         equal += k == prefix;
@@ -146,7 +149,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
     Pair total;
     const Pair before = block_scan(above, equal, warp_sums, &total);
     int ahead = before.a, same = before.b;
-    for (int i = lo; i < hi; ++i) {
+    for (unsigned i = lo; i < hi; ++i) {
         const uint32_t k = key_of(i);
         if (k > prefix || (k == prefix && same < more)) kept[p.sinks + ahead + min(same, more)] = first + i;
         ahead += k > prefix;
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
     serve::wait_for_previous_kernel();
     const int h = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
     const int n = p.src.length(p.lengths, b, p.status, false);
-    const int left = min(n, p.keep);
+    const unsigned left = min(n, p.keep);                              // unsigned: a chunk's end may pass 2^31
     const int* kept = p.kept + static_cast<long long>(blockIdx.x) * p.keep;
     const bool is_mass = static_cast<int>(blockIdx.y) == 4 * p.slices;
     const int width = is_mass ? 2 : p.row16 / p.slices;                // threads a row (two share a mass: the first moves it)
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
     const bool idle = is_mass && threadIdx.x % width != 0;
     uint4* pool = is_mass ? nullptr : p.pool[blockIdx.y / p.slices];
     // places of a chunk's rows: source row, target row; the source is -1 where nothing moves
-    auto look = [&](int base, int buf) {
+    auto look = [&](unsigned base, int buf) {
         for (int i = threadIdx.x; i < chunk && base + i < left; i += MOVE_THREADS) {
             int s = p.src.row(b, kept[base + i]);
             const int d = p.dst.row(b, base + i);
@@ -182,7 +185,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
     look(0, 0);
     __syncthreads();
     int buf = 0;
-    for (int base = 0; base < left; base += chunk, buf ^= 1) {
+    for (unsigned base = 0; base < left; base += chunk, buf ^= 1) {
         uint4 v[MOVE_UNROLL];
 #pragma unroll
         for (int u = 0; u < MOVE_UNROLL; ++u) {

@@ -804,3 +804,19 @@ def test_decode_whole_boxes_many_times_round_the_ring(page, D):
     ck.device_status()
     Y64, A, _ = ref.decode(Q[1:2], c.pools, c.table[1:2], lengths[1:2])
     close(first[1:2], Y64, (1 + HALF) * HALF * (Y64.abs() + A) + 2e-4 * A, "Y")
+
+
+def test_evict_that_keeps_everything():
+    """keep = 2^31 - 1, "all of them": the places behind the last slot are -1 up to the end."""
+    from att3ntion_b200 import _cuda_kernels as ck, gather_cache_evict
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 12 GB")
+    c = Made(32, [100], 1, 16, 16)
+    pools, table, n = c.gpu()
+    kept, left = gather_cache_evict(pools, c.mass.cuda(), table, n, 2 ** 31 - 1, sinks=1, recent=2)
+    ck.device_status()
+    assert kept.shape == (1, 1, 2 ** 31 - 1) and left.tolist() == [100]
+    assert kept[0, 0, :100].tolist() == list(range(100))
+    assert all(bool((kept[0, 0, a: a + (1 << 28)] == -1).all()) for a in range(100, 2 ** 31 - 1, 1 << 28))
+    for p, old in zip(pools, c.pools):
+        assert torch.equal(p.cpu(), old)
