@@ -12,8 +12,9 @@
 // next chunk's places are looked up (kept slot, page, row: three dependent loads), one thread a row.
 //
 // The move is bound by memory traffic (16 D + 4 bytes read and written per kept token and key head): 32 sequences of
-// 8000 slots down to 4000, 4 key heads of 128: 193 us, 5.5 TB/s of rows of 256 bytes, 0.84 of a plain copy's rate; the
-// selection before it 22 us.  Two sequences of 700 down to 333 take 9 and 4 us, bound by the latency of the passes.
+// 8000 slots down to 4000, 4 key heads of 128: 183 us, 5.8 TB/s of rows of 256 bytes, 0.88 of a plain copy's rate; the
+// selection before it 22 us.  (A row's address as one 64-bit product from the block's own pointer: formed from row, head
+// and piece each time, the same loop took 225.)  Two sequences of 700 down to 333 take 9 and 4 us, bound by the latency of the passes.
 #include <algorithm>
 
 #include "att3_abi_internal.h"
@@ -171,7 +172,9 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
     const int at = is_mass ? 0 : (blockIdx.y % p.slices) * width + threadIdx.x % width;
     const int rows = MOVE_THREADS / width, mine = threadIdx.x / width, chunk = rows * MOVE_UNROLL;
     const bool idle = is_mass && threadIdx.x % width != 0;
-    uint4* pool = is_mass ? nullptr : p.pool[blockIdx.y / p.slices];
+    uint4* pool = is_mass ? nullptr : p.pool[blockIdx.y / p.slices] + static_cast<long long>(h) * p.row16 + at;
+    const unsigned pitch = static_cast<unsigned>(p.Hkv) * p.row16;
+    float* mass = p.mass + h;
     // places of a chunk's rows: source row, target row; the source is -1 where nothing moves
     auto look = [&](unsigned base, int buf) {
         for (int i = threadIdx.x; i < chunk && base + i < left; i += MOVE_THREADS) {
@@ -193,9 +196,8 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
             if (idle || base + i >= left) continue;
             const int s = from[buf][i];
             if (s < 0) continue;
-            const long long row = static_cast<long long>(s) * p.Hkv + h;
-            if (is_mass) v[u].x = __float_as_uint(p.mass[row]);
-            else v[u] = pool[row * p.row16 + at];
+            if (is_mass) v[u].x = __float_as_uint(mass[static_cast<long long>(s) * p.Hkv]);
+            else v[u] = pool[static_cast<unsigned long long>(static_cast<unsigned>(s)) * pitch];
         }
         look(base + chunk, buf ^ 1);
         __syncthreads();
@@ -203,9 +205,8 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
         for (int u = 0; u < MOVE_UNROLL; ++u) {
             const int i = u * rows + mine;
             if (idle || base + i >= left || from[buf][i] < 0) continue;
-            const long long row = static_cast<long long>(to[buf][i]) * p.Hkv + h;
-            if (is_mass) p.mass[row] = __uint_as_float(v[u].x);
-            else pool[row * p.row16 + at] = v[u];
+            if (is_mass) mass[static_cast<long long>(to[buf][i]) * p.Hkv] = __uint_as_float(v[u].x);
+            else pool[static_cast<unsigned long long>(static_cast<unsigned>(to[buf][i])) * pitch] = v[u];
         }
         __syncthreads();                                               // the buffer is looked up into again
     }
