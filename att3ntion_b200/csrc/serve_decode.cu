@@ -49,7 +49,7 @@ int check(const char* who, int B, int Hq, int Hkv, int D, int window, int sinks)
         return att3::set_error(ATT3_ERR_INVALID, "%s: Hq=%d is not divisible by Hkv=%d", who, Hq, Hkv);
     if (D != 64 && D != 128) return att3::set_error(ATT3_ERR_INVALID, "%s: D must be 64 or 128, got %d", who, D);
     if (window < 0 || sinks < 0) return att3::set_error(ATT3_ERR_INVALID, "%s: window and sinks must not be negative", who);
-    if (static_cast<long long>(B) * Hq > (1 << 24) || static_cast<long long>(window) + sinks > (1 << 30))
+    if (static_cast<long long>(B) * Hq >= (1 << 24) || static_cast<long long>(window) + sinks > (1 << 30))
         return att3::set_error(ATT3_ERR_INVALID, "%s: too many heads, or too wide a window", who);
     return ATT3_OK;
 }

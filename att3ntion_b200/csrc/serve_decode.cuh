@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
         const uint32_t tiles_at = smem_u32(tile_hi);
         auto fetch = [&](const __nv_bfloat16* pool, const Walk<MASS>& at, uint32_t tile, int from_row) {
             const char* src = reinterpret_cast<const char*>(pool + static_cast<size_t>(at.head) * D + chunk * 8);
-            const uint32_t pitch = p.Hkv * D * 2;
+            const uint32_t pitch = static_cast<uint32_t>(p.Hkv) * D * 2;
             // rows of a batch first, then its copies: a shuffle's result is not waited for before every copy.  A row behind
             // the last key repeats row 0's place of the lane's shuffle; the build and the collapse leave it out.
             constexpr int BATCH = 8;

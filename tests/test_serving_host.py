@@ -344,3 +344,10 @@ def test_kernels_set_up_early_use_no_read_only_loads():
     for path in sources:
         code = re.sub(r"//.*", "", path.read_text())
         assert not re.search(r"__ldg|ld\.global\.nc|__restrict__", code), path.name
+
+
+def test_decode_refuses_heads_whose_rows_pass_32_bits():
+    """2^24 key heads of 128 make a slot of 2^32 bytes, which the copies' 32-bit pitch cannot hold."""
+    assert lib.att3_sg_decode_workspace_bytes(1, 1 << 24, 1 << 24, 128, 0, 0, 16, 0) == 0
+    assert "too many heads" in _cabi.last_error()
+    assert lib.att3_sg_decode_workspace_bytes(1, (1 << 24) - 1, (1 << 24) - 1, 128, 0, 0, 16, 0) > 0
