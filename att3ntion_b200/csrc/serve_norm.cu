@@ -346,7 +346,7 @@ __device__ __forceinline__ void backward_rows(const Params& p, const Tensor& t, 
                     for (int k = 0; k < 8; ++k) wg[k] = g[k];
                     scale8(wg, w);
                     const float ss = row_sum<LANES>(dot8(v, v)), m = row_sum<LANES>(dot8(v, wg));
-                    const float q = rsqrtf(ss * (1.f / D) + eps);
+                    const float q = here ? rsqrtf(ss * (1.f / D) + eps) : 0.f;          // with eps = 0 infinite: no row, no share of dw
                     const uint64_t qq = sm100::pair_f32(q, q);
                     const float f1 = -q * q * (m * q) * (1.f / D);
                     const uint64_t ff = sm100::pair_f32(f1, f1);

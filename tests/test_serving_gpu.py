@@ -820,3 +820,26 @@ def test_evict_that_keeps_everything():
     assert all(bool((kept[0, 0, a: a + (1 << 28)] == -1).all()) for a in range(100, 2 ** 31 - 1, 1 << 28))
     for p, old in zip(pools, c.pools):
         assert torch.equal(p.cpu(), old)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-60])
+@pytest.mark.parametrize("N,heads,D,dtype", [(5, (3, 1), 64, torch.float32), (17, (1,), 128, torch.bfloat16), (1, (5, 8), 16, torch.float16)])
+def test_norm_rotate_gradients_without_eps(N, heads, D, dtype, eps):
+    """eps = 0, or one that is 0 in FP32, on rows that are nowhere zero; numbers of rows that leave groups of rows part empty."""
+    from att3ntion_b200 import norm_rotate
+    g = torch.Generator().manual_seed(N)
+    xs = [rand(g, 2, N, h, D, dtype=dtype).double().sign().to(dtype) * (1 + torch.rand(2, N, h, D, generator=g)).to(dtype) for h in heads]
+    ws = [1 + 0.3 * torch.randn(D, generator=g) for _ in heads]
+    leaves, scales = [x.cuda().requires_grad_() for x in xs], [w.cuda().requires_grad_() for w in ws]
+    dys = [rand(g, 2, N, h, D) for h in heads]
+    ys = norm_rotate(leaves, scales, eps=eps)
+    torch.autograd.backward(ys, [d.cuda() for d in dys])
+    half = torch.finfo(dtype).eps / 2
+    for x, w, dy, y, leaf, scale in zip(xs, ws, dys, ys, leaves, scales):
+        x64, w64 = x.double().requires_grad_(), w.double().requires_grad_()
+        y64 = ref.norm_rotate(x64, w64, None, None, 0.0, False)
+        close(y, y64.detach(), HALF * y64.detach().abs() + 2e-6 * y64.detach().abs().amax(-1, keepdim=True), "y")
+        y64.backward(dy.double())
+        close(leaf.grad, x64.grad, half * x64.grad.abs() + 4e-6 * x64.grad.abs().amax(-1, keepdim=True) + 1e-6, "dx")
+        u = (x64 * x64.pow(2).mean(-1, keepdim=True).rsqrt()).detach()
+        close(scale.grad, w64.grad, 3e-6 * (dy.double().abs().amax(-1, keepdim=True) * u.abs()).sum((0, 1, 2)) + 1e-7, "dw")
