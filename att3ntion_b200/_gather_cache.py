@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _serve_native as _native
-from ._norm_rotate import _accepted, _check_eps, _check_heads, _check_scale, _check_table, _on_gpu
+from ._norm_rotate import _accepted, _check_eps, _check_heads, _check_scale, _check_table, _no_tangent, _on_gpu
 
 _BF16 = torch.bfloat16
 _POOLS = ("R", "S", "Vr", "Vs")
@@ -68,6 +68,7 @@ def _check_mass(who, mass, pool):
 def _no_grad(who, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{who}: has no gradient; call it under torch.no_grad()")
+    _no_tangent(who, *tensors)
 
 
 def gather_cache_append(pools, page_table, lengths, R, S, Vr, Vs, *, counts=None, Q=None, weights=None, table=None,
@@ -103,7 +104,7 @@ def _refuse_append(pools, page_table, lengths, new, counts, weights, table, posi
     _check_mass(who, mass, pool)
     if len(weights) != 3:
         raise RuntimeError(f"{who}: weights are three scales, of Q, R and S")
-    _no_grad(who, *new, *weights)
+    _no_grad(who, *new, *weights, *pools, table, mass)
     for k, w in enumerate(weights):
         _check_scale(w, who, f"weight {k}", D, dev)
     _check_table(who, table, D, dev)
@@ -151,7 +152,7 @@ def _refuse_decode(Q, pools, page_table, lengths, window, sinks, mass):
     if sinks and not window:
         raise RuntimeError(f"{who}: sinks go with a window")
     _check_mass(who, mass, pool)
-    _no_grad(who, Q, *pools)
+    _no_grad(who, Q, *pools, mass)
     _on_gpu(who, Q)
     raise RuntimeError(f"{who}: arguments of a type or size that the kernels do not take")
 
@@ -180,6 +181,7 @@ def _refuse_evict(pools, mass, page_table, lengths, keep, sinks, recent, out_tab
         raise RuntimeError(f"{who}: needs the mass that it goes by")
     _check_mass(who, mass, pool)
     _check_table_of_pages(who, page_table, lengths, pool.device)
+    _no_grad(who, *pools, mass)
     B = page_table.shape[0]
     if int(keep) < 1 or int(sinks) < 0 or int(recent) < 0 or int(sinks) + int(recent) > int(keep):
         raise RuntimeError(f"{who}: sinks + recent must fit in keep >= 1, got {sinks} + {recent} in {keep}")

@@ -8,6 +8,7 @@ its heads nor takes positions: att3ntion/_autograd.py:327-329 refuses them.)
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi  # noqa: F401  (the library that the binding is linked against; says what to do if it is missing)
 from . import _serve_native as _native
@@ -93,6 +94,11 @@ def _check_eps(who: str, eps):
         raise RuntimeError(f"{who}: eps must not be negative, got {eps}")
 
 
+def _no_tangent(who: str, *tensors) -> None:
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{who}: has no forward-mode derivative, and an argument carries a tangent")
+
+
 def _on_gpu(who: str, t: torch.Tensor) -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{who}: inputs must be CUDA tensors")
@@ -113,6 +119,9 @@ def _refuse_norm_rotate(xs, ws, table, positions, eps):
     if positions is None and table is not None and N > table.shape[0]:
         raise RuntimeError(f"{who}: {N} positions and a table of {table.shape[0]}")
     _check_eps(who, eps)
+    _no_tangent(who, *xs, *ws, table)
+    if table is not None and table.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{who}: the table has no gradient; detach it")
     _on_gpu(who, xs[0])
     raise RuntimeError(f"{who}: arguments of a type or size that the kernels do not take")
 
@@ -128,7 +137,8 @@ def norm_rotate(xs, weights=None, table=None, positions=None, *, eps=1e-6, inter
     position 0 and reported by `device_status()`.
 
     Returns BF16 tensors, [B,N,heads,D] contiguous, or [B,heads,N,D] with heads_first=True.  Gradients of the inputs come
-    back in their type, those of the scales are summed in FP32 in a fixed order; cotangents are taken as BF16."""
+    back in their type, those of the scales are summed in FP32 in a fixed order; cotangents are taken as BF16.  The table has no
+    gradient, and there is no forward-mode derivative: arguments that ask for either are refused."""
     single = isinstance(xs, torch.Tensor)
     xs = (xs,) if single else tuple(xs)
     if weights is None:

@@ -75,6 +75,17 @@ bool are_heads(const Tensors& xs) {
     return type_of(xs[0]) >= 0 && (D == 16 || D == 32 || D == 64 || D == 128) && small(xs[0].size(0)) && small(xs[0].size(1));
 }
 
+// Whether autograd would miss something: a gradient that the call has none of, or a tangent of forward differentiation
+// (which follows tensors that require no gradient, under no_grad too).
+bool carries(const Tensor& t, bool gradient) { return t.defined() && ((gradient && t.requires_grad()) || t._fw_grad(0).defined()); }
+bool carries(const MaybeTensor& t, bool gradient) { return t && carries(*t, gradient); }
+template <typename List>
+bool any_carries(const List& list, bool gradient) {
+    for (const auto& t : list)
+        if (carries(t, gradient)) return true;
+    return false;
+}
+
 // ------------------------------------------------------------------ norms with rotation
 
 struct Positions {
@@ -252,6 +263,7 @@ py::object norm_rotate(const Tensors& xs, const std::vector<MaybeTensor>& weight
     const at::Device dev = xs[0].device();
     if (table && !is_table(*table, D, dev)) return py::none();
     if (!are_positions(positions, B, N, dev) || (table && !positions && N > table->size(0))) return py::none();
+    if (any_carries(xs, false) || any_carries(weights, false) || carries(table, at::GradMode::is_enabled())) return py::none();
     Tensors tensors(xs), ws;
     int64_t scaled = 0;
     bool graph = false;
@@ -323,13 +335,11 @@ py::object append(const Tensors& pools, const Tensor& page_table, const Tensor& 
     if (!is_page_table(page_table, dev) || page_table.size(0) != B || !are_ints(lengths, B, dev)) return py::none();
     if ((counts && !are_ints(*counts, B, dev)) || (positions && !are_ints(*positions, B, dev)) || !is_mass(mass, pool)) return py::none();
     if (table && !is_table(*table, D, dev)) return py::none();
-    bool graph = false;
-    for (const Tensor& x : xs) graph = graph || x.requires_grad();
-    for (const MaybeTensor& w : weights) {
+    for (const MaybeTensor& w : weights)
         if (w && !is_scale(*w, D, dev)) return py::none();
-        graph = graph || (w && w->requires_grad());
-    }
-    if (graph && at::GradMode::is_enabled()) return py::none();
+    const bool graph = at::GradMode::is_enabled();
+    if (any_carries(xs, graph) || any_carries(weights, graph) || any_carries(pools, graph) || carries(table, graph) || carries(mass, graph))
+        return py::none();
     const c10::cuda::CUDAGuard guard(dev);
     const auto stream = at::cuda::getCurrentCUDAStream();
     att3_head_rows rows[5] = {};
@@ -378,9 +388,8 @@ py::object decode(const Tensor& Q, const Tensors& pools, const Tensor& page_tabl
     if ((D != 64 && D != 128) || D != pool.size(3) || Hq < 1 || Hq % Hkv != 0 || Q.device() != dev || !small(B) || !small(Hq)) return py::none();
     if (!is_page_table(page_table, dev) || page_table.size(0) != B || !are_ints(lengths, B, dev)) return py::none();
     if (window < 0 || sinks < 0 || (sinks > 0 && window == 0) || !is_mass(mass, pool)) return py::none();
-    if (at::GradMode::is_enabled() && (Q.requires_grad() || pools[0].requires_grad() || pools[1].requires_grad() || pools[2].requires_grad() ||
-                                       pools[3].requires_grad()))
-        return py::none();
+    const bool graph = at::GradMode::is_enabled();
+    if (carries(Q, graph) || any_carries(pools, graph) || carries(mass, graph)) return py::none();
     const int64_t slots = page_table.size(1) * pool.size(1);
     if (!small(slots)) return py::none();
     window = std::min(window, slots);
@@ -411,6 +420,8 @@ py::object evict(const Tensors& pools, const MaybeTensor& mass, const Tensor& pa
     const int64_t Hkv = pool.size(2), D = pool.size(3);
     if (D != 16 && D != 32 && D != 64 && D != 128) return py::none();
     if (!is_page_table(page_table, dev) || !small(page_table.size(0)) || !are_ints(lengths, page_table.size(0), dev)) return py::none();
+    const bool graph = at::GradMode::is_enabled();
+    if (any_carries(pools, graph) || carries(mass, graph)) return py::none();
     if (keep < 1 || !small(keep) || sinks < 0 || recent < 0 || sinks > keep || recent > keep || sinks + recent > keep) return py::none();
     const int64_t B = page_table.size(0), slots = page_table.size(1) * pool.size(1);
     if (out_table && (!is_page_table(*out_table, dev) || out_table->size(0) != B || out_table->size(1) * pool.size(1) < std::min(keep, slots)))

@@ -843,3 +843,35 @@ def test_norm_rotate_gradients_without_eps(N, heads, D, dtype, eps):
         close(leaf.grad, x64.grad, half * x64.grad.abs() + 4e-6 * x64.grad.abs().amax(-1, keepdim=True) + 1e-6, "dx")
         u = (x64 * x64.pow(2).mean(-1, keepdim=True).rsqrt()).detach()
         close(scale.grad, w64.grad, 3e-6 * (dy.double().abs().amax(-1, keepdim=True) * u.abs()).sum((0, 1, 2)) + 1e-7, "dw")
+
+
+def test_derivatives_are_refused_on_the_gpu():
+    """Tangents, and arguments without a gradient that want one: none is dropped in silence."""
+    from torch.autograd import forward_ad
+    from att3ntion_b200 import gather_cache_append, gather_cache_evict, norm_rotate, rotary_table, single_gather_decode
+    c = Made(33, [20, 9], 1, 64, 16, room=1)
+    pools, table, n = c.gpu()
+    mass, rot = c.mass.cuda(), rotary_table(64, 64).cuda()
+    new = [torch.randn(2, 1, 1, 64, device="cuda") for _ in range(4)]
+    Q = torch.randn(2, 4, 64, device="cuda")
+    dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+    calls = [lambda d: norm_rotate(d(new[0])), lambda d: norm_rotate(new[0], d(rot[0])), lambda d: norm_rotate(new[0], None, d(rot)),
+             lambda d: gather_cache_append(pools, table, n, *new[:3], d(new[3])), lambda d: gather_cache_append(pools, table, n, *new, mass=d(mass)),
+             lambda d: gather_cache_append([d(pools[0]), *pools[1:]], table, n, *new), lambda d: gather_cache_append(pools, table, n, *new, table=d(rot)),
+             lambda d: single_gather_decode(d(Q), pools, table, n), lambda d: single_gather_decode(Q, [*pools[:3], d(pools[3])], table, n),
+             lambda d: single_gather_decode(Q, pools, table, n, mass=d(mass)), lambda d: gather_cache_evict(pools, d(mass), table, n, 4)]
+    before = [p.clone() for p in (*pools, mass)]
+    for k, call in enumerate(calls):
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), forward_ad.dual_level(), pytest.raises(RuntimeError, match="tangent"):
+                call(dual)
+        if k > 1:
+            with pytest.raises(RuntimeError, match="gradient"):
+                call(lambda t: t.detach().requires_grad_())
+    for call in (lambda: torch.func.jvp(norm_rotate, (new[0],), (new[1],)), lambda: torch.func.vmap(norm_rotate)(torch.stack(new))):
+        with pytest.raises(RuntimeError):
+            call()
+    leaf = new[0].clone().requires_grad_()
+    with forward_ad.dual_level(), pytest.raises(RuntimeError):
+        norm_rotate(dual(leaf))
+    assert all(torch.equal(a, b) for a, b in zip(before, (*pools, mass)))

@@ -351,3 +351,44 @@ def test_decode_refuses_heads_whose_rows_pass_32_bits():
     assert lib.att3_sg_decode_workspace_bytes(1, 1 << 24, 1 << 24, 128, 0, 0, 16, 0) == 0
     assert "too many heads" in _cabi.last_error()
     assert lib.att3_sg_decode_workspace_bytes(1, (1 << 24) - 1, (1 << 24) - 1, 128, 0, 0, 16, 0) > 0
+
+
+# --------------------------------------------------------------------------- what autograd would miss
+
+def dual(t):
+    return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+
+@pytest.mark.parametrize("call", [
+    lambda: norm_rotate(dual(bf(1, 2, 3, 64))),
+    lambda: norm_rotate([bf(1, 2, 3, 64)] * 2, [None, dual(torch.ones(64))]),
+    lambda: norm_rotate(bf(1, 2, 3, 64), None, dual(torch.zeros(8, 64))),
+    lambda: append(new=[bf(2, 1, 2, 64)] * 3 + [dual(bf(2, 1, 2, 64))]),
+    lambda: append(weights=[None, dual(torch.ones(64)), None]),
+    lambda: append(Q=dual(bf(2, 1, 4, 64))),
+    lambda: append(cache=([bf(4, 16, 2, 64)] * 3 + [dual(bf(4, 16, 2, 64))], *cache_args()[1:])),
+    lambda: decode(dual(bf(2, 4, 64))),
+    lambda: decode(cache=([dual(bf(4, 16, 2, 64))] + [bf(4, 16, 2, 64)] * 3, *cache_args()[1:])),
+    lambda: decode(mass=dual(torch.zeros(4, 16, 2))),
+    lambda: evict(mass=dual(torch.zeros(4, 16, 2))),
+    lambda: evict(cache=([bf(4, 16, 2, 64)] * 3 + [dual(bf(4, 16, 2, 64))], *cache_args()[1:])),
+])
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(call, grad):
+    """A dual tensor requires no gradient, and forward differentiation goes on under no_grad."""
+    with torch.set_grad_enabled(grad), torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="tangent"):
+            call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: norm_rotate(bf(1, 2, 3, 64), None, torch.zeros(8, 64, requires_grad=True)),
+    lambda: append(cache=([bf(4, 16, 2, 64).requires_grad_()] + [bf(4, 16, 2, 64)] * 3, *cache_args()[1:])),
+    lambda: append(table=torch.zeros(8, 64, requires_grad=True)),
+    lambda: decode(mass=torch.zeros(4, 16, 2, requires_grad=True)),
+    lambda: evict(mass=torch.zeros(4, 16, 2, requires_grad=True)),
+    lambda: evict(cache=([bf(4, 16, 2, 64).requires_grad_()] + [bf(4, 16, 2, 64)] * 3, *cache_args()[1:])),
+])
+def test_gradients_that_there_are_none_of_are_refused(call):
+    with pytest.raises(RuntimeError, match="gradient"):
+        call()
