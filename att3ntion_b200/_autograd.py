@@ -168,17 +168,39 @@ class HypergraphAttention(nn.Module):
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
                                       error_msgs)
 
+    @torch.compiler.disable
     def _rotary(self, length, device):
         """The angle table, at least `length` positions long, or None.  It grows by doubling, and the shorter ones are kept:
-        a captured graph may still read them."""
+        a captured graph may still read them.  Every later caller gets what this one makes, so it is an ordinary tensor
+        whatever mode the caller is in, and finished when this returns, on whatever stream the next one works.  During a
+        capture it would be filled by the graph's replays only: that one is the graph's own and not kept."""
         if not self.rotary_base:
             return None
         for t in reversed(self._tables):
             if t.device == device and t.shape[0] >= length:
                 return t
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            return rotary_table(length, self.head_dim, self.rotary_base, device)
         most = max((t.shape[0] for t in self._tables if t.device == device), default=256)
-        self._tables.append(rotary_table(max(length, 2 * most), self.head_dim, self.rotary_base, device))
-        return self._tables[-1]
+        with torch.inference_mode(False), torch.no_grad():
+            table = rotary_table(max(length, 2 * most), self.head_dim, self.rotary_base, device)
+        if type(table) is torch.Tensor:                         # and not a stand-in of a tracer
+            if device.type == "cuda":
+                torch.cuda.current_stream(device).synchronize()
+            self._tables.append(table)
+        return table
+
+    def __getstate__(self):
+        return {**self.__dict__, "_tables": []}                 # copies make their own
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        # a layer that was pickled before it had these
+        for name, value in (("sinks", 0), ("rotary_base", None), ("norm_eps", 1e-6), ("_tables", [])):
+            self.__dict__.setdefault(name, value)
+        for name in ("q_norm", "r_norm", "s_norm"):
+            if name not in self._parameters:
+                self.__dict__.setdefault(name, None)
 
     def _qrs(self, x, heads_first):
         """The score operands of every position, [B,N,H,D] or [B,H,N,D]: projected, and normed and rotated in one pass

@@ -875,3 +875,38 @@ def test_derivatives_are_refused_on_the_gpu():
     with forward_ad.dual_level(), pytest.raises(RuntimeError):
         norm_rotate(dual(leaf))
     assert all(torch.equal(a, b) for a, b in zip(before, (*pools, mass)))
+
+
+@pytest.mark.parametrize("first", ["inference mode", "capture", "side stream"])
+def test_angle_table_first_made_elsewhere(first):
+    """A layer whose first call ran in inference mode, was captured, or ran behind other work of a side stream, then trains."""
+    import copy
+    from att3ntion_b200 import HypergraphAttention
+    torch.manual_seed(6)
+    layer = HypergraphAttention(128, 2, gather_mode=1, window=16, rotary_base=1e4, qk_norm=True).cuda()
+    x = torch.randn(2, 48, 128, device="cuda")
+    twin = copy.deepcopy(layer)
+    want = twin(x)
+    want.sum().backward()
+    if first == "inference mode":
+        with torch.inference_mode():
+            assert torch.equal(layer(x), want)
+    elif first == "capture":
+        graph = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.graph(graph):
+            y = layer(x)
+    else:
+        torch.full((1 << 20,), float("nan"), device="cuda")       # what the table's memory may hold before it is filled
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(1 << 28)
+            layer._rotary(48, x.device)
+    got = layer(x)
+    got.sum().backward()
+    assert torch.equal(got, want)
+    for a, b in zip(layer.parameters(), twin.parameters()):
+        assert torch.equal(a.grad, b.grad)
+    if first == "capture":
+        for _ in range(2):
+            graph.replay()
+            assert torch.equal(y, want)

@@ -392,3 +392,32 @@ def test_tangents_are_refused(call, grad):
 def test_gradients_that_there_are_none_of_are_refused(call):
     with pytest.raises(RuntimeError, match="gradient"):
         call()
+
+
+# --------------------------------------------------------------------------- the layer's angle table
+
+def test_angle_table_is_an_ordinary_tensor_whoever_asks_first():
+    import copy
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    cpu = torch.device("cpu")
+    layer = HypergraphAttention(64, 1, gather_mode=1, window=16, rotary_base=1e4)
+    with FakeTensorMode():
+        layer._rotary(8, cpu)
+    assert layer._tables == []
+    with torch.inference_mode():
+        t = layer._rotary(8, cpu)
+    assert not t.is_inference() and layer._rotary(512, cpu) is t
+    (t * torch.ones(1, requires_grad=True)).sum().backward()                      # saved for the backward pass
+    twin = copy.deepcopy(layer)
+    assert twin._tables == [] and layer._tables[0] is t and torch.equal(twin._rotary(8, cpu), t)
+
+
+def test_layers_pickled_before_they_had_norms_and_tables_load():
+    import pickle
+    old = HypergraphAttention(64, 1, gather_mode=1, window=16)
+    for name in ("sinks", "rotary_base", "norm_eps", "_tables", "q_norm", "r_norm", "s_norm"):
+        old.__dict__.pop(name)
+    new = pickle.loads(pickle.dumps(old))
+    assert new.sinks == 0 and not new.rotary_base and new.q_norm is None and new._rotary(4, torch.device("cpu")) is None
+    normed = pickle.loads(pickle.dumps(HypergraphAttention(64, 1, gather_mode=1, window=16, qk_norm=True, rotary_base=10.0)))
+    assert isinstance(normed.q_norm, torch.nn.Parameter) and normed.rotary_base == 10.0 and normed._tables == []
