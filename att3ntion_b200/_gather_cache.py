@@ -211,13 +211,14 @@ class GatherCache:
             raise ValueError(f"GatherCache: head_dim must be 64 or 128, got {head_dim}")
         self.sequences, self.page_size, self.slots = sequences, page_size, slots
         shape = (pages, page_size, n_kv_heads, head_dim)
-        self.pools = [torch.zeros(shape, dtype=_BF16, device=device) for _ in range(4)]
-        self.mass = torch.zeros(shape[:3], dtype=torch.float32, device=device) if track_mass else None
-        self._book = torch.full((sequences, -(-slots // page_size)), -1, dtype=torch.int32)      # the host's page table
-        self.page_table = self._book.to(device)
-        # slots in use and tokens seen (which stay apart once tokens have been evicted), one tensor so that one add moves both
-        self._counters = torch.zeros((2, sequences), dtype=torch.int32, device=device)
-        self.lengths, self.positions = self._counters[0], self._counters[1]
+        with torch.inference_mode(False):           # a cache made in inference mode may be used outside it
+            self.pools = [torch.zeros(shape, dtype=_BF16, device=device) for _ in range(4)]
+            self.mass = torch.zeros(shape[:3], dtype=torch.float32, device=device) if track_mass else None
+            self._book = torch.full((sequences, -(-slots // page_size)), -1, dtype=torch.int32)      # the host's page table
+            self.page_table = self._book.to(device, copy=True)
+            # slots in use and tokens seen (which stay apart once tokens have been evicted), one tensor so that one add moves both
+            self._counters = torch.zeros((2, sequences), dtype=torch.int32, device=device)
+            self.lengths, self.positions = self._counters[0], self._counters[1]
         self.host_lengths, self.host_positions = [0] * sequences, [0] * sequences
         self._free = list(range(pages - 1, -1, -1))
 

@@ -910,3 +910,21 @@ def test_angle_table_first_made_elsewhere(first):
         for _ in range(2):
             graph.replay()
             assert torch.equal(y, want)
+
+
+def test_cache_in_and_out_of_inference_mode():
+    from att3ntion_b200 import GatherCache
+    new = [torch.randn(2, 3, 1, 64, device="cuda") for _ in range(4)]
+    q = torch.randn(2, 4, 64, device="cuda")
+    out = []
+    for made, used in ((True, False), (False, True), (False, False)):
+        with torch.inference_mode(made):
+            c = GatherCache(2, 1, 64, pages=4, slots=32, page_size=16, track_mass=True)
+        with torch.inference_mode(used):
+            c.append(*new)
+            c.append(*new, counts=[1, 0])
+            y = c.decode(q)
+            kept = c.evict(2)
+        assert c.lengths.tolist() == [2, 2] and c.positions.tolist() == [4, 3]
+        out.append((y, kept))
+    assert all(torch.equal(a, b) for o in out[:2] for a, b in zip(o, out[2]))

@@ -421,3 +421,16 @@ def test_layers_pickled_before_they_had_norms_and_tables_load():
     assert new.sinks == 0 and not new.rotary_base and new.q_norm is None and new._rotary(4, torch.device("cpu")) is None
     normed = pickle.loads(pickle.dumps(HypergraphAttention(64, 1, gather_mode=1, window=16, qk_norm=True, rotary_base=10.0)))
     assert isinstance(normed.q_norm, torch.nn.Parameter) and normed.rotary_base == 10.0 and normed._tables == []
+
+
+def test_cache_made_in_inference_mode_is_used_outside_it():
+    with torch.inference_mode():
+        c = GatherCache(2, 1, 64, pages=4, slots=32, page_size=16, track_mass=True, device="cpu")
+    assert not any(t.is_inference() for t in (*c.pools, c.mass, c.page_table, c.lengths, c.positions))
+    c._counters.add_(1)
+    assert c.lengths.tolist() == c.positions.tolist() == [1, 1]
+    c.reserve([17, 0])
+    with torch.inference_mode():
+        c._counters.add_(1)
+        c.clear(0)
+    assert c.lengths.tolist() == [0, 2] and len(c._free) == 4
