@@ -7,9 +7,11 @@
 // during its capture.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/extension.h>
 
 #include <limits>
+#include <unordered_set>
 
 #include "../../include/att3_b200.h"
 
@@ -243,16 +245,29 @@ struct NormRotate : torch::autograd::Function<NormRotate> {
 
 // During a capture autograd runs a leaf's accumulation on the stream that the leaf's accumulator was made on.  One that an
 // eager graph still keeps alive is of a stream outside the capture, and the backward pass would then end the capture, and
-// with it the process; so the forward pass refuses.
-void check_capture(const Tensors& leaves) {
+// with it the process; so the forward pass refuses.  The leaves are the inputs, or lie behind what the capture made of them
+// (views, projections); what was computed before the capture is not gone through, since a captured backward pass has to end
+// there in any case.
+void check_capture(const Tensors& inputs) {
     if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
-    for (const Tensor& t : leaves) {
-        if (!t.requires_grad() || !t.is_leaf()) continue;
-        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
-        if (!accumulator) continue;
-        const auto stream = accumulator->stream();
-        if (stream && *stream != at::cuda::getCurrentCUDAStream(t.device().index()).unwrap())
-            throw std::runtime_error("norm_rotate: an autograd graph of these leaves made outside the capture is still alive; release it first");
+    std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+    std::unordered_set<torch::autograd::Node*> seen;
+    const auto add = [&](std::shared_ptr<torch::autograd::Node> node) {
+        if (node && seen.insert(node.get()).second) todo.push_back(std::move(node));
+    };
+    for (const Tensor& t : inputs)
+        if (t.requires_grad()) add(t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn());
+    const auto here = at::cuda::getCurrentCUDAStream(inputs[0].device().index()).unwrap();
+    while (!todo.empty()) {
+        const std::shared_ptr<torch::autograd::Node> node = std::move(todo.back());
+        todo.pop_back();
+        const auto stream = node->stream();
+        const bool outside = stream && *stream != here;
+        if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
+            if (outside)
+                throw std::runtime_error("norm_rotate: an autograd graph of these leaves made outside the capture is still alive; release it first");
+        } else if (!outside)
+            for (const auto& edge : node->next_edges()) add(edge.function);
     }
 }
 

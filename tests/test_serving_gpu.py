@@ -928,3 +928,49 @@ def test_cache_in_and_out_of_inference_mode():
         assert c.lengths.tolist() == [2, 2] and c.positions.tolist() == [4, 3]
         out.append((y, kept))
     assert all(torch.equal(a, b) for o in out[:2] for a, b in zip(o, out[2]))
+
+
+@pytest.mark.parametrize("through", ["view", "projection", "scale"])
+def test_norm_rotate_captured_on_what_the_capture_makes_of_leaves(through):
+    """The leaves behind a view, a projection or a cast count as the inputs do; inputs computed before the capture do not
+    stand in its way."""
+    from att3ntion_b200 import norm_rotate
+    x = torch.randn(2, 33, 192, device="cuda", requires_grad=True)
+    weight = torch.randn(192, 192, device="cuda", requires_grad=True)
+    w = torch.rand(64, device="cuda", dtype=torch.float64, requires_grad=True)
+    dy = torch.randn(2, 33, 3, 64, device="cuda").bfloat16()
+
+    def forward():
+        if through == "view":
+            return norm_rotate(x.view(2, 33, 3, 64)), [x]
+        if through == "projection":
+            return norm_rotate((x.detach() @ weight).view(2, 33, 3, 64)), [weight]
+        return norm_rotate(x.detach().view(2, 33, 3, 64), w.float()), [w]
+
+    def step():
+        y, leaves = forward()
+        return (y, *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [t.detach().clone() for t in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    alive = forward()
+    other = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside the capture"):
+        with torch.cuda.graph(other):
+            forward()
+    del alive
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del got
+    h = (x @ weight).view(2, 33, 3, 64)                   # its graph stays alive
+    part = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(part):
+        norm_rotate(h)
+    torch.cuda.synchronize()
