@@ -9,7 +9,7 @@ namespace {
 struct Layout {
     size_t part, rows, row_ref, cols, col_ref, lse, unit_base, tile_base, bytes;
     long long units;
-    int ctas, wide, brief;
+    int ctas, wide, brief, col_steps;
 };
 
 // The workspace for the longest sequences that the arguments admit.
@@ -35,7 +35,9 @@ Layout layout(int B, int Hq, int Hkv, int D, int window, int sinks, long long ma
     if (mass) {
         o.rows = take((static_cast<size_t>(tiles) + o.ctas) * 8 * 32 * 4);
         o.row_ref = take((static_cast<size_t>(tiles) + o.ctas) * 8 * 4);
-        const size_t sums = static_cast<size_t>(o.units) * (o.brief ? 8 : 2);
+        // column sums by (head, CTA): no more pairs than heads and CTAs, since both only go up along the line of units
+        o.col_steps = static_cast<int>((seen + 127) / 128);
+        const size_t sums = o.brief ? static_cast<size_t>(o.units) * 8 : (static_cast<size_t>(B) * Hq + o.ctas) * 2 * o.col_steps;
         o.cols = take(sums * 128 * 4);
         o.col_ref = take(sums * 4);
         o.lse = take(static_cast<size_t>(B) * Hq * 4);
@@ -64,7 +66,7 @@ int launch(const serve::DecodeParams& p, const Layout& lay, long long max_seen, 
     e = serve::launch_early(serve::decode_kernel<D, MASS, WIDE>, dim3(lay.ctas), dim3(serve::DEC_THREADS), smem, st, p);
     if (e == cudaSuccess) e = serve::launch_early(serve::decode_join_kernel<D, MASS>, dim3(p.B * p.Hq), dim3(256), 0, st, p, lay.ctas);
     if (MASS && e == cudaSuccess)
-        e = serve::launch_early(serve::decode_mass_kernel, dim3(static_cast<unsigned>((max_seen + 127) / 128), p.B * p.Hkv), dim3(128), 0, st, p, lay.ctas);
+        e = serve::launch_early(serve::decode_mass_kernel, dim3(static_cast<unsigned>((max_seen + 127) / 128), p.B * p.Hkv), dim3(128, std::min(p.G, serve::MASS_PARTS)), 0, st, p, lay.ctas);
     return e == cudaSuccess ? ATT3_OK : att3::set_cuda_error(e, who);
 }
 
@@ -115,6 +117,7 @@ extern "C" int att3_sg_decode(const void* Q, const void* R, const void* S, const
     p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.window = window; p.sinks = sinks;
     p.wide = lay.wide;
     p.brief = lay.brief;
+    p.col_steps = lay.col_steps;
     p.c2 = sgring::LOG2E / std::sqrt(static_cast<float>(D));
     char* ws = static_cast<char*>(workspace);
     p.part = reinterpret_cast<float*>(ws + lay.part);

@@ -77,8 +77,8 @@ struct DecodeParams {
     float* part;                           // [head + CTA][8 warps] records of D + 4 floats: y, m, l
     float* rows;                           // mass: [tile + CTA][8 warps][32] row sums
     float* row_ref;                        // mass: [tile + CTA][8 warps] the maximum they are relative to
-    float* cols;                           // mass: [unit][2 halves][128] column sums, or with `brief` [unit][8 strips][128]
-    float* col_ref;                        // mass: [unit][2] or [unit][8], the maximum they are relative to
+    float* cols;                           // mass: column sums, [head + CTA][2 halves][col_steps][128], or with `brief` [unit][8 strips][128]
+    float* col_ref;                        // mass: the maximum that each 128 of them are relative to
     float* lse;                            // mass: [B,Hq] log2 of the softmax sum
     int* unit_base;                        // [B + 1]; the host admits no more than 2^31 - 1 units
     int* tile_base;                        // [B + 1]
@@ -86,6 +86,7 @@ struct DecodeParams {
     // pools as [pages * page_size, Hkv * D], 64 columns of one row, or of `box` rows of a page (0: not used)
     CUtensorMap tmS, tmVs, tmS_box, tmVs_box;
     int box;
+    int col_steps;                         // key steps of the longest sequence
     int brief;                             // with masses, 1: no sequence shows more than 128 slots
     int wide;                              // 1: no sequence shows more than 192 slots, and a tile has one step of up to 192 keys
 };
@@ -115,7 +116,8 @@ __device__ __forceinline__ Shape shape_of(const DecodeParams& p, int b, bool tel
 }
 
 // A block of query heads: `heads` of them from g0 on (inside the key head), its tiles from tile0 on.  With masses every
-// block is one head, so that a half's column sums are one head's and can be added up; but where a tile has one key step
+// block is one head, so that a half's column sums are one head's and can be added up, over the strips of a tile and over the
+// tiles that a CTA goes through (so they take memory by the slot, not by the pair); but where a tile has one key step
 // at most (`brief`) they are kept strip by strip and heads share tiles as without masses (8 heads a key head, 128 key
 // heads: at window 16, one tile in place of eight, 66 -> 27 us, at window 128 72 -> 55).
 struct Block { int g0, log_heads, tile0; };
@@ -193,9 +195,12 @@ struct Walk {
     int left, unit, slot;                  // units still to do, of the first step, row sums' slot
     Block block;                           // of the tile, and the tile behind it
     int block_end;
+    int first_tile, first_k;               // where the CTA came into the block
     __device__ __forceinline__ void enter(const DecodeParams& p) {
         block = block_of_tile<MASS>(p, s, tile);
         block_end = block.tile0 + block_tiles(1 << block.log_heads, s.groups);
+        first_tile = tile;
+        first_k = 0;
     }
     __device__ __forceinline__ void start(const DecodeParams& p, int b0, int off, int count, int tile_base, int unit0) {
         b = b0;
@@ -210,7 +215,10 @@ struct Walk {
         slot = tile_base + head * s.tiles + tile + blockIdx.x;
         k1 = min(s.steps, k0 + left);
         enter(p);
+        first_k = k0;
     }
+    // whether the CTA has been at key step k of this block before
+    __device__ __forceinline__ bool again(int k) const { return tile > first_tile + (k < first_k ? 1 : 0); }
     // false when the stretch is done
     __device__ __forceinline__ bool next(const DecodeParams& p) {
         left -= k1 - k0;
@@ -624,7 +632,16 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     }
                 } else if (MASS) {
                     // The half's column sums, relative to the largest of its four maxima: warps 2 and 3 hand theirs to
-                    // 0 and 1, then 1 to 0.  (The first warp of a live half has keys, so that maximum is finite.)
+                    // 0 and 1, then 1 to 0.  (The first warp of a live half has keys, so that maximum is finite.)  Warp 0 adds
+                    // them to what the CTA's earlier tiles of the head left, which is on its way meanwhile.
+                    const size_t at = ((static_cast<size_t>(w.b * p.Hq + w.head * p.G + g) + blockIdx.x) * 2 + half) * p.col_steps + k;
+                    const bool more = wq == 0 && w.again(k);
+                    float old[4] = {0.f, 0.f, 0.f, 0.f}, old_ref = -INFINITY;
+                    if (more) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) old[c] = p.cols[at * 128 + c * 32 + lane];
+                        old_ref = p.col_ref[at];
+                    }
                     float* buf = reinterpret_cast<float*>(smem + L::OFF_COL) + half * 256;
                     if (lane == 0) sh_ref[half * 4 + wq] = valid > 0 ? ref : -INFINITY;
                     if (wq >= 2) {
@@ -648,10 +665,10 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                     ok = pipe_wait(&bars[DB_COL0 + half], cols_phase++ & 1, fail, 11);
                     if (!ok) break;
                     if (wq == 0) {
-                        const size_t at = (static_cast<size_t>(w.unit) + (k - w.k0)) * 2 + half;
+                        const float joint = fmaxf(top, old_ref), f = fast_exp2(top - joint), f_old = fast_exp2(old_ref - joint);
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) p.cols[at * 128 + c * 32 + lane] = col[c] + buf[128 + c * 32 + lane];
-                        if (lane == 0) p.col_ref[at] = top;
+                        for (int c = 0; c < 4; ++c) p.cols[at * 128 + c * 32 + lane] = (col[c] + buf[128 + c * 32 + lane]) * f + old[c] * f_old;
+                        if (lane == 0) p.col_ref[at] = joint;          // the arrival below orders it before the warp's next look at it
                     }
                     warp_arrive(&bars[DB_COL0 + half], lane);
                     ok = pipe_wait(&bars[DB_COL0 + half], cols_phase++ & 1, fail, 11);
@@ -953,19 +970,22 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant_
     }
 }
 
-// Adds every visible slot's share of the attention to its mass: a thread a slot, the heads and partials in a fixed order.
-__global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant__ DecodeParams p, int ctas) {
+// Adds every visible slot's share of the attention to its mass: up to four threads a slot, which share the heads; heads and
+// partials in a fixed order.
+constexpr int MASS_PARTS = 4;
+__global__ void __launch_bounds__(128 * MASS_PARTS) decode_mass_kernel(const __grid_constant__ DecodeParams p, int ctas) {
+    __shared__ float sums[MASS_PARTS][128];
     const int b = blockIdx.y / p.Hkv, kv = blockIdx.y % p.Hkv;
     wait_for_previous_kernel();
     const Shape s = shape_of<true>(p, b);
     const int e = blockIdx.x * 128 + threadIdx.x;
+    if (blockIdx.x * 128 >= static_cast<unsigned>(s.seen)) return;
     const int row = e < s.seen ? p.pages.row(b, slot_of(p, s, e)) : -1;
-    if (row < 0) return;
     const int total = p.unit_base[p.B], units0 = p.unit_base[b] + kv * s.tiles * s.steps;
     const int tiles0 = p.tile_base[b] + kv * s.tiles;
     const int step = e / DEC_KEYS, col = e % DEC_KEYS;
     float share = 0.f;
-    for (int g = 0; g < p.G; ++g) {
+    for (int g = threadIdx.y; row >= 0 && g < p.G; g += blockDim.y) {
         const float lse = p.lse[b * p.Hq + kv * p.G + g];
         const Block k = block_of_head<true>(p, s, g);
         auto strip_of = [&](int group) { return (group << k.log_heads) + g - k.g0; };
@@ -987,14 +1007,27 @@ __global__ void __launch_bounds__(128) decode_mass_kernel(const __grid_constant_
                 share += p.cols[at * 128 + col] * fast_exp2(p.col_ref[at] - lse);
             }
         } else {
+            // of every CTA that came by this key step, the half tile of its second half if it saw one
+            const int u0 = units0 + k.tile0 * s.steps, u1 = u0 + block_tiles(1, s.groups) * s.steps;
+            const int first = cta_of(u0, total, ctas), last = cta_of(u1 - 1, total, ctas);
+            // no branches: the loads of several CTAs are under way together
 #pragma unroll 4
-            for (int t = 0; t < block_tiles(1, s.groups); ++t) {
-                const size_t at = (static_cast<size_t>(units0) + (k.tile0 + t) * s.steps + step) * 2;
-                share += p.cols[at * 128 + col] * fast_exp2(p.col_ref[at] - lse);
-                if (t * 256 + 128 < s.seen) share += p.cols[(at + 1) * 128 + col] * fast_exp2(p.col_ref[at + 1] - lse);
+            for (int c = first; c <= last; ++c) {
+                const int from = max(stretch(total, c, ctas), u0) - u0, to = min(stretch(total, c + 1, ctas), u1) - u0;
+                const int t = from / s.steps + (step < from % s.steps ? 1 : 0);        // its first tile with the step
+                const bool one = t * s.steps + step < to, two = one && t * 256 + 128 < s.seen;
+                const size_t at = (static_cast<size_t>(b * p.Hq + kv * p.G + g) + c) * 2 * p.col_steps + step, at2 = at + p.col_steps;
+                const float v1 = one ? p.cols[at * 128 + col] : 0.f, r1 = one ? p.col_ref[at] : -INFINITY;
+                const float v2 = two ? p.cols[at2 * 128 + col] : 0.f, r2 = two ? p.col_ref[at2] : -INFINITY;
+                share += v1 * fast_exp2(r1 - lse);
+                share += v2 * fast_exp2(r2 - lse);
             }
         }
     }
+    sums[threadIdx.y][threadIdx.x] = share;
+    __syncthreads();
+    if (threadIdx.y > 0 || row < 0) return;
+    for (unsigned i = 1; i < blockDim.y; ++i) share += sums[i][threadIdx.x];
     p.mass[static_cast<long long>(row) * p.Hkv + kv] += share / (2.f * p.G);
 }
 

@@ -352,7 +352,9 @@ int att3_gather_cache_evict(void* R, void* S, void* Vr, void* Vs, float* mass, c
  * and the BF16 residual, without rounding.  mass, if given, is FP32 [pages, page_size, Hkv] and gains every visible
  * slot's share of the attention: half the probability of the pairs with it on the R side plus half of those with it
  * on the S side, averaged over the query heads of the key head (1 in all a sequence and key head).  Heads, the
- * table's width and B fix the workspace; the lengths do not. */
+ * table's width and B fix the workspace; the lengths do not: 32 D + 128 bytes for every query head (B Hq) and as much
+ * for every SM; with masses also 12 bytes for every pair of a query head and a visible slot and 8 for every pair of an
+ * SM and a visible slot, max_slots of them without a window. */
 size_t att3_sg_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int window, int sinks, int max_slots, int with_mass);
 int att3_sg_decode(const void* Q, const void* R, const void* S, const void* Vr, const void* Vs, float* mass, void* Y,
                    const att3_gather_pages* pages, const int32_t* lengths, int B, int Hq, int Hkv, int D, int window,

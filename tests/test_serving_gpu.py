@@ -974,3 +974,53 @@ def test_norm_rotate_captured_on_what_the_capture_makes_of_leaves(through):
     with torch.cuda.graph(part):
         norm_rotate(h)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("lengths,Hq,Hkv,D,page,window,sinks", [
+    # many tiles of a head on one CTA, begun and ended inside a tile's keys; last tiles of one half
+    ([2000], 24, 3, 64, 64, 0, 0),
+    ([1924, 300, 129, 257], 16, 2, 128, 16, 0, 0),
+    ([1500, 40, 900, 385], 32, 4, 64, 32, 700, 30),
+    ([700] * 12, 16, 16, 128, 64, 0, 0),
+])
+def test_masses_over_many_tiles(lengths, Hq, Hkv, D, page, window, sinks):
+    from att3ntion_b200 import _cuda_kernels as ck, single_gather_decode
+    c = Made(34, lengths, Hkv, D, page)
+    # scores that grow along the sequence, so that what was added up before has to follow a new maximum
+    for b, n in enumerate(lengths):
+        for p in range(-(-n // page)):
+            c.pools[0][int(c.table[b, p])] *= 0.2 + 2.0 * p * page / n
+    Q = rand(c.g, c.B, Hq, D)
+    Y64, A, share = ref.decode(Q, c.pools, c.table, lengths, window, sinks)
+    pools, table, n = c.gpu()
+    mass = c.mass.cuda()
+    Y = single_gather_decode(Q.cuda(), pools, table, n, window=window, sinks=sinks, mass=mass)
+    ck.device_status()
+    close(Y, Y64, (1 + HALF) * HALF * (Y64.abs() + A) + 4e-4 * A, "Y")
+    want = c.mass.double()
+    for at, v in share.items():
+        want[at] += v
+    # as in test_decode, at scores up to 2.2 times as large
+    close(mass, want, 2.0 ** -24 * want + 5e-5 * (want - c.mass.double()), "mass")
+    again = c.mass.cuda()
+    assert torch.equal(single_gather_decode(Q.cuda(), pools, table, n, window=window, sinks=sinks, mass=again), Y) and torch.equal(again, mass)
+
+
+def test_masses_with_a_wide_table():
+    """Tables for 131072 slots of 16 sequences, most of it empty: the scratch is by the slot and fits."""
+    from att3ntion_b200 import _cuda_kernels as ck, single_gather_decode
+    lengths = [100] * 15 + [700]
+    c = Made(35, lengths, 1, 128, 16)
+    pools, table, n = c.gpu()
+    wide = torch.full((16, 131072 // 16), -1, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    Q = rand(c.g, 16, 8, 128).cuda()
+    out = []
+    for t in (table, wide):
+        mass = c.mass.cuda()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out.append((single_gather_decode(Q, pools, t, n, mass=mass), mass))
+        assert torch.cuda.max_memory_allocated() - before < 1 << 30
+    ck.device_status()
+    assert all(torch.equal(a, b) for a, b in zip(*out))

@@ -434,3 +434,15 @@ def test_cache_made_in_inference_mode_is_used_outside_it():
         c._counters.add_(1)
         c.clear(0)
     assert c.lengths.tolist() == [0, 2] and len(c._free) == 4
+
+
+def test_scratch_for_masses_goes_by_the_slots():
+    """Linear in the page table's width and in the heads: 12 bytes a query head and slot, 8 an SM and slot, and what the call
+    without masses takes."""
+    sms = 148
+    for B, Hq, Hkv, D in ((1, 8, 1, 128), (16, 8, 8, 64), (8, 32, 4, 128)):
+        for slots in (1 << 12, 1 << 15, 1 << 16, 131072, 1 << 20):
+            plain = lib.att3_sg_decode_workspace_bytes(B, Hq, Hkv, D, 0, 0, slots, 0)
+            extra = lib.att3_sg_decode_workspace_bytes(B, Hq, Hkv, D, 0, 0, slots, 1) - plain
+            tail = 256 * (B * Hq + sms) * 16 + 65536            # references, partial tiles, rounding of the parts
+            assert 0 < extra <= 13 * B * Hq * slots + 9 * sms * slots + tail, (B, Hq, slots, extra)
