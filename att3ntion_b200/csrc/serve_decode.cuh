@@ -276,11 +276,14 @@ __device__ __forceinline__ void tma_gather4(void* dst, const void* map, int x, c
 }
 
 // Residual of a packed BF16 product hi = bf16x2(a b): a b - hi has at most 8 significant bits, so the fused
-// multiply-add, which rounds once, gives it exactly.
+// multiply-add, which rounds once, gives it exactly.  Where the product itself is out of range the residual is NaN; the
+// minimum, which prefers a number, makes it the largest that a residual can be, which changes nothing beside the infinite
+// value (a NaN factor is in hi too).
 __device__ __forceinline__ uint32_t residual_bf16x2(uint32_t a, uint32_t b, uint32_t hi) {
     const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b),
                                      __hneg2(*reinterpret_cast<const __nv_bfloat162*>(&hi)));
-    return *reinterpret_cast<const uint32_t*>(&r);
+    const __nv_bfloat162 n = __hmin2(r, __float2bfloat162_rn(0x1p120f));
+    return *reinterpret_cast<const uint32_t*>(&n);
 }
 
 // 16 bytes from global to shared memory, asynchronously; a thread's copies complete in groups.
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(DEC_THREADS, 1) decode_kernel(const __grid_con
                 // far follows.  (The products issued so far are complete: this step's scores came after them.)
                 auto renew = [&](float mx) {
                     mx = lane < valid ? mx * p.c2 : -INFINITY;
-                    if (k == w.k0) ref = warp_max(mx);
+                    if (k == w.k0) ref = fmaxf(warp_max(mx), -3e38f);      // scores that are -inf throughout count nothing, not NaN
                     else if (__any_sync(0xFFFFFFFFu, mx > ref + GROW)) {
                         const float now = warp_max(mx), f = fast_exp2(ref - now);
                         ref = now;

@@ -1006,6 +1006,34 @@ def test_masses_over_many_tiles(lengths, Hq, Hkv, D, page, window, sinks):
     assert torch.equal(single_gather_decode(Q.cuda(), pools, table, n, window=window, sinks=sinks, mass=again), Y) and torch.equal(again, mass)
 
 
+@pytest.mark.parametrize("D,with_mass", [(64, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("where", ["rows", "columns"])
+def test_decode_scores_below_the_range_count_nothing(D, with_mass, where):
+    """Scores that are -inf in FP32 for whole groups of rows, or for the first steps of keys, beside ordinary ones.  All
+    factors are powers of two, so the products are exact."""
+    from att3ntion_b200 import single_gather_decode
+    n, page = 420, 64
+    c = Made(36, [n], 1, D, page)
+    Q = torch.zeros(1, 2, D, dtype=torch.bfloat16)
+    Q[..., 0] = 2.0 ** 40
+    for k in (0, 1):
+        c.pools[k].zero_()
+        c.pools[k][..., 0] = 2.0 ** -20
+    for e in range(288):
+        at = (int(c.table[0, e // page]), e % page)
+        c.pools[0 if where == "rows" else 1][at + (0, 0)] = -2.0 ** 120       # a score of -2^140 / sqrt(D)
+    Y64, A, share = ref.decode(Q, c.pools, c.table, [n])
+    pools, table, length = c.gpu()
+    mass = c.mass.cuda() if with_mass else None
+    Y = single_gather_decode(Q.cuda(), pools, table, length, mass=mass)
+    close(Y, Y64, (1 + HALF) * HALF * (Y64.abs() + A) + 2e-4 * A, "Y")
+    if with_mass:
+        want = c.mass.double()
+        for at, v in share.items():
+            want[at] += v
+        close(mass, want, 2.0 ** -24 * want + 2e-5 * (want - c.mass.double()), "mass")
+
+
 def test_masses_with_a_wide_table():
     """Tables for 131072 slots of 16 sequences, most of it empty: the scratch is by the slot and fits."""
     from att3ntion_b200 import _cuda_kernels as ck, single_gather_decode
