@@ -10,8 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _serve_native as _native
-from ._norm_rotate import _accepted, _check_eps, _check_heads, _check_scale, _check_table, _no_tangent, _on_gpu
+from ._norm_rotate import _accepted, _check_eps, _check_heads, _check_scale, _check_table, _native, _no_tangent, _on_gpu
 
 _BF16 = torch.bfloat16
 _POOLS = ("R", "S", "Vr", "Vs")

@@ -11,7 +11,22 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _cabi  # noqa: F401  (the library that the binding is linked against; says what to do if it is missing)
-from . import _serve_native as _native
+
+try:
+    from . import _serve_native as _native
+except ImportError as _error:
+    class _Missing:
+        """Stands for a binding that is not built, or built against another torch: what needs it says so when it is called,
+        and the operators that go through the C ABI alone are not held up."""
+
+        def __init__(self, why):
+            self._why = why
+
+        def __getattr__(self, name):
+            raise ImportError(f"{name}: the torch binding att3ntion_b200/_serve_native.so cannot be loaded ({self._why}); build it with "
+                              "`python -m att3ntion_b200.build`")
+
+    _native = _Missing(str(_error))
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 _HEAD_DIMS = (16, 32, 64, 128)

@@ -446,3 +446,28 @@ def test_scratch_for_masses_goes_by_the_slots():
             extra = lib.att3_sg_decode_workspace_bytes(B, Hq, Hkv, D, 0, 0, slots, 1) - plain
             tail = 256 * (B * Hq + sms) * 16 + 65536            # references, partial tiles, rounding of the parts
             assert 0 < extra <= 13 * B * Hq * slots + 9 * sms * slots + tail, (B, Hq, slots, extra)
+
+
+def test_training_does_without_the_serving_binding():
+    """Without the torch binding the layers and operators of the C ABI import and construct; what needs it says so."""
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.modules["att3ntion_b200._serve_native"] = None
+import torch, att3ntion
+from att3ntion_b200 import GatherCache, HypergraphAttention, norm_rotate, single_gather_attention
+HypergraphAttention(64, 1)
+cache = GatherCache(1, 1, 64, pages=1, slots=16, page_size=16, track_mass=True, device="cpu")
+x = torch.zeros(1, 1, 1, 64)
+for call in (lambda: norm_rotate(x), lambda: cache.append(x, x, x, x), lambda: cache.decode(x[0]), lambda: cache.evict(1)):
+    try:
+        call()
+    except ImportError as e:
+        assert "att3ntion_b200.build" in str(e), e
+    else:
+        raise SystemExit("no ImportError")
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=REPO)
+    assert r.returncode == 0 and r.stdout.strip() == "fine", r.stderr
