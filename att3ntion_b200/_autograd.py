@@ -309,11 +309,12 @@ class HypergraphAttention(nn.Module):
     @torch.no_grad()
     def prefill(self, x, cache, counts=None):
         """The layer over the prompts x [B,N,d_model] of empty sequences, storing their rows in `cache`.  counts (a list of
-        ints): the prompts' lengths, right-padded to N; what comes back behind a prompt's end means nothing."""
+        ints): the prompts' lengths, right-padded to N; what comes back behind a prompt's end means nothing.  A sequence
+        of count 0 is left as it is, so that one that was cleared can start anew beside the others."""
         self._check_serving("prefill", x, cache)
-        if any(cache.host_lengths):
-            raise ValueError("prefill: the cache's sequences must be empty")
         b, n, _ = x.shape
+        if any(have and new for have, new in zip(cache.host_lengths, cache._counts(counts, n))):
+            raise ValueError("prefill: the sequences of its prompts must be empty")
         # a window of causal keys: the padding behind a prompt is never seen by its own positions
         last = self._reads_in_place(n, None)
         Q, R, S = self._qrs(x, heads_first=not last)
@@ -327,16 +328,17 @@ class HypergraphAttention(nn.Module):
         return self._gather(x, Q, R, S, side(vr), side(vs), mask, last)
 
     @torch.no_grad()
-    def decode(self, x, cache):
+    def decode(self, x, cache, counts=None):
         """The layer over one new token of every sequence, x [B,1,d_model], after storing its rows in `cache`: the last
-        `window` cached tokens and the first `sinks` are visible."""
+        `window` cached tokens and the first `sinks` are visible.  counts (a list of 0 and 1): a sequence of 0 sits out,
+        nothing is stored for it and what comes back for it means nothing."""
         self._check_serving("decode", x, cache)
         if x.shape[1] != 1:
             raise ValueError(f"decode: one token a sequence, got {x.shape[1]}")
         b = x.shape[0]
         split = lambda t: t.view(b, 1, self.n_heads, self.head_dim)
         table = self._rotary(max(cache.host_positions, default=0) + 1, x.device)
-        q = cache.append(split(self.Wr(x)), split(self.Ws(x)), split(self.Wv_r(x)), split(self.Wv_s(x)), Q=split(self.Wq(x)),
+        q = cache.append(split(self.Wr(x)), split(self.Ws(x)), split(self.Wv_r(x)), split(self.Wv_s(x)), counts=counts, Q=split(self.Wq(x)),
                          weights=(self.q_norm, self.r_norm, self.s_norm), table=table, eps=self.norm_eps)
-        y = self.gelu(cache.decode(q[:, 0], window=self.window, sinks=self.sinks).to(x.dtype))
+        y = self.gelu(cache.decode(q[:, 0], window=self.window, sinks=self.sinks, counts=counts).to(x.dtype))
         return self.Wo(y.reshape(b, 1, self.n_heads * self.head_dim))

@@ -196,14 +196,17 @@ def _refuse_evict(pools, mass, page_table, lengths, keep, sinks, recent, out_tab
 
 
 class GatherCache:
-    """A paged gather cache of a batch of sequences that move together: pools, page table and lengths on the device, and
-    the book-keeping of pages on the host.
+    """A paged gather cache of a batch of sequences: pools, page table and lengths on the device, and the book-keeping of
+    pages on the host.  A sequence that is done is left out by a count of 0 (`append`, `decode`), or emptied by `clear` and
+    filled anew.
 
     sequences: rows of the page table.  pages: pages of `page_size` slots in each pool.  slots: the most that a sequence
     may hold.  track_mass: add up every token's share of the attention in `decode`, for `evict`.
 
     Pages are handed out in Python when a call needs them, so these methods are not for capture into a graph: a captured
-    step calls the functions above on tensors of its own (or this cache's), which read lengths and tables as they are."""
+    step calls the functions above on tensors of its own (or this cache's), which read lengths and tables as they are.
+    `reserve` copies the table from pageable memory when a call needs a page, and counts are copied likewise: both wait for
+    the stream."""
 
     def __init__(self, sequences, n_kv_heads, head_dim, *, pages, slots, page_size=64, track_mass=False, device="cuda"):
         if min(sequences, n_kv_heads, pages, slots, page_size) < 1:
@@ -231,6 +234,9 @@ class GatherCache:
             raise ValueError(f"GatherCache: counts must be {self.sequences} numbers of 0 .. {T}")
         return counts
 
+    def _on_device(self, counts):
+        return torch.tensor(counts, dtype=torch.int32, device=self.page_table.device)
+
     def reserve(self, counts):
         """Hands out the pages that `counts[b]` more slots of every sequence need."""
         want = []
@@ -253,8 +259,7 @@ class GatherCache:
         T = R.shape[1]
         host = self._counts(counts, T)
         self.reserve(host)
-        device = self.page_table.device
-        on_device = None if counts is None else torch.tensor(host, dtype=torch.int32, device=device)
+        on_device = None if counts is None else self._on_device(host)
         q = gather_cache_append(self.pools, self.page_table, self.lengths, R, S, Vr, Vs, counts=on_device, Q=Q, weights=weights,
                                 table=table, positions=self.positions, mass=self.mass, eps=eps, interleaved=interleaved)
         self._counters.add_(T if on_device is None else on_device)
@@ -263,9 +268,11 @@ class GatherCache:
             self.host_positions[b] += c
         return q
 
-    def decode(self, Q, *, window=0, sinks=0):
-        """`single_gather_decode` of Q [B,Hq,D] over the cached rows, adding to the masses if they are tracked."""
-        return single_gather_decode(Q, self.pools, self.page_table, self.lengths, window=window, sinks=sinks, mass=self.mass)
+    def decode(self, Q, *, window=0, sinks=0, counts=None):
+        """`single_gather_decode` of Q [B,Hq,D] over the cached rows, adding to the masses if they are tracked.  counts (a
+        list of 0 and 1): a sequence of 0 sits out, gives zeros and keeps its masses."""
+        lengths = self.lengths if counts is None else self.lengths * self._on_device(self._counts(counts, 1))
+        return single_gather_decode(Q, self.pools, self.page_table, lengths, window=window, sinks=sinks, mass=self.mass)
 
     def evict(self, keep, *, sinks=0, recent=0):
         """`gather_cache_evict` in place; the pages behind the kept slots become free.  Returns the slots that stayed,

@@ -1052,3 +1052,44 @@ def test_masses_with_a_wide_table():
         assert torch.cuda.max_memory_allocated() - before < 1 << 30
     ck.device_status()
     assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.parametrize("kw", [dict(window=16, qk_norm=True, rotary_base=1e4), dict(window=48, sinks=3)])
+def test_sequences_that_end_and_start_at_their_own_time(kw):
+    """One sequence ends, is cleared and starts anew while the others go on or sit out: each gives what it gives alone."""
+    from att3ntion_b200 import GatherCache, HypergraphAttention
+    torch.manual_seed(8)
+    layer = HypergraphAttention(128, 2, gather_mode=1, **kw).cuda()
+    x = torch.randn(3, 80, 128, device="cuda")
+    new = torch.randn(1, 80, 128, device="cuda")
+    make = lambda n: GatherCache(n, 2, 64, pages=10 * n, slots=80, page_size=8, track_mass=True)
+    cache, alone = make(3), [make(3) for _ in range(2)]
+
+    def near(a, b):                                     # projections of another batch may be summed in another order
+        assert (a - b).norm() <= 0.01 * b.norm()
+
+    layer.prefill(x[:, :30], cache, counts=[30, 12, 25])
+    for _ in range(3):
+        layer.decode(x[:, 40:41], cache)
+    assert cache.host_lengths == [33, 15, 28]
+    cache.clear(1)
+    layer.decode(x[:, 41:42], cache, counts=[1, 0, 1])
+    assert cache.host_lengths == cache.lengths.tolist() == [34, 0, 29] and cache.host_positions == [34, 0, 29]
+    assert len(cache._free) == 30 - 5 - 4 and cache.page_table[1].tolist() == [-1] * 10
+    y = layer.prefill(torch.cat([x[:1, :20], new[:, :20], x[:1, :20]]), cache, counts=[0, 17, 0])
+    assert cache.host_lengths == [34, 17, 29]
+    before = cache.mass.clone()
+    y2 = layer.decode(torch.cat([x[:1, 42:43], new[:, 17:18], x[2:, 42:43]]), cache, counts=[1, 1, 0])
+    assert cache.host_lengths == cache.lengths.tolist() == [35, 18, 29]
+    pages = cache.page_table[2][:4].long()
+    assert torch.equal(cache.mass[pages], before[pages])           # what sat out gained nothing
+    # the same three sequences, each with a batch of copies of its own
+    for b, (rows, steps) in enumerate((((x[0:1, :30], 30), (40, 40, 40, 41, 42)), ((new[:, :20], 17), (17,)))):
+        c = alone[b]
+        z = layer.prefill(rows[0].expand(3, -1, -1).contiguous(), c, counts=[rows[1]] * 3)
+        if b == 1:
+            near(y[1, :17], z[1, :17])
+        source = x[0:1] if b == 0 else new
+        for s in steps:
+            z = layer.decode(source[:, s: s + 1].expand(3, -1, -1).contiguous(), c)
+        near(y2[b], z[b])

@@ -471,3 +471,19 @@ print("fine")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=REPO)
     assert r.returncode == 0 and r.stdout.strip() == "fine", r.stderr
+
+
+def test_counts_of_sequences_that_sit_out():
+    layer = HypergraphAttention(64, 1, gather_mode=1, window=16)
+    cache = GatherCache(2, 1, 64, pages=4, slots=32, page_size=16, device="cpu")
+    for bad in ([1], [2, 0], [-1, 1]):
+        with pytest.raises(ValueError, match="counts"):
+            cache.decode(bf(2, 1, 64), counts=bad)
+        with pytest.raises(ValueError, match="counts"):
+            layer.decode(torch.zeros(2, 1, 64), cache, counts=bad)
+    cache.host_lengths = [3, 0]
+    for counts in (None, [1, 0], [4, 4]):
+        with pytest.raises(ValueError, match="must be empty"):
+            layer.prefill(torch.zeros(2, 4, 64), cache, counts=counts)
+    with pytest.raises(ValueError, match="counts"):
+        layer.prefill(torch.zeros(2, 4, 64), cache, counts=[0, 5])
