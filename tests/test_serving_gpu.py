@@ -1093,3 +1093,100 @@ def test_sequences_that_end_and_start_at_their_own_time(kw):
         for s in steps:
             z = layer.decode(source[:, s: s + 1].expand(3, -1, -1).contiguous(), c)
         near(y2[b], z[b])
+
+
+@pytest.mark.parametrize("N,head_dim,kw", [
+    (48, 64, dict(gather_mode=1, window=16, qk_norm=True, rotary_base=100.0, sinks=3)),
+    (48, 64, dict(gather_mode=1, window=16, qk_norm=True, rotary_base=100.0)),
+    (45, 128, dict(gather_mode=1, window=20, qk_norm=True, rotary_base=1e4, sinks=1)),
+    (40, 64, dict(gather_mode=1, window=200, rotary_base=1e4, sinks=5)),
+    (33, 128, dict(gather_mode=1, qk_norm=True)),
+    (48, 32, dict(gather_mode=1, window=9, qk_norm=True, rotary_base=100.0, sinks=4)),
+    (32, 64, dict(gather_mode=0, qk_norm=True, rotary_base=100.0)),
+    (27, 16, dict(gather_mode=0, qk_norm=True, rotary_base=100.0)),
+])
+def test_layer_gradients_against_64_bits(N, head_dim, kw):
+    """Every parameter's gradient, and the input's, of the layer with norms, rotation and sinks against a restatement in 64
+    bits whose gather operands are rounded to BF16 as the layer's are.
+
+    Tolerances, in the 2-norm.  A gather's gradient dO of an operand O is held to |error| <= g |dO|, g = 0.06 for Q, R, S and
+    0.04 for the values, the result to 0.03 |Y| (the gates of the operators' own tests).  The result's error moves its
+    cotangent too, by 0.03 |Y| max |dY gelu''| / |dY|, and BF16 rounds it by 2^-8: both are added to g.  From there on all is
+    linear: |error dW| <= g |dO| s |X|_2 with s the largest factor of the norm's backward pass, |w| / rms.  A scale's gradient
+    sums error times u = x / rms over the rows, whose errors are roundings of their own: taken as independent, their sum has
+    the 2-norm sum error^2 u^2, at most (g |dO| max |u|)^2.  The output projection: 0.03 |Y| max |gelu'| |dy|_2
+    + 2^-8 |gelu(Y)| |dy|_2; a projection's bias: g |dO| sqrt(rows)."""
+    from oracle import triplet_oracle as O
+    from att3ntion_b200 import HypergraphAttention, rotary_table, window_mask
+    torch.manual_seed(N + head_dim)
+    B, H = 2, 2
+    layer = HypergraphAttention(H * head_dim, H, **kw).cuda()
+    with torch.no_grad():
+        for p in (layer.q_norm, layer.r_norm, layer.s_norm):
+            if p is not None:
+                p.uniform_(0.5, 1.5)
+    x, dy = torch.randn(B, N, H * head_dim, device="cuda", requires_grad=True), torch.randn(B, N, H * head_dim, device="cuda")
+    layer(x).backward(dy)
+
+    P = {n: p.detach().double().cpu().requires_grad_() for n, p in layer.named_parameters()}
+    X = x.detach().double().cpu().requires_grad_()
+    round_bf16 = lambda t: t + (t.detach().to(torch.bfloat16).double() - t.detach())
+    heads = lambda t: t.view(B, N, H, head_dim).transpose(1, 2)
+    table = rotary_table(N, head_dim, kw["rotary_base"]).double() if kw.get("rotary_base") else None
+    pos = torch.arange(N).expand(B, N)
+    ops, factor, spread = {}, {}, {}
+    for name, w, scale in (("Q", "Wq", "q_norm"), ("R", "Wr", "r_norm"), ("S", "Ws", "s_norm")):
+        raw = (X @ P[w + ".weight"].T).view(B, N, H, head_dim)
+        t = ref.norm_rotate(raw, P.get(scale), table, pos, 1e-6, False)
+        inverse = (raw.pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt().detach() if scale in P else None
+        factor[name] = 1.0 if inverse is None else float(P[scale].abs().max() * inverse.max())
+        spread[name] = None if inverse is None else float((raw.detach() * inverse).abs().max())
+        ops[name] = round_bf16(t.transpose(1, 2))
+    for name, w in (("Vr", "Wv_r"), ("Vs", "Wv_s"), ("Vq", "Wv_q")):
+        if w + ".weight" in P:
+            ops[name], factor[name] = round_bf16(heads(X @ P[w + ".weight"].T + P.get(w + ".bias", 0.0))), 1.0
+    for t in ops.values():
+        t.retain_grad()
+    mask = window_mask(N, kw["window"], "cpu", kw.get("sinks", 0)).expand(B, N, N) if kw.get("window") else None
+    zero = torch.zeros_like(ops["Vr"])
+    out, _ = O.hypergraph_dense(ops["Q"], ops["R"], ops["S"], ops.get("Vq", zero), zero, ops["Vr"], zero, ops["Vs"], zero, mask=mask,
+                                gather_mode=kw["gather_mode"], scatter=False)
+    out = [t for t in out[: 3 if kw["gather_mode"] == 0 else 1]]
+    for t in out:
+        t.retain_grad()
+    acts = [t * torch.sigmoid(1.702 * t) for t in out]
+    y = sum(acts).transpose(1, 2).reshape(B, N, H * head_dim)
+    (y @ P["Wo.weight"].T + P["Wo.bias"]).backward(dy.double().cpu())
+
+    more = 2.0 ** -8
+    for t, a in zip(out, acts):
+        s = torch.sigmoid(1.702 * t.detach())
+        first, second = s + 1.702 * t.detach() * s * (1 - s), 1.702 * s * (1 - s) * (2 + 1.702 * t.detach() * (1 - 2 * s))
+        cotangent = t.grad / first                                     # before the activation
+        more = max(more, 2.0 ** -8 + 0.03 * float(t.detach().norm() * (cotangent * second).abs().max() / t.grad.norm()))
+    assert more < 0.2
+    share = {n: ((0.04 if n[0] == "V" else 0.06) + more) * float(t.grad.norm()) * factor[n] for n, t in ops.items()}
+    flat = X.detach().flatten(0, 1)
+    size = float(torch.linalg.matrix_norm(flat, 2))
+    of = {"Wq": "Q", "Wr": "R", "Ws": "S", "Wv_r": "Vr", "Wv_s": "Vs", "Wv_q": "Vq"}
+    tol = {"Wo.bias": 1e-5 * float(dy.norm()) * N}
+    edge = float(torch.linalg.matrix_norm(dy.double().cpu().flatten(0, 1), 2))
+    tol["Wo.weight"] = edge * sum(0.03 * float(t.detach().norm()) * 1.1 + 2.0 ** -8 * float(a.detach().norm()) for t, a in zip(out, acts))
+    total = 0.0
+    for w, o in of.items():
+        if w + ".weight" in P:
+            tol[w + ".weight"] = share[o] * size
+            if w + ".bias" in P:
+                tol[w + ".bias"] = share[o] * (B * N) ** 0.5
+            total += share[o] * float(torch.linalg.matrix_norm(P[w + ".weight"].detach(), 2))
+    for scale, o in (("q_norm", "Q"), ("r_norm", "R"), ("s_norm", "S")):
+        if scale in P:
+            tol[scale] = share[o] / factor[o] * spread[o]
+    assert set(tol) == set(P)
+    for name, p in layer.named_parameters():
+        off = float((p.grad.double().cpu() - P[name].grad).norm())
+        assert off <= tol[name], (name, off, tol[name], float(P[name].grad.norm()))
+        if not name.endswith("bias"):                              # a tolerance that a wrong gradient would meet says nothing
+            assert tol[name] < 0.9 * float(P[name].grad.norm()), (name, tol[name], float(P[name].grad.norm()))
+    off = float((x.grad.double().cpu() - X.grad).norm())
+    assert off <= total, (off, total)
