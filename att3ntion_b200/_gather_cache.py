@@ -123,8 +123,8 @@ def single_gather_decode(Q, pools, page_table, lengths, *, window=0, sinks=0, ma
 
     mass (FP32 [pages,page_size,Hkv]), if given, gains every visible slot's share of the attention: the mean over the
     key head's query heads of half the probability of the pairs that hold the slot as j plus half of those that hold it
-    as k, 1 in all for every sequence and key head.  No two sequences of a call with masses may share a page.  The call's
-    scratch memory goes by what the page table could hold, not by the lengths: with masses about 12 bytes a query head and
+    as k, 1 in all for every sequence and key head.  A slot that several sequences share gains each one's, in no fixed order.
+    The call's scratch memory goes by what the page table could hold, not by the lengths: with masses about 12 bytes a query head and
     slot (of the window and sinks, if there is a window) and 8 bytes an SM and slot."""
     y = _accepted(_native.decode, Q, pools, page_table, lengths, window, sinks, mass)
     if y is None:

@@ -1031,7 +1031,8 @@ __global__ void __launch_bounds__(128 * MASS_PARTS) decode_mass_kernel(const __g
     __syncthreads();
     if (threadIdx.y > 0 || row < 0) return;
     for (unsigned i = 1; i < blockDim.y; ++i) share += sums[i][threadIdx.x];
-    p.mass[static_cast<long long>(row) * p.Hkv + kv] += share / (2.f * p.G);
+    // atomically: sequences may share the pages of a prefix, and each adds its own share (elsewhere there is one addition)
+    atomicAdd(p.mass + static_cast<long long>(row) * p.Hkv + kv, share / (2.f * p.G));
 }
 
 }  // namespace serve

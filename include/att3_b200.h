@@ -351,7 +351,8 @@ int att3_gather_cache_evict(void* R, void* S, void* Vr, void* Vs, float* mass, c
  * window == 0: all are.  A sequence of length 0 gives zeros.  Scores are formed from Q o R split into its BF16 value
  * and the BF16 residual, without rounding.  mass, if given, is FP32 [pages, page_size, Hkv] and gains every visible
  * slot's share of the attention: half the probability of the pairs with it on the R side plus half of those with it
- * on the S side, averaged over the query heads of the key head (1 in all a sequence and key head).  Heads, the
+ * on the S side, averaged over the query heads of the key head (1 in all a sequence and key head);
+ * a slot that several sequences share gains each one's, in no fixed order.  Heads, the
  * table's width and B fix the workspace; the lengths do not: 32 D + 128 bytes for every query head (B Hq) and as much
  * for every SM; with masses also 12 bytes for every pair of a query head and a visible slot and 8 for every pair of an
  * SM and a visible slot, max_slots of them without a window. */

@@ -1139,7 +1139,7 @@ def test_layer_gradients_against_64_bits(N, head_dim, kw):
         raw = (X @ P[w + ".weight"].T).view(B, N, H, head_dim)
         t = ref.norm_rotate(raw, P.get(scale), table, pos, 1e-6, False)
         inverse = (raw.pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt().detach() if scale in P else None
-        factor[name] = 1.0 if inverse is None else float(P[scale].abs().max() * inverse.max())
+        factor[name] = 1.0 if inverse is None else float(P[scale].detach().abs().max() * inverse.max())
         spread[name] = None if inverse is None else float((raw.detach() * inverse).abs().max())
         ops[name] = round_bf16(t.transpose(1, 2))
     for name, w in (("Vr", "Wv_r"), ("Vs", "Wv_s"), ("Vq", "Wv_q")):
@@ -1190,3 +1190,26 @@ def test_layer_gradients_against_64_bits(N, head_dim, kw):
             assert tol[name] < 0.9 * float(P[name].grad.norm()), (name, tol[name], float(P[name].grad.norm()))
     off = float((x.grad.double().cpu() - X.grad).norm())
     assert off <= total, (off, total)
+
+
+def test_masses_of_shared_pages_gain_every_share():
+    """Sequences with a common prefix, or a table that names a page twice: no share is lost."""
+    from att3ntion_b200 import _cuda_kernels as ck, single_gather_decode
+    B, page = 24, 32
+    c = Made(37, [300] + [40] * (B - 1), 2, 64, page)
+    c.table[1:, :7] = c.table[0, :7]
+    c.table[3, 5] = c.table[3, 2]
+    lengths = [300, 224] + [200 + b for b in range(B - 2)]
+    Q = rand(c.g, B, 4, 64)
+    _, _, share = ref.decode(Q, c.pools, c.table, lengths)
+    pools, table, _ = c.gpu()
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    want = c.mass.double()
+    for at, v in share.items():
+        want[at] += v
+    for _ in range(5):
+        mass = c.mass.cuda()
+        single_gather_decode(Q.cuda(), pools, table, n, mass=mass)
+        # FP32 sums and exponentials of each share, and a rounding of the running value an addition (25 of them)
+        close(mass, want, 25 * 2.0 ** -24 * want + 2e-5 * (want - c.mass.double()), "mass")
+    ck.device_status()
