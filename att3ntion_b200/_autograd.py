@@ -106,6 +106,14 @@ class QuickGELU(nn.Module):
         return x * torch.sigmoid(1.702 * x)
 
 
+def _captured(device) -> bool:
+    """Whether the device's current stream is being captured into a graph."""
+    if device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class HypergraphAttention(nn.Module):
     """Three-way hypergraph attention layer on the sm_100a kernels.
 
@@ -179,7 +187,7 @@ class HypergraphAttention(nn.Module):
         for t in reversed(self._tables):
             if t.device == device and t.shape[0] >= length:
                 return t
-        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        if _captured(device):
             return rotary_table(length, self.head_dim, self.rotary_base, device)
         most = max((t.shape[0] for t in self._tables if t.device == device), default=256)
         with torch.inference_mode(False), torch.no_grad():

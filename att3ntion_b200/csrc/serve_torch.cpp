@@ -293,6 +293,7 @@ py::object norm_rotate(const Tensors& xs, const std::vector<MaybeTensor>& weight
         ws.push_back(weights[k] ? *weights[k] : Tensor());
     }
     Tensors ys;
+    const c10::cuda::CUDAGuard guard(dev);         // the capture that is asked for is one of this device's stream
     if (graph && at::GradMode::is_enabled()) {
         check_capture(tensors);
         ys = NormRotate::apply(at::TensorList(tensors), static_cast<int64_t>(xs.size()), scaled, table, positions, eps, interleaved,
