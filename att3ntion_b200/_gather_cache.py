@@ -276,7 +276,10 @@ class GatherCache:
 
     def evict(self, keep, *, sinks=0, recent=0):
         """`gather_cache_evict` in place; the pages behind the kept slots become free.  Returns the slots that stayed,
-        int32 [B,Hkv,keep]."""
+        int32 [B,Hkv,keep].
+
+        Masses come from `decode` alone: rows that were appended since have none yet, and slots that no query sees, behind
+        a window, gain none.  keep = sinks + recent = sinks + window keeps what a windowed layer sees and frees the rest."""
         if self.mass is None:
             raise RuntimeError("GatherCache.evict: the cache does not track masses (track_mass=True)")
         kept, left = gather_cache_evict(self.pools, self.mass, self.page_table, self.lengths, keep, sinks=sinks, recent=recent)

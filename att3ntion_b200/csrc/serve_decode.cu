@@ -23,7 +23,7 @@ Layout layout(int B, int Hq, int Hkv, int D, int window, int sinks, long long ma
     const long long per_key_head = mass && !o.brief ? G * block(1) : G / 8 * groups + (G & 4 ? block(4) : 0) + (G & 2 ? block(2) : 0) + (G & 1 ? block(1) : 0);
     const long long tiles = static_cast<long long>(B) * Hkv * per_key_head;
     // One step of up to 192 keys a tile in place of two, where the longest needs no more (128 sequences of 8 heads at
-    // window 128 with 4 sinks: 42 us in place of 57).  The masses' column sums are laid out for steps of 128.
+    // window 128 with 4 sinks: 45 us in place of 58).  The masses' column sums are laid out for steps of 128.
     o.wide = !mass && seen > serve::DEC_KEYS && seen <= serve::DEC_WIDE;
     o.units = tiles * (o.wide ? 1 : (seen + 127) / 128);
     o.ctas = static_cast<int>(std::max<long long>(1, std::min<long long>(att3::sm_count(), o.units)));

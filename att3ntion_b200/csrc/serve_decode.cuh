@@ -33,7 +33,7 @@
 // of a page where every slot is visible (no window, a full key step), else row gathers, four rows an instruction, for
 // which neither the page size nor where a window begins matters.  Issuing is what costs: a tile of 128 rows of 128
 // takes 4200 cycles as row gathers from one warp (62 an instruction), 1700 from three, 930 as boxes of 16 rows and 720
-// as boxes of 64; 16-byte asynchronous copies from three warps took 3000.  While one half exponentiates, the other
+// as boxes of 64; 16-byte asynchronous copies from three warps took 2060.  While one half exponentiates, the other
 // half's products run.
 //
 // Tensor memory: per half 128 columns of scores, over which P is written, then 128 of U.  Where no sequence shows more
@@ -41,10 +41,17 @@
 // which nothing is in before the step's second product, and a stage of the ring holds 192 rows.  Without that, 132 visible
 // slots take two steps, the second for four columns.
 //
-// Measured: 2 sequences of 8191 keys, 8 heads of 128: 567 us, 970 TFLOP/s of the formula's operations and 1455 of the
-// products issued, bound by the tensor pipe and the shared memory that feeds it; 16 sequences of up to 2000 keys, 8 heads
-// of 64: 125 us, the exponentials; 128 sequences with 132 visible slots, 8 heads of 128: 42 us, and one sequence with 128:
-// 10 us, the chain from row addresses to the collapse.
+// Masses (a token's share of the attention) need column sums of P too: a lane has a row, so 32 columns cost an exchange of
+// 31 shuffles, and the four warps of a half add theirs up through shared memory.  A CTA keeps the sums of a head over all
+// the tiles that it goes through, relative to the largest maximum so far; decode_mass_kernel puts them together once the
+// head's sum is known.
+//
+// Measured, calls among others, in short runs and (in brackets) in long ones, where the power cap lowers the clock: 2
+// sequences of 8191 keys, 8 heads of 128: 562 us (650), 980 TFLOP/s of the formula's operations and 1470 of the products
+// issued, bound by the tensor pipe and the shared memory that feeds it; 16 sequences of up to 2000 keys, 8 heads of 64: 120
+// us (134-160), the exponentials; 4 of up to 2500 keys with masses: 111 us (119-124), 15 us of them the join and the masses;
+// 128 sequences with 132 visible slots, 8 heads of 128: 44.7 us, and one sequence with 128: 12.2 us, the chain from row
+// addresses to the collapse.
 #pragma once
 
 #include "att3_abi_internal.h"
