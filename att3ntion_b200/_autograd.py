@@ -176,7 +176,6 @@ class HypergraphAttention(nn.Module):
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
                                       error_msgs)
 
-    @torch.compiler.disable
     def _rotary(self, length, device):
         """The angle table, at least `length` positions long, or None.  It grows by doubling, and the shorter ones are kept:
         a captured graph may still read them.  Every later caller gets what this one makes, so it is an ordinary tensor

@@ -487,3 +487,12 @@ def test_counts_of_sequences_that_sit_out():
             layer.prefill(torch.zeros(2, 4, 64), cache, counts=counts)
     with pytest.raises(ValueError, match="counts"):
         layer.prefill(torch.zeros(2, 4, 64), cache, counts=[0, 5])
+
+
+def test_import_brings_no_tracer():
+    """The package's layers import in milliseconds; torch's tracer takes seconds."""
+    import subprocess
+    import sys
+    code = "import sys, torch; before = 'torch._dynamo' in sys.modules; import att3ntion; print(before, 'torch._dynamo' in sys.modules)"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=REPO)
+    assert r.returncode == 0 and len(set(r.stdout.split())) == 1, (r.stdout, r.stderr)
