@@ -62,6 +62,14 @@ def _cuda_home() -> Path:
     return Path(_nvcc()).resolve().parent.parent
 
 
+def _has_torch() -> bool:
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return False
+    return True
+
+
 def _compile_binding(force: bool) -> Path:
     """The torch binding's object; linked against the library afterwards."""
     import sysconfig
@@ -97,16 +105,19 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [PKG.parent / "include" / "att3_b200.h"]
+    with_torch = _has_torch()
     with cf.ThreadPoolExecutor(max_workers=min(8, len(sources) + 1)) as ex:
-        binding = ex.submit(_compile_binding, force)
+        binding = ex.submit(_compile_binding, force) if with_torch else None
         objs = list(ex.map(lambda s: _compile(s, headers, force), sources))
-        binding = binding.result()
     if force or not _newer(LIB, objs):
         cmd = [_nvcc(), "-shared", "-o", str(LIB), *map(str, objs), "-Xcompiler", "-fPIC"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    _link_binding(binding, force)
+    if with_torch:                               # the library does not wait for it, nor fall with it
+        _link_binding(binding.result(), force)
+    else:
+        print(f"no torch in this Python: {BINDING.name} is not built, the C library is", file=sys.stderr)
     if verbose:
         for s in sources:
             log = OBJ / (s.stem + ".ptxas.log")

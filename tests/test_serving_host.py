@@ -496,3 +496,11 @@ def test_import_brings_no_tracer():
     code = "import sys, torch; before = 'torch._dynamo' in sys.modules; import att3ntion; print(before, 'torch._dynamo' in sys.modules)"
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=REPO)
     assert r.returncode == 0 and len(set(r.stdout.split())) == 1, (r.stdout, r.stderr)
+
+
+def test_library_builds_without_torch():
+    import subprocess
+    import sys
+    code = "import sys; sys.modules['torch'] = None; from att3ntion_b200 import build; print(build.build())"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=REPO)
+    assert r.returncode == 0 and r.stdout.strip().endswith("libatt3_b200.so") and "not built" in r.stderr, r.stderr
